@@ -53,7 +53,7 @@ class _W4Part(ctypes.Structure):
     _fields_ = [("qw", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p),
                 ("zero_bias", ctypes.c_int), ("N", ctypes.c_int64), ("out", ctypes.c_void_p)]
 
-# name -> (restype, argtypes) for every entry point of include/mcv_quant.h
+# name -> (restype, argtypes) for every entry point of include/mcv_quant.h and mcv_mixers.h
 _SIGS = {
     "mcv_last_error": (ctypes.c_char_p, []),
     "mcv_version": (ctypes.c_char_p, []),
@@ -125,6 +125,17 @@ _SIGS = {
     "mcv_argmax_f16": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp]),
     "mcv_rms_norm": (_c_int, [_vp, _vp, _c_i64, _c_i64, ctypes.c_double, _vp, _vp]),
     "mcv_rms_norm_w8a8_quantize": (_c_int, [_vp, _vp, _c_i64, _c_i64, ctypes.c_double, _vp, _vp, _vp, _vp, _vp]),
+    # include/mcv_mixers.h; a strided operand is a pointer and its strides
+    "mcv_delta_rule": (_c_int, [*[_vp, _c_i64, _c_i64] * 3, *[_vp, _c_i64] * 2, _vp, _vp, _vp, _c_i64, _vp, *[_c_i64] * 6,
+                                ctypes.c_double, _c_int, _vp, _vp, _c_i64, _vp]),
+    "mcv_delta_rule_workspace_bytes": (_c_i64, [_c_i64] * 6),
+    "mcv_paged_attention": (_c_int, [_vp, _c_i64, _c_i64, *[_vp, _c_i64, _c_i64, _c_i64] * 2, _c_i64, _c_i64,
+                                     _vp, _c_i64, _c_i64, _vp, *[_c_i64] * 5, ctypes.c_double, _vp, _vp, _c_i64, _vp]),
+    "mcv_paged_attention_workspace_bytes": (_c_i64, [_c_i64] * 5),
+    "mcv_rotary_axes": (_c_int, [*[_vp, _c_i64, _c_i64] * 3, _c_i64, _vp, _vp, *[_c_i64] * 5, *[_vp, _c_i64, _c_i64] * 2,
+                                 _vp]),
+    "mcv_rotary_axes_cached": (_c_int, [*[_vp, _c_i64, _c_i64] * 4, _c_i64, _vp, _vp, *[_c_i64] * 5, _vp, _c_i64, _c_i64,
+                                        *[_vp, _c_i64, _c_i64, _c_i64] * 2, _c_i64, _c_i64, _vp, _vp]),
 }
 
 
@@ -1132,3 +1143,7 @@ def rms_norm_w8a8_quantize(x, gamma, eps: float, normed=None, want_normed: bool 
 
 def version() -> str:
     return lib().mcv_version().decode()
+
+
+from .mixers import (gated_delta_rule, gated_delta_rule_step, paged_attention_decode, rotary_axes,  # noqa: E402,F401
+                     rotary_axes_cached, rotary_axes_table)
