@@ -24,6 +24,11 @@ def _heads(who: str, name: str, t, rows: int | None = None, heads: int | None = 
     return t.data_ptr(), s[0], s[1]
 
 
+def _workspace(nbytes: int, device, stream):
+    """gemm_workspace's buffer of the next power of two: few sizes, whatever the calls'."""
+    return gemm_workspace(1 << (nbytes - 1).bit_length(), device, stream)
+
+
 def _same_device(who: str, t, *others) -> None:
     for o in others:
         if o is not None and o.device != t.device:
@@ -65,7 +70,7 @@ def _delta(who, q, k, v, g, beta, state, cu, B, scale, normalize, state_index, o
     _same_device(who, q, k, v, g, beta, state, state_out, state_index, cu, out)
     L = lib()
     nbytes = L.mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv)
-    ws = gemm_workspace(nbytes, q.device, stream) if nbytes else None
+    ws = _workspace(nbytes, q.device, stream) if nbytes else None
     rc = L.mcv_delta_rule(*qa, *ka, *va, *gates, state.data_ptr() if state is not None else _NULL, state_out.data_ptr(),
                           state_index.data_ptr() if state_index is not None else _NULL, n_states,
                           cu.data_ptr() if cu is not None else _NULL, B, T, Hk, Hv, Dk, Dv,
@@ -158,7 +163,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale=
     _same_device(who, q, k_cache, v_cache, block_table, seq_lens, out)
     L = lib()
     nbytes = L.mcv_paged_attention_workspace_bytes(B, Hq, Hkv, D, most)
-    ws = gemm_workspace(nbytes, q.device, stream) if nbytes else None
+    ws = _workspace(nbytes, q.device, stream) if nbytes else None
     rc = L.mcv_paged_attention(*qa, *ka, *va, pages, page_size, block_table.data_ptr(), ts[0], width, seq_lens.data_ptr(),
                                most, B, Hq, Hkv, D, D ** -0.5 if scale is None else scale, out.data_ptr(),
                                ws.data_ptr() if nbytes else _NULL, nbytes, _stream(stream))
