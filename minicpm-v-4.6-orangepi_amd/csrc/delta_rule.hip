@@ -11,33 +11,12 @@
 // 16-byte column chunks over the lanes, R consecutive rows a thread (so its part of
 // q and k is one vector load).  Sums over Dk: R rows in the thread, the row groups
 // of a wave by lane swaps, the four waves through LDS.
-#include <cstdio>
-
-#include "mixers.h"
+#include "delta_rule.h"
 
 namespace mcv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kNormEps = 1e-6f;
-
-struct DeltaArgs {
-    const uint16_t* q;
-    const uint16_t* k;
-    const uint16_t* v;
-    const float* g;
-    const float* beta;
-    const float* state;
-    float* state_out;
-    const int32_t* state_index;
-    const int32_t* cu;
-    uint16_t* out;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, beta_row, n_states;
-    int T, per_seq, Hv, group, Dv;
-    float scale;
-    int normalize;
-};
-
 template <int DK, int DVW>
 __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) {
     constexpr int C4 = DVW / 4;                  // lanes over one row's columns
@@ -50,9 +29,8 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
     const int slice = blockIdx.x % slices;
     const int bh = blockIdx.x / slices;
     const int h = bh % p.Hv, b = bh / p.Hv, hk = h / p.group;
-    int t0 = p.cu ? p.cu[b] : b * p.per_seq, t1 = p.cu ? p.cu[b + 1] : t0 + p.per_seq;
-    t0 = t0 < 0 ? 0 : t0;
-    t1 = t1 > p.T ? p.T : t1;
+    int t0, t1;
+    delta_span(p, b, t0, t1);
     const int col = slice * DVW + 4 * c4;
     const int64_t at = p.state_index ? p.state_index[b] : b;
     if (at < 0 || at >= p.n_states) {
@@ -116,8 +94,8 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
             kk += dots[buf][w][1];
             qq += dots[buf][w][2];
         }
-        const float rk = p.normalize ? 1.0f / sqrtf(kk + kNormEps) : 1.0f;
-        const float rq = p.normalize ? 1.0f / sqrtf(qq + kNormEps) : 1.0f;
+        const float rk = p.normalize ? 1.0f / sqrtf(kk + kDeltaEps) : 1.0f;
+        const float rq = p.normalize ? 1.0f / sqrtf(qq + kDeltaEps) : 1.0f;
         const float vs[4] = {h2f(vw.x & 0xffff), h2f(vw.x >> 16), h2f(vw.y & 0xffff), h2f(vw.y >> 16)};
         float4_t u;
 #pragma unroll
@@ -139,6 +117,8 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
         *reinterpret_cast<float4_t*>(p.state_out + base + static_cast<int64_t>(j) * p.Dv) = S[j];
 }
 
+bool long_enough(int64_t B, int64_t T) { return T >= 16 * B; }
+
 }  // namespace
 }  // namespace mcv
 
@@ -147,8 +127,8 @@ using namespace mcv;
 extern "C" {
 
 int64_t mcv_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv) {
-    (void)B, (void)T, (void)Hk, (void)Hv, (void)Dk, (void)Dv;
-    return 0;
+    if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || (Dk != 64 && Dk != 128) || Dv <= 0 || Dv % 16 != 0 || !long_enough(B, T)) return 0;
+    return delta_chunk_workspace(B, T, Hk, Hv, Dk, Dv);
 }
 
 int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
@@ -180,9 +160,15 @@ int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, 
                 static_cast<const float*>(g), static_cast<const float*>(beta), static_cast<const float*>(state),
                 static_cast<float*>(state_out), static_cast<const int32_t*>(state_index),
                 static_cast<const int32_t*>(cu_seqlens), static_cast<uint16_t*>(out), q_row, q_head, k_row, k_head,
-                v_row, v_head, g_row, beta_row, n_states, static_cast<int>(T),
+                v_row, v_head, g_row, beta_row, n_states, static_cast<int>(T), static_cast<int>(B),
                 static_cast<int>(cu_seqlens ? 0 : T / B), static_cast<int>(Hv), static_cast<int>(Hv / Hk),
                 static_cast<int>(Dv), static_cast<float>(scale), normalize};
+    if (long_enough(B, T) && workspace && workspace_bytes >= delta_chunk_workspace(B, T, Hk, Hv, Dk, Dv)) {
+        if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+            return fail(MCV_ERR_INVALID_ARG, "delta_rule: workspace must be 256-byte aligned");
+        return launch_delta_chunk(a, static_cast<int>(Hk), static_cast<int>(Dk), workspace, workspace_bytes,
+                                  static_cast<hipStream_t>(stream));
+    }
     const int64_t grid = B * Hv * (Dv / 16);
     if (grid > 0x7fffffff) return fail(MCV_ERR_SHAPE, "delta_rule: too many states");
     hipLaunchKernelGGL((Dk == 64 ? delta_recurrent_kernel<64, 16> : delta_recurrent_kernel<128, 16>),

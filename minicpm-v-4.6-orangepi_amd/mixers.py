@@ -9,7 +9,7 @@ of one head are contiguous.
 """
 from __future__ import annotations
 
-from . import McvError, _check, _stream, _torch, gemm_workspace, lib
+from . import _GEMM_COUNTER_BYTES, McvError, _check, _stream, _torch, gemm_workspace, lib
 
 _NULL = 0
 
@@ -25,7 +25,8 @@ def _heads(who: str, name: str, t, rows: int | None = None, heads: int | None = 
 
 
 def _workspace(nbytes: int, device, stream):
-    """gemm_workspace's buffer of the next power of two: few sizes, whatever the calls'."""
+    """gemm_workspace's buffer of the next power of two: few sizes, whatever the calls'.  Other calls
+    on the stream use it too, so its first _GEMM_COUNTER_BYTES are counters and stay zero."""
     return gemm_workspace(1 << (nbytes - 1).bit_length(), device, stream)
 
 
@@ -70,12 +71,12 @@ def _delta(who, q, k, v, g, beta, state, cu, B, scale, normalize, state_index, o
     _same_device(who, q, k, v, g, beta, state, state_out, state_index, cu, out)
     L = lib()
     nbytes = L.mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv)
-    ws = _workspace(nbytes, q.device, stream) if nbytes else None
+    ws = _workspace(_GEMM_COUNTER_BYTES + nbytes, q.device, stream) if nbytes else None      # behind the counters
     rc = L.mcv_delta_rule(*qa, *ka, *va, *gates, state.data_ptr() if state is not None else _NULL, state_out.data_ptr(),
                           state_index.data_ptr() if state_index is not None else _NULL, n_states,
                           cu.data_ptr() if cu is not None else _NULL, B, T, Hk, Hv, Dk, Dv,
                           Dk ** -0.5 if scale is None else scale, 1 if normalize else 0, out.data_ptr(),
-                          ws.data_ptr() if nbytes else _NULL, nbytes, _stream(stream))
+                          ws.data_ptr() + _GEMM_COUNTER_BYTES if nbytes else _NULL, nbytes, _stream(stream))
     if rc:
         _check(rc, who)
     return out, state_out

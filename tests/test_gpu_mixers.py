@@ -476,3 +476,19 @@ def test_mixers_in_a_graph(mcv, cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all((x == y).all() for x, y in zip(got, want)), turn
+
+
+def test_mixers_share_a_workspace_with_the_gemm(mcv, cuda):
+    """On one stream all of them use one buffer, whose counters each leaves zero."""
+    torch = _torch()
+    c = [x.to(cuda) for x in _delta_case(1, [500], 1, 1, 64, 64)]
+    a = [x.to(cuda) for x in _attn_case(1, [900, 3], 8, 2, 64, 16)[:5]]
+    w = mcv.W4A16QuantizedWeight.from_awq(*mcv.quantize_int4(torch.randn(3584, 1024, generator=_gen(1)).half().view(torch.int16).numpy()))
+    x = torch.randn(70, 3584, generator=_gen(2)).half().to(cuda)
+    first = None
+    for _ in range(3):
+        got = (mcv.matmul_w4a16(x, w), *mcv.gated_delta_rule(*c, normalize=True), mcv.paged_attention_decode(*a))
+        first = first or [t.clone() for t in got]
+        assert all((t == u).all() for t, u in zip(got, first))
+    for ws in mcv._GEMM_WS.values():
+        assert (ws[:4096] == 0).all()
