@@ -33,7 +33,7 @@ __device__ __forceinline__ void delta_span(const DeltaArgs& p, int b, int& t0, i
 }
 
 // The chunked form (delta_chunk.hip).
-int64_t delta_chunk_workspace(int64_t B, int64_t T, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv);
+int64_t delta_chunk_workspace(int64_t B, int64_t T, int64_t Hk, int64_t Hv, int64_t Dk);
 int launch_delta_chunk(const DeltaArgs& a, int Hk, int Dk, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 }  // namespace mcv

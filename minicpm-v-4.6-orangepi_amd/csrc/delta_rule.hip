@@ -128,7 +128,7 @@ extern "C" {
 
 int64_t mcv_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv) {
     if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || (Dk != 64 && Dk != 128) || Dv <= 0 || Dv % 16 != 0 || !long_enough(B, T)) return 0;
-    return delta_chunk_workspace(B, T, Hk, Hv, Dk, Dv);
+    return delta_chunk_workspace(B, T, Hk, Hv, Dk);
 }
 
 int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
@@ -163,7 +163,7 @@ int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, 
                 v_row, v_head, g_row, beta_row, n_states, static_cast<int>(T), static_cast<int>(B),
                 static_cast<int>(cu_seqlens ? 0 : T / B), static_cast<int>(Hv), static_cast<int>(Hv / Hk),
                 static_cast<int>(Dv), static_cast<float>(scale), normalize};
-    if (long_enough(B, T) && workspace && workspace_bytes >= delta_chunk_workspace(B, T, Hk, Hv, Dk, Dv)) {
+    if (long_enough(B, T) && workspace && workspace_bytes >= delta_chunk_workspace(B, T, Hk, Hv, Dk)) {
         if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
             return fail(MCV_ERR_INVALID_ARG, "delta_rule: workspace must be 256-byte aligned");
         return launch_delta_chunk(a, static_cast<int>(Hk), static_cast<int>(Dk), workspace, workspace_bytes,
