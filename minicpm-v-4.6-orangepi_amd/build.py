@@ -3,6 +3,7 @@
 Outputs (all git-ignored, all shipped to the GPU box with the source tree):
   lib/libmcv_quant.so     C-ABI (include/mcv_quant.h): HIP kernels + host packers
   lib/libminicpmv_ops.so  C++ operator surface (namespace minicpmv) over the C-ABI
+  lib/_mcv_mixers.so      the token mixers' Python calls, native, over the C-ABI
   tests/cpp/bin/*         C++ test programs mirroring the reference's tests
 
 Every call recompiles everything (objects go to _build/); compiles run in
@@ -100,6 +101,25 @@ def build_cpp_layer(jobs: int | None = None) -> Path:
     return out
 
 
+def build_binding() -> Path:
+    """Compile binding/mixers_ext.cpp into lib/_mcv_mixers.so (links torch and the C-ABI)."""
+    import sysconfig
+
+    import torch
+
+    tdir = Path(torch.__file__).resolve().parent
+    out = LIB / "_mcv_mixers.so"
+    tmp = LIB / "_mcv_mixers.so.tmp"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
+          "-isystem", str(tdir / "include"), "-isystem", str(tdir / "include/torch/csrc/api/include"),
+          "-isystem", sysconfig.get_paths()["include"], "-isystem", "/opt/rocm/include",
+          str(PKG / "binding" / "mixers_ext.cpp"), "-o", str(tmp), f"-L{tdir / 'lib'}", "-ltorch_python", "-ltorch_cpu",
+          "-lc10", "-lc10_hip", f"-L{LIB}", "-lmcv_quant", "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, out)
+    return out
+
+
 def build_cpp_tests(jobs: int | None = None) -> list[Path]:
     """Compile tests/cpp/*.cpp into tests/cpp/bin/ against the C++ layer.  The
     test programs also link the CPU oracle (oracle/build/libmcv_oracle.so, test
@@ -129,6 +149,7 @@ def build_cpp_tests(jobs: int | None = None) -> list[Path]:
 def build_all() -> None:
     build_capi()
     build_cpp_layer()
+    build_binding()
     build_cpp_tests()
 
 
