@@ -5,29 +5,32 @@
 // heads of one cache head share every byte of K and V (and are one side of the matrix
 // products, however few they are: the matrix cores have time to spare here).
 //
-// A wave takes 32 tokens at a time, straight from memory into registers, no LDS:
+// A wave takes 32 tokens at a time:
 //   S^T = K Q^T   v_mfma_f32_16x16x32_f16, twice 16 tokens as rows; lane (c, j), c =
 //                 lane % 16, j = lane / 16, then holds head c and tokens 4j .. 4j + 3 of each half
 //   O^T += V^T P^T  the sum over tokens may run in any order, so lane (c, j)'s eight
 //                 weights are the product's operand as they stand, and the lane loads V's
 //                 same eight rows, 8 d of each, whose 8 x 8 values it turns in registers
+// K as an operand has its 16 rows on 16 neighbouring lanes, and a load costs a cycle a
+// line touched: K comes as whole rows instead and turns through LDS, each wave its own.
 // What lies past the sequence's end, or in a page that is not there, has score -inf and
 // its V is set to zero (it may hold NaN).
 //
-// A unit is `unit` tokens of one (sequence, cache head), shared by the four waves of a
-// workgroup tile by tile.  Units of one sequence meet through the workspace: each
-// writes its 32-bit part with device-scope stores (written through; see
-// w4a16_gemm_sk.hip) and counts itself in; the last of each kFan units joins them in
-// order, and where there are more than kFan the last of those joins the joined, so
-// the bits do not depend on who is last and nobody waits.
+// Only the device knows the lengths: every workgroup adds them up, and each (sequence, cache
+// head) is cut into parts of one size, about the work over the workgroups that the chip
+// holds, so that none waits for the longest sequence.  Parts of one (sequence, cache head)
+// meet through the workspace: each writes its 32-bit part with device-scope stores
+// (written through; see w4a16_gemm_sk.hip) and counts itself in; the last of each kFan
+// parts joins them in order, and where there are more than kFan the last of those joins
+// the joined, so the bits do not depend on who is last and nobody waits.
+#include <algorithm>
+
 #include "mixers.h"
 
 namespace mcv {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kTile = 32;                        // tokens a wave takes at a time
-constexpr int kStep = kWaves * kTile;            // units are whole multiples of this
 constexpr int kHeads = 16;                       // query heads of one matrix product
 constexpr int kFan = 16;                         // parts joined by one workgroup
 constexpr int64_t kCounterBytes = 4096;
@@ -43,14 +46,25 @@ struct AttnArgs {
     uint16_t* out;
     uint8_t* ws;
     int64_t q_row, q_head, k_page, k_head, v_page, v_head, table_row;
-    int k_token, v_token, pages, page16, max_len, Hq, Hkv, group, htiles, unit, max_units;
+    int k_token, v_token, pages, page16, max_len, B, Hq, Hkv, group, htiles;
     uint32_t page16_inv;                         // ceil(2^32 / page16), page16 > 1
     float scale_log2;
+    int split;                                   // workgroups to cut for; 0: every (sequence, cache head) whole
 };
 
 // Bytes of one part: [rows][D] sums, [rows][2] maximum and sum, whole 16-byte chunks.
 __host__ __device__ constexpr int64_t part_bytes(int rows, int D) { return int64_t(rows) * D * 4 + ((rows * 8 + 15) & ~15); }
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);       // rows of 16: one to the right, two, four, eight
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);       // a row's last lane to the next row
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);       // lane 31 to the upper half
+    return v;
+}
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max4(float v) {          // over the four lanes of one column
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -65,49 +79,6 @@ __device__ __forceinline__ float sum4(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Weights of two parts with maxima m and n against their common one (-inf: a part of nothing).
-__device__ __forceinline__ void join_weights(float m, float n, float& top, float& wm, float& wn) {
-    top = fmaxf(m, n);
-    wm = m == -INFINITY ? 0.f : exp2_of(m - top);
-    wn = n == -INFINITY ? 0.f : exp2_of(n - top);
-}
-
-// Joins parts 0 .. n - 1 at byte `from` of the workspace, in order.  Thread i has the
-// float4s i, i + 256, ... of [rows][D]; `put` takes (float4 number, sum, m, l).
-template <int D, class Put>
-__device__ __forceinline__ void join_parts(const AttnArgs& p, int64_t from, int n, int rows, Put put) {
-    const int64_t bytes = part_bytes(rows, D);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(p.ws + from, 0, static_cast<int>(n * bytes), 0x00020000);
-    for (int i = threadIdx.x; i < rows * D / 4; i += 64 * kWaves) {
-        const int row = i / (D / 4);
-        float4_t sum = {0, 0, 0, 0};
-        float m = -INFINITY, l = 0.f;
-        constexpr int kBatch = 8;                // loads of a batch go out together
-        for (int u0 = 0; u0 < n; u0 += kBatch) {
-            int4_t o[kBatch];
-            uint2 st[kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int at = static_cast<int>((u0 + u < n ? u0 + u : n - 1) * bytes);
-                o[u] = __builtin_amdgcn_raw_buffer_load_b128(r, at + i * 16, 0, 16);
-                const auto s = __builtin_amdgcn_raw_buffer_load_b64(r, at + rows * D * 4 + row * 8, 0, 16);
-                st[u] = make_uint2(s[0], s[1]);
-            }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                if (u0 + u >= n) break;
-                float top, a, b;
-                join_weights(m, __uint_as_float(st[u].x), top, a, b);
-                m = top;
-                l = l * a + __uint_as_float(st[u].y) * b;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) sum[x] = sum[x] * a + __int_as_float(o[u][x]) * b;
-            }
-        }
-        put(i, sum, m, l);
-    }
-}
-
 template <int D>
 __device__ __forceinline__ void put_out(const AttnArgs& p, int64_t head0, int i, float4_t sum, float l) {
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);          // a row of nothing: zeros; NaN stays
@@ -117,6 +88,11 @@ __device__ __forceinline__ void put_out(const AttnArgs& p, int64_t head0, int i,
     *reinterpret_cast<uint2*>(p.out + head0 * D + i * 4) =
         make_uint2(r[0] | (static_cast<uint32_t>(r[1]) << 16), r[2] | (static_cast<uint32_t>(r[3]) << 16));
 }
+
+// What no kernel in flight writes, at an address that a whole wave shares: read through the scalar cache, whose
+// loads have a counter of their own (a wait for a page number must not be one for all the K and V in flight).
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ __forceinline__ scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)reinterpret_cast<uintptr_t>(p); }
 
 // Counts this workgroup in; true in every thread of the one that is the last of n.
 __device__ __forceinline__ bool last_in(unsigned* counter, int n, int* flag) {
@@ -132,48 +108,74 @@ __device__ __forceinline__ bool last_in(unsigned* counter, int n, int* flag) {
     return *flag != 0;
 }
 
-template <int D>
-__device__ __forceinline__ void put_part(const AttnArgs& p, int64_t at, int rows, int i, float4_t sum, float m, float l) {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(p.ws + at, 0, static_cast<int>(part_bytes(rows, D)), 0x00020000);
-    const int4_t v = {__float_as_int(sum[0]), __float_as_int(sum[1]), __float_as_int(sum[2]), __float_as_int(sum[3])};
-    __builtin_amdgcn_raw_buffer_store_b128(v, r, i * 16, 0, 16);
-    if (i % (D / 4) == 0) {
-        typedef unsigned u2 __attribute__((ext_vector_type(2)));
-        __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(m), __float_as_uint(l)}, r, rows * D * 4 + i / (D / 4) * 8, 0, 16);
-    }
-}
-
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArgs p) {
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) {
     constexpr int KS = D / 32;                   // steps of the score product
+    constexpr int RC = D / 8;                    // 16-byte chunks of a row
     constexpr int VW = D / 16;                   // d of V a lane loads of one token
     constexpr int VC = VW < 8 ? VW : 8;          // ... in chunks of this many
     constexpr int VN = VW / VC;
     typedef uint32_t vchunk __attribute__((ext_vector_type(VC / 2)));
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];        // K [wave][32][D + 8]; then the waves' parts [wave][head][D]
+    __shared__ float2 stat[W][kHeads];
+    __shared__ int flag;
     const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int bh = blockIdx.x;
-    const int ht = bh % p.htiles, hk = bh / p.htiles % p.Hkv, b = bh / p.htiles / p.Hkv;
+    const int per_seq = p.Hkv * p.htiles;
+    auto length = [&](int b) {
+        const int n = b < p.B ? p.lens[b] : 0;
+        return n < 0 ? 0 : n > p.max_len ? p.max_len : n;
+    };
+    auto tiles_of = [&](int b, int len) { return b >= p.B ? 0 : len <= kTile ? 1 : (len + kTile - 1) / kTile; };   // none: one, its zeros
+
+    // Tiles of a part, and this workgroup's sequence b, whose first part has number w_first and whose first tile b_first.
+    int per = 0x3fffffff, b = 0, len = 0, b_first = 0, w_first = 0;
+    {
+        int mine = length(lane);                 // of the first 64 sequences
+        if (p.split) {
+            int total = 0;
+            for (int b0 = 0; b0 < p.B; b0 += 64)
+                total += __builtin_amdgcn_readlane(wave_scan(tiles_of(b0 + lane, b0 ? length(b0 + lane) : mine)), 63);
+            per = (total * per_seq + p.split - 1) / p.split;
+            per = (per + W - 1) / W * W;
+        }
+        for (int b0 = 0;; b0 += 64) {
+            if (b0 >= p.B) return;
+            if (b0) mine = length(b0 + lane);
+            const int tiles = tiles_of(b0 + lane, mine), parts = (tiles + per - 1) / per;
+            const int upto = wave_scan(parts * per_seq), tiles_upto = wave_scan(tiles * per_seq);
+            const unsigned long long past = __ballot(w_first + upto > static_cast<int>(blockIdx.x));
+            const int at = past ? __builtin_ctzll(past) : 64;    // the first lane past it
+            b = b0 + at;
+            if (past) len = __builtin_amdgcn_readlane(mine, at);
+            if (at) {
+                w_first += __builtin_amdgcn_readlane(upto, at - 1);
+                b_first += __builtin_amdgcn_readlane(tiles_upto, at - 1);
+            }
+            if (past) break;
+        }
+    }
+    per = __builtin_amdgcn_readfirstlane(per);
+    const int tiles = len <= kTile ? 1 : (len + kTile - 1) / kTile, parts = (tiles + per - 1) / per;
+    const int in_seq = (static_cast<int>(blockIdx.x) - w_first) / parts, part = static_cast<int>(blockIdx.x) - w_first - in_seq * parts;
+    const int s0 = part * per, hk = in_seq / p.htiles, ht = in_seq - hk * p.htiles;
     const int rows = p.group - ht * kHeads < kHeads ? p.group - ht * kHeads : kHeads;
     const int64_t head0 = static_cast<int64_t>(b) * p.Hq + hk * p.group + ht * kHeads;
-    int len = p.lens[b];
-    len = len < 0 ? 0 : len > p.max_len ? p.max_len : len;
-    const int unit = blockIdx.y, units = len == 0 ? 1 : (len - 1) / p.unit + 1;
-    if (unit >= units) return;
-    const int t1 = len - unit * p.unit < p.unit ? len : (unit + 1) * p.unit;
+    const int t1 = part < parts - 1 ? (s0 + per) * kTile : len;
 
-    half8_t q[KS];
+    constexpr int RS = RC + 1;                   // chunks from row to row: 16 rows' same chunk are in 16 places of the banks
+    half8_t* const kl = reinterpret_cast<half8_t*>(lds) + wave * kTile * RS;
+    half8_t *const k_in = kl + lane / RC * RS + lane % RC, *const k_out = kl + c * RS + j;
+    const int koff = 2 * (lane / RC * p.k_token + lane % RC * 8), voff = 2 * (4 * j * p.v_token + VC * c);
+
+    half8_t q[KS];                           // lanes past the last head: the first again, never stored
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (c < rows)
-            w = *reinterpret_cast<const uint4*>(p.q + b * p.q_row + static_cast<int64_t>(hk * p.group + ht * kHeads + c) * p.q_head + 32 * s + 8 * j);
-        q[s] = __builtin_bit_cast(half8_t, w);
-    }
-    const int32_t* __restrict__ table = p.table + b * p.table_row;
+    for (int s = 0; s < KS; ++s)
+        q[s] = *reinterpret_cast<const half8_t*>(p.q + b * p.q_row + static_cast<int64_t>(hk * p.group + ht * kHeads + (c < rows ? c : 0)) * p.q_head +
+                                                 32 * s + 8 * j);
+    const scalar_ints table = as_scalar(p.table + b * p.table_row);
     const uint16_t* kh = p.k + hk * p.k_head;
     const uint16_t* vh = p.v + hk * p.v_head;
-    const int koff = c * p.k_token + 8 * j, voff = 4 * j * p.v_token + VC * c;
 
     // Rows of 16 tokens from t on: their page's number (-1: not there, or past the end) and first row in it.
     auto place = [&](int t, int& page, int& row) {
@@ -187,189 +189,248 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
             row = 16 * r;
         }
         page = t < t1 ? table[at] : -1;
-        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.pages)) page = -1;
+        page = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages) ? page : -1);
     };
-    half8_t kf[2][KS];
+    // Loads are unconditional, of no bytes where there is no page, so that a wait counts those in flight exactly.
+    auto rows16 = [](const uint16_t* base, int page, int row, int64_t page_stride, int token_stride) {
+        const uint16_t* at = base + (page < 0 ? 0 : page) * page_stride + static_cast<int64_t>(row) * token_stride;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, page < 0 ? 0 : 2 * (15 * token_stride + D), 0x00020000);
+    };
+    int4_t kr[2][KS];
     vchunk vr[8][VN];
     auto load_k = [&](const int (&page)[2], const int (&row)[2]) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const uint16_t* at = kh + (page[x] < 0 ? 0 : page[x]) * p.k_page + static_cast<int64_t>(row[x]) * p.k_token;
+            const __amdgpu_buffer_rsrc_t r = rows16(kh, page[x], row[x], p.k_page, p.k_token);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kf[x][s] = *reinterpret_cast<const half8_t*>(at + koff + 32 * s);
+            for (int i = 0; i < KS; ++i) kr[x][i] = __builtin_amdgcn_raw_buffer_load_b128(r, koff, 2 * i * (64 / RC) * p.k_token, 0);
         }
     };
     auto load_v = [&](const int (&page)[2], const int (&row)[2]) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const uint16_t* at = vh + (page[x] < 0 ? 0 : page[x]) * p.v_page + static_cast<int64_t>(row[x]) * p.v_token;
+            const __amdgpu_buffer_rsrc_t r = rows16(vh, page[x], row[x], p.v_page, p.v_token);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int n = 0; n < VN; ++n)
-                    vr[4 * x + i][n] = *reinterpret_cast<const vchunk*>(at + static_cast<int64_t>(i) * p.v_token + voff + 128 * n);
+                for (int n = 0; n < VN; ++n) {
+                    if constexpr (VC == 8)
+                        vr[4 * x + i][n] = __builtin_bit_cast(vchunk, __builtin_amdgcn_raw_buffer_load_b128(r, voff + 256 * n, 2 * i * p.v_token, 0));
+                    else
+                        vr[4 * x + i][n] = __builtin_bit_cast(vchunk, __builtin_amdgcn_raw_buffer_load_b64(r, voff, 2 * i * p.v_token, 0));
+                }
         }
     };
 
     float4_t acc[VN][VC] = {};
     float m = -INFINITY, l = 0.f;
-    int t = unit * p.unit + wave * kTile;
-    int page[2], row[2];
-    if (t < t1) {
-        place(t, page[0], row[0]);
-        place(t + 16, page[1], row[1]);
-        load_k(page, row);
-        load_v(page, row);
-    }
-    while (t < t1) {
-        const int tn = t + kStep;
-        int npage[2] = {-1, -1}, nrow[2] = {0, 0};
-        if (tn < t1) {
-            place(tn, npage[0], nrow[0]);
-            place(tn + 16, npage[1], nrow[1]);
-        }
+    int t = (s0 + wave - W) * kTile;         // the tile in the registers: none yet
+    int page[2] = {-1, -1};
+    bool have = false;
+    do {
+        const int tn = t + W * kTile;
+        int npage[2], nrow[2];
+        place(tn, npage[0], nrow[0]);
+        place(tn + 16, npage[1], nrow[1]);
         float4_t s[2] = {};
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int i = 0; i < KS; ++i) s[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x][i], q[i], s[x], 0, 0, 0);
-        if (tn < t1) load_k(npage, nrow);
-        const bool whole = t + kTile <= t1 && page[0] >= 0 && page[1] >= 0;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v = s[x][r] * p.scale_log2;
-                if (!whole && (page[x] < 0 || t + 16 * x + 4 * j + r >= t1)) v = -INFINITY;
-                s[x][r] = v;
-                mx = fmaxf(mx, v);
-            }
-        mx = fmaxf(max4(mx), m);
-        if (__any(mx > m)) {
-            const float keep = m == -INFINITY ? 0.f : exp2_of(m - mx);
-            l *= keep;
-#pragma unroll
-            for (int n = 0; n < VN; ++n)
-#pragma unroll
-                for (int i = 0; i < VC; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[n][i][r] *= keep;
-            m = mx;
-        }
-        const float base = m == -INFINITY ? 0.f : m;         // nothing so far: every weight 2^-inf
-        half8_t w;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = exp2_of(s[x][r] - base);
-                l += e;
-                w[4 * x + r] = static_cast<_Float16>(e);     // the product's operand: one rounding of each weight
-            }
-        if (!whole)
+        if (have) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (page[x] < 0 || t + 16 * x + 4 * j + i >= t1)
+                for (int i = 0; i < KS; ++i)
+                    k_in[(16 * x + i * (64 / RC)) * RS] = __builtin_bit_cast(half8_t, kr[x][i]);
+        }
+        load_k(npage, nrow);
+        if (have) {
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                        for (int n = 0; n < VN; ++n) vr[4 * x + i][n] = vchunk(0);
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                    s[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_out[16 * x * RS + 4 * i], q[i], s[x], 0, 0, 0);
+            __builtin_amdgcn_wave_barrier();
+            const bool whole = t + kTile <= t1 && page[0] >= 0 && page[1] >= 0;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = s[x][r] * p.scale_log2;
+                    if (!whole && (page[x] < 0 || t + 16 * x + 4 * j + r >= t1)) v = -INFINITY;
+                    s[x][r] = v;
+                    mx = fmaxf(mx, v);
+                }
+            mx = fmaxf(max4(mx), m);
+            if (__any(mx > m)) {
+                const float keep = m == -INFINITY ? 0.f : exp2_of(m - mx);
+                l *= keep;
+#pragma unroll
+                for (int n = 0; n < VN; ++n)
+#pragma unroll
+                    for (int i = 0; i < VC; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[n][i][r] *= keep;
+                m = mx;
+            }
+            const float base = m == -INFINITY ? 0.f : m;         // nothing so far: every weight 2^-inf
+            half8_t w;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = exp2_of(s[x][r] - base);
+                    l += e;
+                    w[4 * x + r] = static_cast<_Float16>(e);     // the product's operand: one rounding of each weight
+                }
+            if (!whole)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (page[x] < 0 || t + 16 * x + 4 * j + i >= t1)
+#pragma unroll
+                            for (int n = 0; n < VN; ++n) vr[4 * x + i][n] = vchunk(0);
+#pragma unroll
+            for (int n = 0; n < VN; ++n)
+#pragma unroll
+                for (int d = 0; d < VC; ++d) {
+                    const uint32_t pick = d & 1 ? 0x07060302u : 0x05040100u;
+                    uint4 a;
+                    a.x = __builtin_amdgcn_perm(vr[1][n][d / 2], vr[0][n][d / 2], pick);
+                    a.y = __builtin_amdgcn_perm(vr[3][n][d / 2], vr[2][n][d / 2], pick);
+                    a.z = __builtin_amdgcn_perm(vr[5][n][d / 2], vr[4][n][d / 2], pick);
+                    a.w = __builtin_amdgcn_perm(vr[7][n][d / 2], vr[6][n][d / 2], pick);
+                    acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w, acc[n][d], 0, 0, 0);
+                }
+        }
+        load_v(npage, nrow);
+        t = tn;
+        have = true;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) page[x] = npage[x];
+    } while (t < t1);
+    l = sum4(l);
+
+    // The waves' parts meet in LDS.
+    const int slot = static_cast<int>(part_bytes(p.group < kHeads ? p.group : kHeads, D));     // sized for the widest head tile
+    // Part i has the id w0 + i, w0 the part of an even cut of all tiles that the first tile falls into.  A part 0
+    // has slot 2 id + 1, others 2 id: ids of one (sequence, cache head) are its own but for its last,
+    // which may be the next one's first.
+    const int w0 = (b_first + in_seq * tiles) / per;
+    const int slots0 = static_cast<int>(kCounterBytes);
+    auto part_at = [&](int i) { return slots0 + (i == 0 ? 2 * w0 + 1 : 2 * (w0 + i)) * slot; };
+    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(p.ws, 0, 0x7fffffff, 0x00020000);
+    auto put = [&](int at, int i, float4_t sum, float m2, float l2) {
+        if (at < 0) {
+            put_out<D>(p, head0, i, sum, l2);
+            return;
+        }
+        const int4_t v = {__float_as_int(sum[0]), __float_as_int(sum[1]), __float_as_int(sum[2]), __float_as_int(sum[3])};
+        __builtin_amdgcn_raw_buffer_store_b128(v, ws, at + i * 16, 0, 16);
+        if (i % (D / 4) == 0) {
+            typedef unsigned u2 __attribute__((ext_vector_type(2)));
+            __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(m2), __float_as_uint(l2)}, ws, at + rows * D * 4 + i / (D / 4) * 8, 0, 16);
+        }
+    };
+    int tid = threadIdx.x;                   // (opaque: addresses made from it would be kept through the loop above)
+    asm volatile("" : "+v"(tid));
+    const int tc = tid & 15, tj = (tid & 63) >> 4;
+    float* const meet = reinterpret_cast<float*>(lds);
+    __syncthreads();                         // K has been read
+    if (tc < rows) {
+        if (tj == 0) stat[wave][tc] = make_float2(m, l);
 #pragma unroll
         for (int n = 0; n < VN; ++n)
 #pragma unroll
-            for (int d = 0; d < VC; ++d) {
-                const uint32_t pick = d & 1 ? 0x07060302u : 0x05040100u;
-                uint4 a;
-                a.x = __builtin_amdgcn_perm(vr[1][n][d / 2], vr[0][n][d / 2], pick);
-                a.y = __builtin_amdgcn_perm(vr[3][n][d / 2], vr[2][n][d / 2], pick);
-                a.z = __builtin_amdgcn_perm(vr[5][n][d / 2], vr[4][n][d / 2], pick);
-                a.w = __builtin_amdgcn_perm(vr[7][n][d / 2], vr[6][n][d / 2], pick);
-                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w, acc[n][d], 0, 0, 0);
-            }
-        if (tn < t1) load_v(npage, nrow);
-        t = tn;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) page[x] = npage[x], row[x] = nrow[x];
-    }
-    l = sum4(l);
-
-    // The waves' parts meet in LDS, up to 128 d at a time: [wave][head][DL].
-    constexpr int DL = D < 128 ? D : 128;
-    extern __shared__ float lds[];
-    __shared__ float2 stat[kWaves][kHeads];
-    __shared__ int flag;
-    if (c < rows && j == 0) stat[wave][c] = make_float2(m, l);
-    const int64_t bytes = part_bytes(rows, D);
-    // this (sequence, cache head, head tile)'s parts: sized for the widest tile
-    const int64_t all = part_bytes(p.group < kHeads ? p.group : kHeads, D);
-    const int fans = (p.max_units + kFan - 1) / kFan;
-    const int64_t mine = kCounterBytes + bh * p.max_units * all;
-#pragma unroll
-    for (int n = 0; n < VN; ++n) {
-        if (n) __syncthreads();
-        if (c < rows)
-#pragma unroll
             for (int r = 0; r < 4; ++r) {
                 // acc[n][i][r]: d = 128 n + VC (4 j + r) + i
-                float* at = lds + (wave * rows + c) * DL + VC * (4 * j + r);
+                float* at = meet + (wave * rows + tc) * D + 128 * n + VC * (4 * tj + r);
 #pragma unroll
                 for (int i = 0; i < VC; i += 4)
                     *reinterpret_cast<float4_t*>(at + i) = float4_t{acc[n][i][r], acc[n][i + 1][r], acc[n][i + 2][r], acc[n][i + 3][r]};
             }
-        __syncthreads();
-        for (int e = threadIdx.x; e < rows * DL / 4; e += 64 * kWaves) {
-            const int h = e / (DL / 4);
-            float4_t sum = {0, 0, 0, 0};
-            float top = -INFINITY, tot = 0.f;
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * D / 4; i += 64 * W) {
+        const int h = i / (D / 4);
+        float4_t sum = {0, 0, 0, 0};
+        float top = -INFINITY, tot = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float4_t o = *reinterpret_cast<const float4_t*>(lds + w * rows * DL + e * 4);
-                const float2 st = stat[w][h];
-                float wa, wb, nt;
-                join_weights(top, st.x, nt, wa, wb);
-                top = nt;
-                tot = tot * wa + st.y * wb;
+        for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w][h].x);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) sum[x] = sum[x] * wa + o[x] * wb;
+        for (int w = 0; w < W; ++w) {
+            const float2 st = stat[w][h];
+            const float by = st.x == -INFINITY ? 0.f : exp2_of(st.x - top);
+            const float4_t o = *reinterpret_cast<const float4_t*>(meet + w * rows * D + i * 4);
+            tot = fmaf(st.y, by, tot);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sum[x] = fmaf(o[x], by, sum[x]);
+        }
+        put(parts == 1 ? -1 : part_at(part), i, sum, top, tot);
+    }
+    if (parts > 1) {
+        // Counters: one by w0 (of those cut, each has its own); where there are several fans (then no other such begins
+        // within kFan ids), one for the first and one for each of the others.
+        unsigned* const counters = reinterpret_cast<unsigned*>(p.ws);
+        const int ids = p.split + 2, of_fans = (ids + kFan - 1) / kFan;
+        const int fan = part / kFan, fans = (parts + kFan - 1) / kFan;
+        auto fan_id = [&](int f) { return f == 0 ? w0 / kFan : of_fans + (w0 + f * kFan) / kFan; };
+        const int joined = slots0 + 2 * ids * slot;
+        for (int level = fans == 1 ? 1 : 0; level < 2; ++level) {
+            // level 0: this fan's parts into one; level 1: all there is into the output
+            const int n = level == 0 ? (parts - fan * kFan < kFan ? parts - fan * kFan : kFan) : fans == 1 ? parts : fans;
+            if (!last_in(level == 0 ? counters + ids + fan_id(fan) : counters + w0, n, &flag)) break;
+            const bool of_parts = level == 0 || fans == 1;
+            const int from0 = of_parts ? part_at(level == 0 ? fan * kFan : 0) : joined + fan_id(0) * slot;
+            const int from1 = of_parts ? part_at((level == 0 ? fan * kFan : 0) + 1) : joined + fan_id(1) * slot;
+            const int step = of_parts ? 2 * slot : slot;
+            for (int i = tid; i < rows * D / 4; i += 64 * W) {
+                const int h = i / (D / 4);
+                float4_t sum = {0, 0, 0, 0};
+                float top = -INFINITY, tot = 0.f;
+                constexpr int kBatch = kFan;   // loads of a batch go out together
+                for (int u0 = 0; u0 < n; u0 += kBatch) {
+                    int4_t o[kBatch];
+                    float2 st[kBatch];
+                    float most = top;
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int e = u0 + u < n ? u0 + u : n - 1;
+                        const int at = e == 0 ? from0 : from1 + (e - 1) * step;
+                        o[u] = __builtin_amdgcn_raw_buffer_load_b128(ws, i * 16, at, 16);
+                        const auto x = __builtin_amdgcn_raw_buffer_load_b64(ws, rows * D * 4 + h * 8, at, 16);
+                        st[u] = make_float2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                    }
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) most = fmaxf(most, st[u].x);
+                    const float keep = top == -INFINITY ? 0.f : exp2_of(top - most);
+                    tot *= keep;
+                    sum *= keep;
+                    top = most;
+#pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        if (u0 + u >= n) continue;
+                        const float by = st[u].x == -INFINITY ? 0.f : exp2_of(st[u].x - top);
+                        tot = fmaf(st[u].y, by, tot);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) sum[x] = fmaf(__int_as_float(o[u][x]), by, sum[x]);
+                    }
+                }
+                put(level == 0 ? joined + fan_id(fan) * slot : -1, i, sum, top, tot);
             }
-            const int i = h * (D / 4) + n * (DL / 4) + e % (DL / 4);
-            if (units == 1) put_out<D>(p, head0, i, sum, tot);
-            else put_part<D>(p, mine + unit * bytes, rows, i, sum, top, tot);
         }
     }
-    if (units == 1) return;
-    // counters: one per (.., head tile), then one for each of its fans
-    unsigned* const counters = reinterpret_cast<unsigned*>(p.ws);
-    const int fan = unit / kFan, nfan = (units + kFan - 1) / kFan;
-    const int in_fan = units - fan * kFan < kFan ? units - fan * kFan : kFan;
-    auto out = [&](int i, float4_t sum, float, float l2) { put_out<D>(p, head0, i, sum, l2); };
-    if (nfan == 1) {
-        if (last_in(counters + bh, units, &flag)) join_parts<D>(p, mine, units, rows, out);
-        return;
-    }
-    if (!last_in(counters + gridDim.x + bh * fans + fan, in_fan, &flag)) return;
-    const int64_t joined = kCounterBytes + (static_cast<int64_t>(gridDim.x) * p.max_units + bh * fans) * all;
-    join_parts<D>(p, mine + fan * kFan * bytes, in_fan, rows,
-                  [&](int i, float4_t sum, float m2, float l2) { put_part<D>(p, joined + fan * bytes, rows, i, sum, m2, l2); });
-    if (last_in(counters + bh, nfan, &flag)) join_parts<D>(p, joined, nfan, rows, out);
 }
 
-// Tokens a unit takes and units of the longest sequence, for `most` tokens at most.
-struct Split {
-    int64_t unit, units, fans;
-};
-Split choose_split(int64_t groups, int64_t most) {
-    constexpr int64_t kWant = 1024;              // workgroups
-    Split s;
-    s.unit = ceil_div(ceil_div(groups * most, kWant), kStep) * kStep;
-    if (s.unit < kStep) s.unit = kStep;
-    s.units = most > 0 ? ceil_div(most, s.unit) : 1;
-    s.fans = ceil_div(s.units, kFan);
-    return s;
+// Workgroups to cut the `groups` (sequence, cache head, head tile)s of up to `most` tokens for: what the chip
+// holds at once.  0: nothing to cut.
+int choose_workers(int64_t groups, int64_t most, int64_t D) {
+    const int64_t tiles = ceil_div(most, kTile);
+    if (most <= 4 * kTile || groups * tiles > 0x3fffffff) return 0;
+    return static_cast<int>(std::min<int64_t>(D == 256 ? 512 : 768, groups * ceil_div(tiles, 4)));
 }
-int64_t split_bytes(const Split& s, int64_t groups, int64_t rows, int64_t D) {
-    return s.units == 1 ? 0 : kCounterBytes + groups * (s.units + (s.fans > 1 ? s.fans : 0)) * part_bytes(static_cast<int>(rows), static_cast<int>(D));
+int64_t split_bytes(int64_t workers, int64_t rows, int64_t D) {
+    return workers == 0 ? 0 : kCounterBytes + (2 * (workers + 2) + 2 * ceil_div(workers + 2, kFan)) * part_bytes(static_cast<int>(rows), static_cast<int>(D));
 }
 
 }  // namespace
@@ -383,7 +444,7 @@ int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || B > 0x7fffffff / Hq || D <= 0 || max_seq_len < 0) return 0;
     const int64_t group = Hq / Hkv, groups = B * Hkv * ceil_div(group, kHeads);
     const int64_t most = max_seq_len < kMaxLen ? max_seq_len : kMaxLen;
-    return split_bytes(choose_split(groups, most), groups, group < kHeads ? group : kHeads, D);
+    return split_bytes(choose_workers(groups, most, D), group < kHeads ? group : kHeads, D);
 }
 
 int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
@@ -412,29 +473,28 @@ int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void
         return fail(MCV_ERR_UNSUPPORTED, "paged_attention: pointers must be 16-byte aligned, strides multiples of 8 elements");
     int rc = require_device();
     if (rc != MCV_OK) return rc;
-    if (k_token > (1 << 26) || v_token > (1 << 26))
+    if (k_token > (1 << 25) || v_token > (1 << 25))
         return fail(MCV_ERR_UNSUPPORTED, "paged_attention: tokens of one page too far apart");
     // (width counted in pages first: width * page_size could pass 64 bits)
     const int64_t held = table_width > kMaxLen / page_size ? kMaxLen : table_width * page_size;
     const int64_t most = max_seq_len < held ? max_seq_len : held;
     const int64_t group = Hq / Hkv, htiles = ceil_div(group, kHeads), groups = B * Hkv * htiles;
     const int64_t rows = group < kHeads ? group : kHeads;
-    Split s = choose_split(groups, most);
-    if (s.units > 1 && (!workspace || workspace_bytes < split_bytes(s, groups, rows, D))) s = {ceil_div(most, kStep) * kStep, 1, 1};
-    if (s.units > 1 && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    int workers = choose_workers(groups, most, D);
+    if (workers && (!workspace || workspace_bytes < split_bytes(workers, rows, D))) workers = 0;
+    if (workers && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "paged_attention: workspace must be 256-byte aligned");
     const uint32_t page16 = static_cast<uint32_t>(page_size / 16);
     AttnArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache),
                static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(seq_lens), static_cast<uint16_t*>(out),
                static_cast<uint8_t*>(workspace), q_row, q_head, k_page, k_head, v_page, v_head, table_row,
                static_cast<int>(k_token), static_cast<int>(v_token), static_cast<int>(pages), static_cast<int>(page16),
-               static_cast<int>(most), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
-               static_cast<int>(htiles), static_cast<int>(s.unit > 0 ? s.unit : kStep), static_cast<int>(s.units),
-               page16 > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + page16 - 1) / page16) : 0,
-               static_cast<float>(scale) * kLog2e};
-    auto fn = D == 64 ? paged_attention_kernel<64> : D == 128 ? paged_attention_kernel<128> : paged_attention_kernel<256>;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups), static_cast<unsigned>(s.units)), dim3(64 * kWaves),
-                       static_cast<unsigned>(kWaves * rows * (D < 128 ? D : 128) * 4), static_cast<hipStream_t>(stream), a);
+               static_cast<int>(most), static_cast<int>(B), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
+               static_cast<int>(htiles), page16 > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + page16 - 1) / page16) : 0,
+               static_cast<float>(scale) * kLog2e, workers};
+    auto fn = D == 64 ? paged_attention_kernel<64, 4> : D == 128 ? paged_attention_kernel<128, 4> : paged_attention_kernel<256, 4>;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(groups + workers)), dim3(256),
+                       static_cast<unsigned>(4 * std::max<int64_t>(kTile * 2 * (D + 8), rows * 4 * D)), static_cast<hipStream_t>(stream), a);
     return check_launch("paged_attention_kernel");
 }
 

@@ -70,8 +70,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale=
     Token t lies in row t % page_size of page block_table[b, t // page_size]; a page
     number outside the cache is left out like a masked token, and a sequence of
     length 0 gives zeros.  max_seq_len, at most width * page_size (the default),
-    bounds the lengths and sets how the work is split; pass the longest length
-    known.  Returns out fp16 [B, Hq, D]."""
+    bounds the lengths.  Returns out fp16 [B, Hq, D]."""
     return (_BINDING or binding()).paged(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len, out, stream)
 
 

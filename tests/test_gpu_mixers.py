@@ -268,6 +268,18 @@ def test_paged_attention(mcv, cuda, lens, Hq, Hkv, D, page):
     _attn_close(got, _attn_ref(q, kv, Hkv, 0.05))
 
 
+@pytest.mark.parametrize("B,longest,Hq,Hkv,D,page", [(150, 900, 4, 2, 64, 16), (65, 3000, 8, 1, 128, 32), (300, 40, 6, 3, 256, 16),
+                                                     (64, 700, 20, 1, 128, 16), (129, 130, 16, 8, 64, 16)])
+def test_paged_attention_many_sequences(mcv, cuda, B, longest, Hq, Hkv, D, page):
+    """More sequences than lanes of a wave, from none to the longest: cut in parts, whole, and both together."""
+    torch = _torch()
+    lens = (torch.rand(B, generator=_gen(B)) ** 3 * (longest + 1)).int()
+    lens[0], lens[B // 2], lens[-1] = 0, longest, longest - 1
+    q, k, v, table, n, kv = _attn_case(B + D, lens.tolist(), Hq, Hkv, D, page)
+    got = mcv.paged_attention_decode(*(x.to(cuda) for x in (q, k, v, table, n)))
+    _attn_close(got, _attn_ref(q, kv, Hkv, D ** -0.5))
+
+
 def test_paged_attention_absent_pages(mcv, cuda):
     """Page numbers outside the cache are left out, wherever they stand; a row of none gives zeros."""
     torch = _torch()
