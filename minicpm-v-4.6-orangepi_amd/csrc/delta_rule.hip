@@ -17,6 +17,21 @@ namespace mcv {
 namespace {
 
 constexpr int kThreads = 256;
+
+// Sum over the lanes of one lane % C4 (C4 4 .. 32), in all of them: steps of a butterfly as in wave_butterfly.
+template <int C4>
+__device__ __forceinline__ float sum_over(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    if constexpr (C4 <= 16) {
+        const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
+    if constexpr (C4 <= 8) v += row_ror<8>(v);
+    if constexpr (C4 <= 4) v += row_ror<4>(v);
+    return v;
+}
+
 template <int DK, int DVW>
 __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) {
     constexpr int C4 = DVW / 4;                  // lanes over one row's columns
@@ -70,9 +85,7 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
             s[10] = fmaf(qr[j], qr[j], s[10]);
         }
 #pragma unroll
-        for (int m = 32; m >= C4; m >>= 1)
-#pragma unroll
-            for (int x = 0; x < 11; ++x) s[x] += __shfl_xor(s[x], m, 64);
+        for (int x = 0; x < 11; ++x) s[x] = sum_over<C4>(s[x]);
         const int buf = (i - t0) & 1;            // the other buffer may still be read by a slower wave
         if (lane < C4) {
             part[buf][wave][lane][0] = float4_t{s[0], s[1], s[2], s[3]};
@@ -169,10 +182,14 @@ int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, 
         return launch_delta_chunk(a, static_cast<int>(Hk), static_cast<int>(Dk), workspace, workspace_bytes,
                                   static_cast<hipStream_t>(stream));
     }
-    const int64_t grid = B * Hv * (Dv / 16);
+    // Columns a workgroup holds: 256 bytes of a row at a time unless that leaves most CUs without work.  MI355X, us a
+    // pass of 128 x 128 states, 16 and 64 columns: 16 states 3.8 4.1, 64 5.8 5.2, 256 13.3 9.6, 848 32.7 25.6.
+    const int width = Dv % 64 == 0 && B * Hv * (Dv / 64) >= 96 ? 64 : 16;
+    const int64_t grid = B * Hv * (Dv / width);
     if (grid > 0x7fffffff) return fail(MCV_ERR_SHAPE, "delta_rule: too many states");
-    hipLaunchKernelGGL((Dk == 64 ? delta_recurrent_kernel<64, 16> : delta_recurrent_kernel<128, 16>),
-                       dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    auto fn = Dk == 64 ? (width == 64 ? delta_recurrent_kernel<64, 64> : delta_recurrent_kernel<64, 16>)
+                       : (width == 64 ? delta_recurrent_kernel<128, 64> : delta_recurrent_kernel<128, 16>);
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
     return check_launch("delta_recurrent_kernel");
 }
 
