@@ -36,7 +36,7 @@ namespace {
 constexpr int kC = 64;                           // tokens of a chunk
 constexpr int64_t kSegmentBytes = int64_t(192) << 20;   // workspace of one pass over the chunks
 constexpr int kBet = 0, kBr = 64, kEf = 128, kEq = 192, kOsc = 256;   // of a unit's scalars, 64 each, then:
-constexpr int kKeep = 320, kVmax = 321;          // e^(G_last), largest |v| each wave saw (4)
+constexpr int kKeep = 320, kVmax = 321;          // e^(G_last), largest |v| two waves saw
 constexpr int kScalars = 352;
 constexpr int kTriBytes = 6 * 2 * 64 * 16;       // a triangle of 16 x 32 blocks, two parts
 
@@ -58,19 +58,25 @@ __device__ __forceinline__ int tri_block(int w, int s) { return (w < 2 ? w : 2 *
 // at most T / 64 + B, without a table of chunks.
 __device__ __forceinline__ int first_slot(int t0, int b) { return t0 / kC + b; }
 
-// The sequence whose slots include `slot`: the last b whose first slot is not past it.
-__device__ __forceinline__ int seq_of_slot(const DeltaArgs& p, int slot) {
+// The sequence whose slots include `slot`: the last b whose first slot is not past it; its span.
+__device__ __forceinline__ int seq_of_slot(const DeltaArgs& p, int slot, int& t0, int& t1) {
     const int lane = threadIdx.x & 63;
     int b = 0;
+    t0 = t1 = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int t0 = 0, t1;
+        int from = 0, to = 0;
         const int mine = b0 + lane;
-        if (mine < p.B) delta_span(p, mine, t0, t1);
-        const unsigned long long on = __ballot(mine < p.B && first_slot(t0, mine) <= slot);
-        if (on) b = b0 + 63 - __builtin_clzll(on);
+        if (mine < p.B) delta_span(p, mine, from, to);
+        const unsigned long long on = __ballot(mine < p.B && first_slot(from, mine) <= slot);
+        if (on) {
+            const int at = 63 - __builtin_clzll(on);
+            b = b0 + at;
+            t0 = __builtin_amdgcn_readlane(from, at);
+            t1 = __builtin_amdgcn_readlane(to, at);
+        }
         if (on != ~0ull) break;
     }
-    return __builtin_amdgcn_readfirstlane(b);
+    return b;
 }
 
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
@@ -97,9 +103,36 @@ __device__ __forceinline__ float apart(float x) {
     asm("" : "+v"(x));
     return x;
 }
+// Sum over the lanes up to this one: rows of 16 by one, two, four, eight; a row's last to the next; lane 31 to the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lane_of(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan(double v) {
+    v += lane_of<0x111, 0xf>(v);
+    v += lane_of<0x112, 0xf>(v);
+    v += lane_of<0x114, 0xf>(v);
+    v += lane_of<0x118, 0xf>(v);
+    v += lane_of<0x142, 0xa>(v);
+    return v + lane_of<0x143, 0xc>(v);
+}
+// Lane r's value of each four lanes.
+__device__ __forceinline__ float of_quad(float v, int r) {
+    const int i = __float_as_int(v);
+    return __int_as_float(r == 0   ? __builtin_amdgcn_update_dpp(0, i, 0x00, 0xf, 0xf, false)
+                          : r == 1 ? __builtin_amdgcn_update_dpp(0, i, 0x55, 0xf, 0xf, false)
+                          : r == 2 ? __builtin_amdgcn_update_dpp(0, i, 0xaa, 0xf, 0xf, false)
+                                   : __builtin_amdgcn_update_dpp(0, i, 0xff, 0xf, 0xf, false));
+}
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 // LDS is ready for the other waves; global loads in flight stay there.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Global loads after this stay behind the LDS writes before it, which others wait for.
+__device__ __forceinline__ void lds_first() { asm volatile("" ::: "memory"); }
 
 // Position of token t's value in row d of a transposed tile [D][64] fp16: operand order,
 // 16-byte blocks moved so that neither the pair stores nor the operand loads conflict.
@@ -116,9 +149,8 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % p.Hv, local = blockIdx.x / p.Hv, hk = h / p.group;
     const int slot = a.slot0 + local;
-    const int b = seq_of_slot(p, slot);
     int t0, t1;
-    delta_span(p, b, t0, t1);
+    const int b = seq_of_slot(p, slot, t0, t1);
     const int chunk = slot - first_slot(t0, b);
     const int64_t start = t0 + static_cast<int64_t>(chunk) * kC;
     if (chunk < 0 || start >= t1) return;
@@ -128,7 +160,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     // k and q as rows, 16-byte chunks moved so that operand reads do not conflict; then k turned and L, T
     constexpr int RC = DK / 8;                   // chunks of a row
     __shared__ __attribute__((aligned(16))) uint8_t space[2][kC * PT * 4];
-    __shared__ __attribute__((aligned(16))) float gh[kC], gl[kC], bet[kC], rkn[kC], rqn[kC], kk[kC], qq[kC];
+    __shared__ __attribute__((aligned(16))) float gh[kC], gl[kC], bet[kC], rkn[kC], rqn[kC], kk[kC], qq[kC], lrow[kC], pcol[kC], fall[4][kC];
     __shared__ __attribute__((aligned(16))) _Float16 kpow[kC];
     half8_t* const kr = reinterpret_cast<half8_t*>(space[0]);
     half8_t* const qr = reinterpret_cast<half8_t*>(space[1]);
@@ -146,6 +178,16 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     float gate = 0.f;
     if (w == 0) gate = p.g[(start + row(lane)) * p.g_row + h];
     else if (w == 1) gate = p.beta[(start + row(lane)) * p.beta_row + h];
+    constexpr int VT = 8;                        // 16-byte chunks of v a thread of waves 0 and 1 has at a time
+    const int vchunks = kC * p.Dv / 8, vrow = p.Dv / 8;
+    uint4 vx[VT];
+    auto load_v = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < VT; ++i) {
+            const int at = from + static_cast<int>(threadIdx.x) + 128 * i, e = at < vchunks ? at : vchunks - 1;
+            vx[i] = *reinterpret_cast<const uint4*>(vb + row(e / vrow) * p.v_row + e % vrow * 8);
+        }
+    };
     {
         constexpr int IT = kC * RC / 256;
         half8_t x[IT], y[IT];
@@ -162,7 +204,8 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
             qr[place(t, ch)] = t < n ? y[i] : none;
         }
     }
-    __syncthreads();
+    if (w < 2) load_v(0);
+    lds_barrier();
     // Products of the raw rows: this wave's 16 tokens against those up to them.
     float4_t kkt[4], kqt[4], qqt = {};
     {
@@ -203,14 +246,26 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     if (w == 0) {
         // a decay below e^-200 is none in 32 bits; G's differences want more than a 32-bit sum
         double G = lane < n ? static_cast<double>(gate < -200.f ? -200.f : gate) * 1.4426950408889634074 : 0.0;
-        for (int m = 1; m < 64; m <<= 1) {
-            const double o = __shfl_up(G, m, 64);
-            if (lane >= m) G += o;
-        }
+        G = wave_scan(G);
         gh[lane] = static_cast<float>(G);
         gl[lane] = static_cast<float>(G - static_cast<double>(static_cast<float>(G)));
     } else if (w == 1) {
         bet[lane] = lane < n ? gate : 0.f;
+    }
+    if (w < 2) {                                 // the largest |v|, for the scan's scale; these have fewer products
+        half2_t most = {0, 0};                   // (a maximum with NaN is the other)
+        for (int from = 0;;) {
+#pragma unroll
+            for (int i = 0; i < VT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    most = __builtin_elementwise_max(most, as_h2((e == 0 ? vx[i].x : e == 1 ? vx[i].y : e == 2 ? vx[i].z : vx[i].w) & 0x7fff7fffu));
+            from += 128 * VT;
+            if (from >= vchunks) break;
+            load_v(from);
+        }
+        const float big = wave_butterfly(fmaxf(static_cast<float>(most[0]), static_cast<float>(most[1])), [](float x, float y) { return fmaxf(x, y); });
+        if (lane == 0) sc[kVmax + w] = big;
     }
     __syncthreads();
     // k turned: a thread packs two tokens of eight d
@@ -221,28 +276,39 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
         for (int e = 0; e < 8; ++e)
             *reinterpret_cast<half2_t*>(kt + turned(8 * ch + e, token_block(t)) + token_in_block(t)) = half2_t{x[e], y[e]};
     }
-    if (w == 0) {
-        const float k2 = kk[lane], q2 = qq[lane];
-        const float rk = p.normalize ? 1.0f / sqrtf(k2 + kDeltaEps) : 1.0f;
-        const float pw = p.normalize ? ldexpf(1.0f, ilogbf(rk)) : 1.0f;
-        const float rn = q2 > 0.f ? 1.0f / sqrtf(q2) : 0.f;
-        const float eg = exp2f(gh[lane] + gl[lane]);
-        const float fall = exp2f((gh[kC - 1] - gh[lane]) + (gl[kC - 1] - gl[lane]));
-        rkn[lane] = rk;
-        rqn[lane] = rn;
-        kpow[lane] = static_cast<_Float16>(pw);
-        sc[kBet + lane] = bet[lane];
-        sc[kBr + lane] = bet[lane] * rk * eg;
-        sc[kEf + lane] = fall * (rk / pw);
-        sc[kEq + lane] = eg * rn;
-        sc[kOsc + lane] = p.scale * (p.normalize ? sqrtf(q2 / (q2 + kDeltaEps)) : sqrtf(q2));
-        if (lane == kC - 1) sc[kKeep] = eg;
+    {
+        // Norm factors within a last bit: the same ones enter T, P and the scan's scalars.
+        const float k2 = kk[lane], q2 = qq[lane], g_hi = gh[lane], g_lo = gl[lane];
+        const float rk = p.normalize ? __builtin_amdgcn_rsqf(k2 + kDeltaEps) : 1.0f;
+        const float rn = q2 > 0.f ? __builtin_amdgcn_rsqf(q2) : 0.f;
+        // e^(G_i - G_j) of tiles below the diagonal is e^(G_i - G_r) e^(G_r - G_j), r the row tile's first token: neither is above one
+        fall[w][lane] = exp2_of((gh[16 * w] - g_hi) + (gl[16 * w] - g_lo)) * rk;
+        if (w == 0) {
+            const float eg = exp2_of(g_hi + g_lo), to_end = exp2_of((gh[kC - 1] - g_hi) + (gl[kC - 1] - g_lo));
+            const uint32_t bits = __float_as_uint(rk);           // pw: the power of two at or below it
+            const float b = bet[lane];
+            kpow[lane] = static_cast<_Float16>(p.normalize ? __uint_as_float(bits & 0x7f800000u) : 1.0f);
+            rkn[lane] = rk;
+            sc[kBet + lane] = b;
+            sc[kBr + lane] = b * rk * eg;
+            sc[kEf + lane] = to_end * (p.normalize ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 1.0f);
+            if (lane == kC - 1) sc[kKeep] = eg;
+        } else if (w == 1) {
+            rqn[lane] = rn;
+            sc[kEq + lane] = exp2_of(g_hi + g_lo) * rn;
+            sc[kOsc + lane] = p.scale * (q2 * rn) * (p.normalize ? __builtin_amdgcn_rsqf(q2 + kDeltaEps) : 1.0f);
+        } else if (w == 2) {
+            const float ea = exp2_of((g_hi - gh[lane & 48]) + (g_lo - gl[lane & 48]));
+            lrow[lane] = bet[lane] * ea * rk;
+            pcol[lane] = ea * rn;
+        }
     }
     __syncthreads();
 
     // L into LDS; P straight out: its tile pairs are operands
-    const float ghc = gh[16 * w + c], glc = gl[16 * w + c], rqc = rqn[16 * w + c];
     float4_t pt[4];
+    const float4_t lr = *reinterpret_cast<const float4_t*>(&lrow[16 * w + 4 * j]);
+    const float pc = pcol[16 * w + c];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         pt[x] = float4_t{0, 0, 0, 0};
@@ -250,17 +316,24 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
             if (x == w + 1 && (w & 1) == 0)      // the other half of T's own step
 #pragma unroll
                 for (int r = 0; r < 4; ++r) tri[16 * w + 4 * j + r][16 * x + c] = 0.f;
-            continue;
-        }
-        const float gx = gh[16 * x + c], gxl = gl[16 * x + c], rkx = rkn[16 * x + c];
+        } else if (x < w) {
+            const float fc = fall[w][16 * x + c];
+            const float4_t fr = *reinterpret_cast<const float4_t*>(&fall[w][16 * x + 4 * j]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * w + 4 * j + r;    // L: row i, column 16 x + c
-            const float f = bet[i] * exp2_of((gh[i] - gx) + (gl[i] - gxl)) * rkn[i] * rkx;
-            tri[i][16 * x + c] = 16 * x + c < i ? f * kkt[x][r] : 0.f;
-            const int y = 16 * x + 4 * j + r;    // P: key y, query 16 w + c
-            const float e = exp2_of((ghc - gh[y]) + (glc - gl[y])) * rkn[y] * rqc;
-            pt[x][r] = y <= 16 * w + c ? e * kqt[x][r] : 0.f;
+            for (int r = 0; r < 4; ++r) {
+                tri[16 * w + 4 * j + r][16 * x + c] = lr[r] * fc * kkt[x][r];        // L: row 16 w + 4 j + r, column 16 x + c
+                pt[x][r] = fr[r] * pc * kqt[x][r];                                   // P: key 16 x + 4 j + r, query 16 w + c
+            }
+        } else {
+            const float ghc = gh[16 * w + c], glc = gl[16 * w + c], rkc = rkn[16 * w + c], rqc = rqn[16 * w + c];
+            const float4_t hr = *reinterpret_cast<const float4_t*>(&gh[16 * w + 4 * j]), lo = *reinterpret_cast<const float4_t*>(&gl[16 * w + 4 * j]);
+            const float4_t rr = *reinterpret_cast<const float4_t*>(&rkn[16 * w + 4 * j]), br = *reinterpret_cast<const float4_t*>(&bet[16 * w + 4 * j]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float d = (hr[r] - ghc) + (lo[r] - glc);
+                tri[16 * w + 4 * j + r][16 * w + c] = c < 4 * j + r ? br[r] * exp2_of(d) * rr[r] * rkc * kkt[x][r] : 0.f;
+                pt[x][r] = 4 * j + r <= c ? exp2_of(-d) * rr[r] * rqc * kqt[x][r] : 0.f;
+            }
         }
     }
 #pragma unroll
@@ -276,9 +349,9 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
         at[64] = as_u4(lo);
     }
     // K turned, scaled, in operand order: row c of tile i is dk 32 (i / 2) + 8 (c / 4) + 4 (i % 2) + c % 4
-    if (h % p.group == 0)
+    if (h % p.group == 0 && w < 2)
 #pragma unroll
-        for (int i = w; i < DK / 16; i += 4) {
+        for (int i = w; i < DK / 16; i += 2) {
             const int d = 32 * (i / 2) + 8 * (c / 4) + 4 * (i % 2) + c % 4;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -289,22 +362,6 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
                     as_u4(*reinterpret_cast<const half8_t*>(kt + turned(d, 4 * s + j)) * pw);
             }
         }
-    // the largest |v|, for the scan's scale
-    {
-        uint32_t most = 0;                       // of fp16 magnitudes as whole numbers; NaN is none
-        for (int i = threadIdx.x; i < kC * p.Dv / 8; i += 256) {
-            const uint4 v = *reinterpret_cast<const uint4*>(vb + row(i / (p.Dv / 8)) * p.v_row + i % (p.Dv / 8) * 8);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t u = (e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w) & 0x7fff7fffu;
-                const uint32_t x = u & 0xffff, y = u >> 16;
-                most = x <= 0x7c00 && x > most ? x : most;
-                most = y <= 0x7c00 && y > most ? y : most;
-            }
-        }
-        const float big = wave_butterfly(h2f(static_cast<uint16_t>(most)), [](float x, float y) { return fmaxf(x, y); });
-        if (lane == 0) sc[kVmax + w] = big;
-    }
     __syncthreads();
 
     // T: the diagonal blocks by substitution, lane c a column; in place
@@ -369,8 +426,8 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
 // Column x of lane c is dv NT c + x of the slice.
 template <int DK, int NT>
 __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
-    constexpr int KS = DK / 32, MT = DK / 64;    // steps over dk; tiles of the state a wave carries
     constexpr int PD = 2;                        // chunks whose operands are in flight
+    constexpr int KS = DK / 32, MT = DK / 64;    // steps over dk; tiles of the state a wave carries
     const DeltaArgs& p = a.d;
     const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
@@ -437,16 +494,21 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
     }
     const int slot = s0 + c0 - a.slot0;          // of chunk c0 in this pass
     const int64_t unit0 = static_cast<int64_t>(slot) * p.Hv + h;     // its unit; the next is Hv on
-    for (int i = threadIdx.x; i < (c1 - c0) * 4; i += 512)
-        big = fmaxf(big, a.sc[(unit0 + static_cast<int64_t>(i / 4) * p.Hv) * kScalars + kVmax + i % 4]);
-    big = wave_butterfly(big, [](float x, float y) { return fmaxf(x, y); });
-    if (lane == 0) maxes[wave] = big;
-    __syncthreads();
+    for (int i = threadIdx.x; i < (c1 - c0) * 2; i += 512)
+        big = fmaxf(big, a.sc[(unit0 + static_cast<int64_t>(i / 2) * p.Hv) * kScalars + kVmax + i % 2]);
+    // Both kinds of waves call this once, with their first operands on the way.
+    float up, down;
+    auto agree_on_scale = [&]() {
+        float most = wave_butterfly(big, [](float x, float y) { return fmaxf(x, y); });
+        if (lane == 0) maxes[wave] = most;
+        lds_barrier();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) big = fmaxf(big, maxes[i]);
-    int ex = big > 0.f && big < INFINITY ? 3 - ilogbf(big) : 0;
-    ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
-    const float up = ldexpf(1.0f, ex), down = ldexpf(1.0f, -ex);
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, maxes[i]);
+        int ex = most > 0.f && most < INFINITY ? 3 - ilogbf(most) : 0;
+        ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
+        up = ldexpf(1.0f, ex);
+        down = ldexpf(1.0f, -ex);
+    };
     const int64_t first = t0 + static_cast<int64_t>(c0) * kC;
     const int n_last = t1 - (first + static_cast<int64_t>(count - 1) * kC) < kC
                            ? static_cast<int>(t1 - (first + static_cast<int64_t>(count - 1) * kC)) : kC;
@@ -457,8 +519,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
         struct Stage {
             half8_t k[KS], kt[MT][2], t[2][2];
             vrow v[4];
-            float4_t bet, br, ef;
-            float keep;
+            float bet, br, ef, keep;             // of token 4 j + c % 4 of the wave's tile; e^(G_last)
         } st[PD];
         // Loads are unconditional (past the last chunk: the last again), so that a wait counts those in flight exactly.
         int64_t voff[4];
@@ -481,9 +542,9 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 s.v[r] = *reinterpret_cast<const vrow*>(vbase + static_cast<int64_t>(i) * kC * p.v_row + voff[r]);
-            const float* sc = a.sc + (unit0 + static_cast<int64_t>(i) * p.Hv) * kScalars + 16 * w + 4 * j;
-            s.bet = *reinterpret_cast<const float4_t*>(sc + kBet);
-            s.br = *reinterpret_cast<const float4_t*>(sc + kBr);
+            const float* sc = a.sc + (unit0 + static_cast<int64_t>(i) * p.Hv) * kScalars + 16 * w + 4 * j + c % 4;
+            s.bet = sc[kBet];
+            s.br = sc[kBr];
         };
         auto load_t = [&](Stage& s, int i) {
             const int64_t unit = unit0 + static_cast<int64_t>(i) * p.Hv;
@@ -492,7 +553,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
                 for (int part = 0; part < 2; ++part)
                     s.t[q][part] = as_h8(a.T[((unit * 6 + tri_block(w, w < 2 ? 0 : q)) * 2 + part) * 64 + lane]);
-            s.ef = *reinterpret_cast<const float4_t*>(a.sc + unit * kScalars + kEf + 16 * w + 4 * j);
+            s.ef = a.sc[unit * kScalars + kEf + 16 * w + 4 * j + c % 4];
         };
         auto load_kt = [&](Stage& s, int i) {
             const uint4* at = a.Kt + (static_cast<int64_t>(slot + i) * a.Hk + hk) * (DK / 16) * 2 * 64 + lane;
@@ -527,6 +588,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
             load_kt(st[q], i);
             asm volatile("" ::: "memory");       // in this order
         }
+        agree_on_scale();
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -537,23 +599,38 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
             for (int q = 0; q < PD; ++q) {
                 const int i = i0 + q;
                 if (i >= count) break;
-                Stage& s = st[q];
+                Stage &s = st[q], &before = st[(q + PD - 1) % PD];
                 const int ahead = next(i + PD);
                 const int live = i == count - 1 ? n_last : kC;
                 lds_barrier();                   // S is there
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    float4_t ks = {0, 0, 0, 0}, kl = {0, 0, 0, 0};
+                half8_t f[2][KS];
+                auto read_state = [&](int x) {
 #pragma unroll
                     for (int k = 0; k < KS; ++k) {
-                        ks = mfma16(s.k[k], as_h8(*reinterpret_cast<const uint4*>(&sf[0][x][k][lane][0])), ks);
-                        kl = mfma16(s.k[k], as_h8(*reinterpret_cast<const uint4*>(&sf[1][x][k][lane][0])), kl);
+                        f[0][k] = as_h8(*reinterpret_cast<const uint4*>(&sf[0][x][k][lane][0]));
+                        f[1][k] = as_h8(*reinterpret_cast<const uint4*>(&sf[1][x][k][lane][0]));
                     }
-                    ks += kl;
+                };
+                // What a phase has used is loaded anew in the next, behind its LDS reads and while they take their time.
+                read_state(0);
+                lds_first();
+                load_kt(before, next(i - 1 + PD));
+                lds_first();
+                const float bet_up = s.bet * up;
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    float4_t ks[4] = {};         // short chains: a product's result is late for the next
+                    if (x) read_state(x);
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        ks[k % 2] = mfma16(s.k[k], f[0][k], ks[k % 2]);
+                        ks[2 + k % 2] = mfma16(s.k[k], f[1][k], ks[2 + k % 2]);
+                    }
+                    ks[0] = (ks[0] + ks[1]) + (ks[2] + ks[3]);
                     float4_t v;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        v[r] = apart(fmaf(s.bet[r] * up, static_cast<float>(s.v[r][x]), -(s.br[r] * ks[r])));
+                        v[r] = apart(fmaf(of_quad(bet_up, r), static_cast<float>(s.v[r][x]), -(of_quad(s.br, r) * ks[0][r])));
                     if (live < kC)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
@@ -563,26 +640,35 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                     xf[0][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, hi);
                     xf[1][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, lo);
                 }
+                lds_barrier();                   // X is there
+                half8_t g[2][2];
+                auto read_x = [&](int x) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) g[part][k] = as_h8(*reinterpret_cast<const uint4*>(&xf[part][x][k][lane][0]));
+                };
+                read_x(0);
+                lds_first();
                 load_k(s, ahead);
                 load_v(s, ahead);
-                lds_barrier();                   // X is there
+                lds_first();
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
+                    if (x) read_x(x);
                     float4_t u = {0, 0, 0, 0}, v = {0, 0, 0, 0}, z = {0, 0, 0, 0};
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         if (2 * k > w) continue;
-                        const half8_t hi = as_h8(*reinterpret_cast<const uint4*>(&xf[0][x][k][lane][0]));
-                        const half8_t lo = as_h8(*reinterpret_cast<const uint4*>(&xf[1][x][k][lane][0]));
-                        u = mfma16(s.t[k][0], hi, u);
-                        v = mfma16(s.t[k][0], lo, v);
-                        z = mfma16(s.t[k][1], hi, z);
+                        u = mfma16(s.t[k][0], g[0][k], u);
+                        v = mfma16(s.t[k][0], g[1][k], v);
+                        z = mfma16(s.t[k][1], g[0][k], z);
                     }
                     u += v + z;
                     float4_t eu;
                     half4_t part[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) eu[r] = apart(s.ef[r] * u[r]);
+                    for (int r = 0; r < 4; ++r) eu[r] = apart(of_quad(s.ef, r) * u[r]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] = apart(u[r]);
                     split<4>(eu, part[2], part[3]);
@@ -590,26 +676,34 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) uf[e][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, part[e]);
                 }
-                load_t(s, ahead);
                 lds_barrier();                   // U is there, S has been read
+                auto read_u = [&](int x) {
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) g[part][k] = as_h8(*reinterpret_cast<const uint4*>(&uf[2 + part][x][k][lane][0]));
+                };
+                read_u(0);
+                lds_first();
+                load_t(s, ahead);
+                lds_first();
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    if (x) read_u(x);
+                    float4_t low[MT] = {};
 #pragma unroll
                     for (int m = 0; m < MT; ++m) S[m][x] *= s.keep;
 #pragma unroll
-                for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const half8_t hi = as_h8(*reinterpret_cast<const uint4*>(&uf[2][x][k][lane][0]));
-                        const half8_t lo = as_h8(*reinterpret_cast<const uint4*>(&uf[3][x][k][lane][0]));
+                    for (int k = 0; k < 2; ++k)
 #pragma unroll
                         for (int m = 0; m < MT; ++m) {
-                            S[m][x] = mfma16(s.kt[m][k], hi, S[m][x]);
-                            S[m][x] = mfma16(s.kt[m][k], lo, S[m][x]);
+                            S[m][x] = mfma16(s.kt[m][k], g[0][k], S[m][x]);
+                            low[m] = mfma16(s.kt[m][k], g[1][k], low[m]);
                         }
-                    }
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) S[m][x] += low[m];
+                }
                 put_state();
-                load_kt(s, ahead);
             }
         store_state(down);
     } else {
@@ -640,15 +734,43 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
             load_p(st[q], i);
             asm volatile("" ::: "memory");
         }
+        agree_on_scale();
+        float4_t o[NT], ol[NT];                  // e^G Q S of a chunk: rows dv, column token
+        auto finish = [&](const Stage& s, int i) {
+            const int64_t t = first + static_cast<int64_t>(i) * kC + 16 * w + c;
+            uint16_t r[4 * NT];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                float4_t y = (o[x] + ol[x]) * s.eq, z = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (2 * k > w) continue;
+                    const half8_t hi = as_h8(*reinterpret_cast<const uint4*>(&uf[0][x][k][lane][0]));
+                    const half8_t lo = as_h8(*reinterpret_cast<const uint4*>(&uf[1][x][k][lane][0]));
+                    y = mfma16(hi, s.pf[k][0], y);
+                    z = mfma16(lo, s.pf[k][0], z);
+                    v = mfma16(hi, s.pf[k][1], v);
+                }
+                const float osc = s.osc * down;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[NT * e + x] = f2h((y[e] + (z[e] + v[e])) * osc);
+            }
+            if (t < t1) {
+                uint2* at_out = reinterpret_cast<uint2*>(p.out + (t * p.Hv + h) * p.Dv + dv0 + 4 * NT * j);
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+                    at_out[x] = make_uint2(r[4 * x] | (static_cast<uint32_t>(r[4 * x + 1]) << 16),
+                                           r[4 * x + 2] | (static_cast<uint32_t>(r[4 * x + 3]) << 16));
+            }
+        };
         for (int i0 = 0; i0 < count; i0 += PD)
 #pragma unroll
             for (int q = 0; q < PD; ++q) {
                 const int i = i0 + q;
                 if (i >= count) break;
-                Stage& s = st[q];
-                const int ahead = next(i + PD);
-                float4_t o[NT], ol[NT];          // rows dv, column token
-                lds_barrier();                   // S is there: for X first
+                Stage &s = st[q], &before = st[(q + PD - 1) % PD];
+                lds_barrier();                   // S is there, and U of the chunk before until X is
+                if (i > 0) finish(before, i - 1);
                 lds_barrier();
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
@@ -659,35 +781,13 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                         ol[x] = mfma16(as_h8(*reinterpret_cast<const uint4*>(&sf[1][x][k][lane][0])), s.q[k], ol[x]);
                     }
                 }
-                load_q(s, ahead);
-                lds_barrier();                   // U is there
-                const int64_t t = first + static_cast<int64_t>(i) * kC + 16 * w + c;
-                uint16_t r[4 * NT];
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    float4_t y = (o[x] + ol[x]) * s.eq, z = {0, 0, 0, 0};
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        if (2 * k > w) continue;
-                        const half8_t hi = as_h8(*reinterpret_cast<const uint4*>(&uf[0][x][k][lane][0]));
-                        const half8_t lo = as_h8(*reinterpret_cast<const uint4*>(&uf[1][x][k][lane][0]));
-                        y = mfma16(hi, s.pf[k][0], y);
-                        z = mfma16(lo, s.pf[k][0], z);
-                        z = mfma16(hi, s.pf[k][1], z);
-                    }
-                    const float osc = s.osc * down;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) r[NT * e + x] = f2h((y[e] + z[e]) * osc);
-                }
-                load_p(s, ahead);
-                if (t < t1) {
-                    uint2* at_out = reinterpret_cast<uint2*>(p.out + (t * p.Hv + h) * p.Dv + dv0 + 4 * NT * j);
-#pragma unroll
-                    for (int x = 0; x < NT; ++x)
-                        at_out[x] = make_uint2(r[4 * x] | (static_cast<uint32_t>(r[4 * x + 1]) << 16),
-                                               r[4 * x + 2] | (static_cast<uint32_t>(r[4 * x + 3]) << 16));
-                }
+                lds_barrier();                   // U is there, S has been read
+                load_p(before, next(i - 1 + PD));
+                load_q(s, next(i + PD));
             }
+#pragma unroll
+        for (int q = 0; q < PD; ++q)
+            if ((count - 1) % PD == q) finish(st[q], count - 1);
     }
 }
 
