@@ -58,25 +58,24 @@ __device__ __forceinline__ int tri_block(int w, int s) { return (w < 2 ? w : 2 *
 // at most T / 64 + B, without a table of chunks.
 __device__ __forceinline__ int first_slot(int t0, int b) { return t0 / kC + b; }
 
-// The sequence whose slots include `slot`: the last b whose first slot is not past it; its span.
+// The sequence whose slots include `slot`: the last b whose first slot is not past it, 64 probes at a time; its span.
 __device__ __forceinline__ int seq_of_slot(const DeltaArgs& p, int slot, int& t0, int& t1) {
     const int lane = threadIdx.x & 63;
     int b = 0;
-    t0 = t1 = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
+    for (int n = p.B;;) {                        // among b .. b + n - 1
+        const int step = (n + 63) / 64, mine = b + lane * step;
         int from = 0, to = 0;
-        const int mine = b0 + lane;
-        if (mine < p.B) delta_span(p, mine, from, to);
-        const unsigned long long on = __ballot(mine < p.B && first_slot(from, mine) <= slot);
-        if (on) {
-            const int at = 63 - __builtin_clzll(on);
-            b = b0 + at;
+        if (lane * step < n) delta_span(p, mine, from, to);
+        const unsigned long long on = __ballot(lane * step < n && first_slot(from, mine) <= slot);
+        const int at = on ? 63 - __builtin_clzll(on) : 0;
+        b += at * step;
+        if (step == 1) {
             t0 = __builtin_amdgcn_readlane(from, at);
             t1 = __builtin_amdgcn_readlane(to, at);
+            return b;
         }
-        if (on != ~0ull) break;
+        n = n - at * step < step ? n - at * step : step;
     }
-    return b;
 }
 
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));

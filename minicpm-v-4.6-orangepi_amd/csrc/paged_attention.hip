@@ -129,35 +129,52 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
     auto tiles_of = [&](int b, int len) { return b >= p.B ? 0 : len <= kTile ? 1 : (len + kTile - 1) / kTile; };   // none: one, its zeros
 
     // Tiles of a part, and this workgroup's sequence b, whose first part has number w_first and whose first tile b_first.
-    int per = 0x3fffffff, b = 0, len = 0, b_first = 0, w_first = 0;
+    // A lane adds up `span` sequences; where that is more than one, the chosen lane's are then taken one a lane.
+    const int me = blockIdx.x, span = (p.B + 63) / 64;
+    int per = 0x3fffffff, b, len = 0, b_first = 0, w_first = 0;
     {
-        int mine = length(lane);                 // of the first 64 sequences
+        int mine = length(lane);                 // (of span 1)
+        auto sum_of = [&](auto f) {
+            if (span == 1) return f(lane, mine);
+            int sum = 0;
+#pragma unroll 4
+            for (int i = 0; i < span; ++i) sum += f(lane * span + i, length(lane * span + i));
+            return sum;
+        };
         if (p.split) {
-            int total = 0;
-            for (int b0 = 0; b0 < p.B; b0 += 64)
-                total += __builtin_amdgcn_readlane(wave_scan(tiles_of(b0 + lane, b0 ? length(b0 + lane) : mine)), 63);
+            const int total = __builtin_amdgcn_readlane(wave_scan(sum_of(tiles_of)), 63);
             per = (total * per_seq + p.split - 1) / p.split;
             per = (per + W - 1) / W * W;
         }
-        for (int b0 = 0;; b0 += 64) {
-            if (b0 >= p.B) return;
-            if (b0) mine = length(b0 + lane);
-            const int tiles = tiles_of(b0 + lane, mine), parts = (tiles + per - 1) / per;
-            const int upto = wave_scan(parts * per_seq), tiles_upto = wave_scan(tiles * per_seq);
-            const unsigned long long past = __ballot(w_first + upto > static_cast<int>(blockIdx.x));
-            const int at = past ? __builtin_ctzll(past) : 64;    // the first lane past it
-            b = b0 + at;
-            if (past) len = __builtin_amdgcn_readlane(mine, at);
+        auto parts_of = [&](int b, int n) { return (tiles_of(b, n) + per - 1) / per; };
+        int upto = wave_scan(sum_of(parts_of) * per_seq), tiles_upto = wave_scan(sum_of(tiles_of) * per_seq);
+        unsigned long long past = __ballot(upto > me);           // lanes at and past this workgroup's
+        if (!past) return;
+        int at = __builtin_ctzll(past);
+        auto go_to = [&]() {
             if (at) {
                 w_first += __builtin_amdgcn_readlane(upto, at - 1);
                 b_first += __builtin_amdgcn_readlane(tiles_upto, at - 1);
             }
+        };
+        go_to();
+        b = at * span;
+        while (span > 1) {
+            mine = length(b + lane);
+            upto = wave_scan(parts_of(b + lane, mine) * per_seq);
+            tiles_upto = wave_scan(tiles_of(b + lane, mine) * per_seq);
+            past = __ballot(w_first + upto > me);
+            at = past ? __builtin_ctzll(past) : 64;
+            go_to();
+            b += at;
             if (past) break;
+            if (b >= p.B) return;                // (lengths that changed meanwhile)
         }
+        len = __builtin_amdgcn_readlane(mine, at);
     }
     per = __builtin_amdgcn_readfirstlane(per);
     const int tiles = len <= kTile ? 1 : (len + kTile - 1) / kTile, parts = (tiles + per - 1) / per;
-    const int in_seq = (static_cast<int>(blockIdx.x) - w_first) / parts, part = static_cast<int>(blockIdx.x) - w_first - in_seq * parts;
+    const int in_seq = (me - w_first) / parts, part = me - w_first - in_seq * parts;
     const int s0 = part * per, hk = in_seq / p.htiles, ht = in_seq - hk * p.htiles;
     const int rows = p.group - ht * kHeads < kHeads ? p.group - ht * kHeads : kHeads;
     const int64_t head0 = static_cast<int64_t>(b) * p.Hq + hk * p.group + ht * kHeads;

@@ -150,6 +150,23 @@ def test_delta_step_of_a_pool(mcv, cuda):
     assert (dev.cpu()[rest] == states[rest]).all()
 
 
+@pytest.mark.parametrize("B,longest", [(64, 90), (65, 70), (130, 40), (700, 30)])
+def test_delta_many_sequences(mcv, cuda, B, longest):
+    """More sequences than lanes of a wave, some empty, with tokens before the first and behind the last."""
+    torch = _torch()
+    lens = (torch.rand(B, generator=_gen(B)) * (longest + 1)).int().tolist()
+    lens[0], lens[B // 2], lens[-1] = longest, 0, 65
+    q, k, v, g, beta, state = _delta_case(B, [3, *lens, 5], 1, 2, 64, 32)
+    rows = slice(3, 3 + sum(lens))
+    ref = _delta_ref(*(x[rows] for x in (q, k, v, g, beta)), state[1:-1], lens, 0.125, True)
+    cu = 3 + _cu(lens, cuda)
+    a = [x.to(cuda) for x in (q, k, v, g, beta)]
+    out = torch.full(v.shape, 7.0, dtype=torch.float16, device=cuda)
+    _, final = mcv.gated_delta_rule(*a, state[1:-1].to(cuda), cu_seqlens=cu, scale=0.125, normalize=True, out=out)
+    _delta_close(out[rows], final, ref)
+    assert (out[:3] == 7).all() and (out[rows.stop:] == 7).all()
+
+
 @pytest.mark.parametrize("n", [1, 40, 333])
 def test_delta_continues(mcv, cuda, n):
     """A sequence cut anywhere and continued from its state, against the whole."""
