@@ -167,6 +167,52 @@ def test_delta_many_sequences(mcv, cuda, B, longest):
     assert (out[:3] == 7).all() and (out[rows.stop:] == 7).all()
 
 
+def test_delta_in_several_passes(mcv, cuda):
+    """So many heads that the workspace holds a few chunks at a time: sequences across its passes, and between them."""
+    lens = [300, 0, 900, 40, 260]
+    q, k, v, g, beta, state = _delta_case(12, lens, 256, 256, 64, 16)
+    assert mcv.lib().mcv_delta_rule_workspace_bytes(5, 1500, 256, 256, 64, 16) < mcv.lib().mcv_delta_rule_workspace_bytes(1, 64, 256, 256, 64, 16) * 14
+    ref = _delta_ref(q, k, v, g, beta, state, lens, 0.125, True)
+    out, final = mcv.gated_delta_rule(*(x.to(cuda) for x in (q, k, v, g, beta, state)), cu_seqlens=_cu(lens, cuda), scale=0.125,
+                                      normalize=True)
+    _delta_close(out, final, ref)
+
+
+def test_delta_pool_over_sequences(mcv, cuda):
+    """Whole sequences at rows of a pool, one absent (its outputs zero), one without tokens; then into another pool."""
+    torch = _torch()
+    lens, index, pool = [70, 33, 0, 150], [5, 8, 2, 0], 8
+    q, k, v, g, beta, state = _delta_case(13, lens, 2, 2, 128, 64)
+    states = torch.randn(pool, 2, 128, 64, generator=_gen(2))
+    for b, i in enumerate(index):
+        if i < pool:
+            states[i] = state[b]
+    ref = _delta_ref(q, k, v, g, beta, state, lens, 128 ** -0.5, True)
+    a = [x.to(cuda) for x in (q, k, v, g, beta)]
+    where = dict(cu_seqlens=_cu(lens, cuda), state_index=torch.tensor(index, dtype=torch.int32, device=cuda), normalize=True)
+    other = torch.full_like(states, 3.0).to(cuda)
+    dev = states.to(cuda)
+    out, final = mcv.gated_delta_rule(*a, dev, state_out=other, **where)
+    assert final is other and (dev.cpu() == states).all()
+    out2, same = mcv.gated_delta_rule(*a, dev, **where)
+    assert same is dev and (out2 == out).all()
+    on = [0, 2, 3]
+    rows = torch.tensor([i for b, n in enumerate(lens) for i in [b] * n])
+    rows_on = rows != 1
+    for got in (other, dev):
+        _delta_close(out[rows_on.to(cuda)], got[[index[b] for b in on]], (ref[0][rows_on], ref[1][rows_on], ref[2][on]))
+    assert (out[(rows == 1).to(cuda)] == 0).all()
+    rest = [i for i in range(pool) if i not in index]
+    assert (dev.cpu()[rest] == states[rest]).all() and (other[rest] == 3).all()
+
+
+def test_delta_no_tokens(mcv, cuda):
+    torch = _torch()
+    q, k, v, g, beta, state = (x.to(cuda) for x in _delta_case(14, [0, 0], 2, 2, 64, 32))
+    out, final = mcv.gated_delta_rule(q, k, v, g, beta, state, cu_seqlens=torch.zeros(3, dtype=torch.int32, device=cuda))
+    assert out.shape == (0, 2, 32) and (final == state).all()
+
+
 @pytest.mark.parametrize("n", [1, 40, 333])
 def test_delta_continues(mcv, cuda, n):
     """A sequence cut anywhere and continued from its state, against the whole."""
