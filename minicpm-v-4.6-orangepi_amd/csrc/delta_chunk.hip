@@ -177,15 +177,13 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     float gate = 0.f;
     if (w == 0) gate = p.g[(start + row(lane)) * p.g_row + h];
     else if (w == 1) gate = p.beta[(start + row(lane)) * p.beta_row + h];
-    constexpr int VT = 8;                        // 16-byte chunks of v a thread of waves 0 and 1 has at a time
-    const int vchunks = kC * p.Dv / 8, vrow = p.Dv / 8;
+    constexpr int VT = 8;                        // 16-byte chunks of v a thread of waves 0 and 1 has: 128 columns at a time
     uint4 vx[VT];
-    auto load_v = [&](int from) {
+    auto load_v = [&](int v0) {
+        const int col = v0 + static_cast<int>(threadIdx.x) % 16 * 8;
+        const uint16_t* at = vb + (col < p.Dv ? col : v0);
 #pragma unroll
-        for (int i = 0; i < VT; ++i) {
-            const int at = from + static_cast<int>(threadIdx.x) + 128 * i, e = at < vchunks ? at : vchunks - 1;
-            vx[i] = *reinterpret_cast<const uint4*>(vb + row(e / vrow) * p.v_row + e % vrow * 8);
-        }
+        for (int i = 0; i < VT; ++i) vx[i] = *reinterpret_cast<const uint4*>(at + row(static_cast<int>(threadIdx.x) / 16 + 8 * i) * p.v_row);
     };
     {
         constexpr int IT = kC * RC / 256;
@@ -259,8 +257,8 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     most = __builtin_elementwise_max(most, as_h2((e == 0 ? vx[i].x : e == 1 ? vx[i].y : e == 2 ? vx[i].z : vx[i].w) & 0x7fff7fffu));
-            from += 128 * VT;
-            if (from >= vchunks) break;
+            from += 128;
+            if (from >= p.Dv) break;
             load_v(from);
         }
         const float big = wave_butterfly(fmaxf(static_cast<float>(most[0]), static_cast<float>(most[1])), [](float x, float y) { return fmaxf(x, y); });
