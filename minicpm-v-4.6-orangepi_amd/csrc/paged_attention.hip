@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kTile = 32;                        // tokens a wave takes at a time
 constexpr int kHeads = 16;                       // query heads of one matrix product
+constexpr int kCus = 256;
 constexpr int kFan = 16;                         // parts joined by one workgroup
 constexpr int64_t kCounterBytes = 4096;
 constexpr int64_t kMaxLen = int64_t(1) << 30;   // tokens of one sequence
@@ -142,9 +143,20 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
             return sum;
         };
         if (p.split) {
-            const int total = __builtin_amdgcn_readlane(wave_scan(sum_of(tiles_of)), 63);
-            per = (total * per_seq + p.split - 1) / p.split;
-            per = (per + W - 1) / W * W;
+            const int total = __builtin_amdgcn_readlane(wave_scan(sum_of(tiles_of)), 63) * per_seq;
+            const auto whole_steps = [](int n) { return (n + W - 1) / W * W; };
+            per = whole_steps((total + p.split - 1) / p.split);
+            // Few (sequence, cache head)s: as many parts as CUs at most, so that none has two while others have one.
+            // MI355X, us of 256, 512 and 768 workgroups: 1 x 200000 77 81 87, 1 x 25000 D 128 26 29 30; where there
+            // are many, small parts even out better than one each: 41 x 4096 ragged 37 30 30, 8 x 20000 D 128 64 53 55.
+            if (p.B * per_seq <= kCus / 8 && total > kCus * W) {
+                per = whole_steps((total + kCus - 1) / kCus);
+                for (int i = 0; i < 4; ++i) {
+                    const int n = __builtin_amdgcn_readlane(wave_scan(sum_of([&](int b, int len) { return (tiles_of(b, len) + per - 1) / per; })), 63) * per_seq;
+                    if (n <= kCus) break;
+                    per = whole_steps(per + (per * (n - kCus) + kCus - 1) / kCus);
+                }
+            }
         }
         auto parts_of = [&](int b, int n) { return (tiles_of(b, n) + per - 1) / per; };
         int upto = wave_scan(sum_of(parts_of) * per_seq), tiles_upto = wave_scan(sum_of(tiles_of) * per_seq);
@@ -174,7 +186,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
     }
     per = __builtin_amdgcn_readfirstlane(per);
     const int tiles = len <= kTile ? 1 : (len + kTile - 1) / kTile, parts = (tiles + per - 1) / per;
-    const int in_seq = (me - w_first) / parts, part = me - w_first - in_seq * parts;
+    // (the cache heads of one part side by side: their rows lie together in memory)
+    const int part = (me - w_first) / per_seq, in_seq = me - w_first - part * per_seq;
     const int s0 = part * per, hk = in_seq / p.htiles, ht = in_seq - hk * p.htiles;
     const int rows = p.group - ht * kHeads < kHeads ? p.group - ht * kHeads : kHeads;
     const int64_t head0 = static_cast<int64_t>(b) * p.Hq + hk * p.group + ht * kHeads;
