@@ -8,9 +8,14 @@
 // and with T = (I + L)^-1:  X = diag(beta) (V - diag(e^G) K^ S),  U = T X.  Two launches:
 //   delta_prepare_kernel  every (chunk, value head) at once: T, P, the scalars, K turned
 //   delta_scan_kernel     a workgroup per 16 NT columns of one state walks its chunks
-// The scan takes K and V as they come and applies T, instead of T K and T V made ahead: three
-// products that wait for one another in place of two, but 41 KiB a (chunk, head) through
-// memory in place of 88, and K, exact in fp16, in place of T K in two parts.
+// The scan takes K and V as they come and applies T: three products that wait for one another
+// where T K and T V made ahead would leave two, but K is exact in fp16 where T K takes two
+// parts, and less goes through memory (8192 tokens: 49 + 144 us, with T K and T V 70 + 147).
+//
+// The first is bound by memory (8192 tokens, 16 heads of 128: 250 MB in 49 us on MI355X).
+// The second walks in series, 1.1 us a chunk: without its outputs 1.04, without the loads of
+// the state's waves 0.85, without both 0.75, which is three times an LDS write, a barrier,
+// an LDS read and a short chain of products; the loads are 76 KB a chunk and CU.
 //
 // Precision.  The state, G, L, T and all sums are fp32 (G's differences from a sum in 64
 // bits; T by substitution, in fp32 products).  Operands of products are two fp16 parts,
@@ -822,7 +827,9 @@ int launch_delta_chunk(const DeltaArgs& d, int Hk, int Dk, void* workspace, int6
     a.Q = reinterpret_cast<uint4*>(take(per * Hk * kC * Dk * 2));
     if (at - static_cast<uint8_t*>(workspace) > workspace_bytes) return fail(MCV_ERR_INVALID_ARG, "delta_rule: workspace too small");
     const int64_t states = ceil_div(static_cast<int64_t>(d.B) * d.Hv, 8) * 8, tiles = d.Dv / 16;
-    const int nt = tiles % 2 == 0 && states * (tiles / 2) >= 512 ? 2 : 1;
+    // 32 columns a workgroup where that still leaves one for every CU.  MI355X, us a pass (Dk = Dv = 128), 16 and 32
+    // columns: 32 states of 1000 tokens 41 49, 64 of 1000 76 76, 128 of 500 84 77, 288 of 100 74 60.
+    const int nt = tiles % 2 == 0 && states * (tiles / 2) >= 256 ? 2 : 1;
     for (int64_t s = 0; s < total; s += per) {
         a.slot0 = static_cast<int>(s);
         a.slots = static_cast<int>(std::min(per, total - s));

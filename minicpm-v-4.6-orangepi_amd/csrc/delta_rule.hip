@@ -5,7 +5,9 @@
 //   a = k . S,  b = q . S,  c = q . k          (sums over Dk)
 //   u = beta (v - e rk a),  S' = e S + rk k u,  out = scale rq (e b + rk c u)
 // so one pass over S gives everything that S' and out need: out comes from the old
-// state and c instead of a second sum over the new one.
+// state and c instead of a second sum over the new one.  One token is bound by the state's
+// way in and out (53 sequences of 16 states of 128 x 128: 24.8 us on MI355X, 4.5 TB/s, a
+// copy 5.2); more tokens take 1.1 us each, one after the other.
 //
 // A workgroup holds DVW columns of one state in registers for the whole sequence:
 // 16-byte column chunks over the lanes, R consecutive rows a thread (so its part of

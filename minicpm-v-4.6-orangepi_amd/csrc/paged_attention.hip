@@ -23,6 +23,11 @@
 // (written through; see w4a16_gemm_sk.hip) and counts itself in; the last of each kFan
 // parts joins them in order, and where there are more than kFan the last of those joins
 // the joined, so the bits do not depend on who is last and nobody waits.
+//
+// Long caches are bound by HBM: 8 heads on 2 of 256, 200000 tokens 77.6 us on MI355X, 5.3
+// TB/s (a read-only stream reaches 6.3).  Short ones by round trips that wait for one
+// another (lengths, page numbers, K and V, the part written through, its counter, the
+// other parts: 1100 tokens 8.9 us).
 #include <algorithm>
 
 #include "mixers.h"

@@ -6,6 +6,8 @@
 // Bound by memory, so the data is on its way while the angles are made: a thread has 32
 // bytes of the same place in a head (two chunks that turn into one another, or two that
 // are copied) of one or four tokens in registers before the workgroup's angles meet in LDS.
+// MI355X, 8 + 2 heads of 256, 64 turned, with the cache: 8192 tokens 20.7 us, 4.9 TB/s (a
+// copy of 1 GiB 5.2); one token 4.2 us, the host's part of a call.
 #include "mixers.h"
 
 namespace mcv {
