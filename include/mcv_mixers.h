@@ -38,7 +38,7 @@ extern "C" {
  *          of T / B tokens each (T % B == 0).
  * Hv % Hk == 0, Dk 64 or 128, Dv a multiple of 16 up to 256.
  *
- * One token a sequence, or a few, runs the recurrence; long sequences run in
+ * Sequences of a few tokens run the recurrence; long sequences run in
  * chunks of 64 tokens on the matrix cores, for which the call needs a workspace
  * of mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv) bytes, 256-byte aligned,
  * of any content (NULL or too small: the recurrence, however long).  Chunks hold

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     const int b = seq_of_slot(p, slot, t0, t1);
     const int chunk = slot - first_slot(t0, b);
     const int64_t start = t0 + static_cast<int64_t>(chunk) * kC;
-    if (chunk < 0 || start >= t1) return;
+    if (chunk < 0 || start >= t1 || t1 - t0 < p.short_below) return;
     const int n = t1 - start < kC ? static_cast<int>(t1 - start) : kC;
     const int64_t unit = static_cast<int64_t>(local) * p.Hv + h;
 
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
     c0 = c0 < 0 ? 0 : c0;
     c1 = c1 > chunks ? chunks : c1;
     const bool starts = s0 >= a.slot0 && s0 < a.slot0 + a.slots;
-    if (c0 >= c1 && !(chunks == 0 && starts)) return;
+    if ((c0 >= c1 && !(chunks == 0 && starts)) || t1 - t0 < p.short_below) return;
     const int dv0 = slice * 16 * NT;
     const int64_t at = p.state_index ? p.state_index[b] : b;
     if (at < 0 || at >= p.n_states) {

@@ -22,6 +22,7 @@ struct DeltaArgs {
     int T, B, per_seq, Hv, group, Dv;            // per_seq: tokens of every sequence where cu is null
     float scale;
     int normalize;
+    int short_below;                             // sequences of fewer tokens are the recurrence's, the others the chunks'; 0: all one's
 };
 
 // First token and one past the last of sequence b, whatever cu holds.

@@ -19,6 +19,7 @@ namespace mcv {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMixed = 16;                   // more sequences than these: short ones by the recurrence, long ones in chunks
 
 // Sum over the lanes of one lane % C4 (C4 4 .. 32), in all of them: steps of a butterfly as in wave_butterfly.
 template <int C4>
@@ -49,6 +50,7 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
     int t0, t1;
     delta_span(p, b, t0, t1);
     const int col = slice * DVW + 4 * c4;
+    if (p.short_below && t1 - t0 >= p.short_below) return;
     const int64_t at = p.state_index ? p.state_index[b] : b;
     if (at < 0 || at >= p.n_states) {
         if (rg == 0)
@@ -134,7 +136,13 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
 
 // Where the chunked form is faster than 1.1 us a token of the longest sequence.  MI355X, us a pass, recurrence and chunks
 // (16 heads of 128): 1 sequence of 8 tokens 11.7 14.5, of 12 16.3 14.6, of 32 39.0 14.6; 4 of 8 on average 26.4 20.3.
-bool long_enough(int64_t B, int64_t T) { return T >= 10 * B; }
+// Lengths are the device's, and one sequence may have all tokens but a few: 100 of one token and one of 800 take 1083 us
+// by the recurrence and 88 as below.
+constexpr int kShort = 10;
+bool may_be_long(int64_t B, int64_t T) {
+    const int64_t even = kShort * B, skewed = B + 64;
+    return T >= (B == 1 || (B <= kMixed && even < skewed) ? even : skewed);
+}
 
 }  // namespace
 }  // namespace mcv
@@ -144,7 +152,7 @@ using namespace mcv;
 extern "C" {
 
 int64_t mcv_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv) {
-    if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || (Dk != 64 && Dk != 128) || Dv <= 0 || Dv % 16 != 0 || !long_enough(B, T)) return 0;
+    if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || (Dk != 64 && Dk != 128) || Dv <= 0 || Dv % 16 != 0 || !may_be_long(B, T)) return 0;
     return delta_chunk_workspace(B, T, Hk, Hv, Dk);
 }
 
@@ -179,12 +187,14 @@ int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, 
                 static_cast<const int32_t*>(cu_seqlens), static_cast<uint16_t*>(out), q_row, q_head, k_row, k_head,
                 v_row, v_head, g_row, beta_row, n_states, static_cast<int>(T), static_cast<int>(B),
                 static_cast<int>(cu_seqlens ? 0 : T / B), static_cast<int>(Hv), static_cast<int>(Hv / Hk),
-                static_cast<int>(Dv), static_cast<float>(scale), normalize};
-    if (long_enough(B, T) && workspace && workspace_bytes >= delta_chunk_workspace(B, T, Hk, Hv, Dk)) {
+                static_cast<int>(Dv), static_cast<float>(scale), normalize, 0};
+    const bool chunks = (cu_seqlens ? may_be_long(B, T) : T >= kShort * B) && workspace && workspace_bytes >= delta_chunk_workspace(B, T, Hk, Hv, Dk);
+    if (chunks) {
         if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
             return fail(MCV_ERR_INVALID_ARG, "delta_rule: workspace must be 256-byte aligned");
-        return launch_delta_chunk(a, static_cast<int>(Hk), static_cast<int>(Dk), workspace, workspace_bytes,
-                                  static_cast<hipStream_t>(stream));
+        a.short_below = cu_seqlens && B > kMixed ? kShort : 0;
+        rc = launch_delta_chunk(a, static_cast<int>(Hk), static_cast<int>(Dk), workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+        if (rc != MCV_OK || a.short_below == 0) return rc;
     }
     // Columns a workgroup holds: 256 bytes of a row at a time unless that leaves most CUs without work.  MI355X, us a
     // pass of 128 x 128 states, 16 and 64 columns: 16 states 3.8 4.1, 64 5.8 5.2, 256 13.3 9.6, 848 32.7 25.6.

@@ -167,6 +167,27 @@ def test_delta_many_sequences(mcv, cuda, B, longest):
     assert (out[:3] == 7).all() and (out[rows.stop:] == 7).all()
 
 
+@pytest.mark.parametrize("lens", [[1] * 20 + [90] + [1] * 20, [0, 3, 9, 10, 11, 64, 65, 200, 2, 1] * 2, [1, 1, 30], [0] * 17 + [300],
+                                  [5, 0, 0, 0, 0, 0, 80], [2] * 30, [6] * 30, [1] * 16 + [63]])
+def test_delta_short_and_long_together(mcv, cuda, lens):
+    """Sequences of one token beside whole prompts, on either side of every rule's border; a pool with one state absent."""
+    torch = _torch()
+    B = len(lens)
+    q, k, v, g, beta, state = _delta_case(B + sum(lens), lens, 2, 4, 128, 64)
+    a = [x.to(cuda) for x in (q, k, v, g, beta, state)]
+    ref = _delta_ref(q, k, v, g, beta, state, lens, 0.1, True)
+    out, final = mcv.gated_delta_rule(*a, cu_seqlens=_cu(lens, cuda), scale=0.1, normalize=True)
+    _delta_close(out, final, ref)
+    index = torch.arange(B - 1, -1, -1, dtype=torch.int32)
+    index[B // 2] = -1
+    pool = state.flip(0).contiguous().to(cuda)
+    out2, same = mcv.gated_delta_rule(*a[:5], pool, cu_seqlens=_cu(lens, cuda), scale=0.1, normalize=True, state_index=index.to(cuda))
+    on = [b for b in range(B) if b != B // 2]
+    rows = torch.repeat_interleave(torch.arange(B), torch.tensor(lens)).to(cuda)
+    assert same is pool and (pool.flip(0)[on] == final[on]).all() and (pool.flip(0)[B // 2].cpu() == state[B // 2]).all()
+    assert (out2[rows != B // 2] == out[rows != B // 2]).all() and (out2[rows == B // 2] == 0).all()
+
+
 def test_delta_in_several_passes(mcv, cuda):
     """So many heads that the workspace holds a few chunks at a time: sequences across its passes, and between them."""
     lens = [300, 0, 900, 40, 260]
