@@ -6,8 +6,9 @@
 //   u = beta (v - e rk a),  S' = e S + rk k u,  out = scale rq (e b + rk c u)
 // so one pass over S gives everything that S' and out need: out comes from the old
 // state and c instead of a second sum over the new one.  One token is bound by the state's
-// way in and out (53 sequences of 16 states of 128 x 128: 24.8 us on MI355X, 4.5 TB/s, a
-// copy 5.2); more tokens take 1.1 us each, one after the other.
+// way in and out, past the caches (non-temporal: 53 sequences of 16 states of 128 x 128 take
+// 21.5 us on MI355X, 5.2 TB/s, as fast as a copy; 24.8 through them); more tokens take 1.1
+// us each, one after the other.
 //
 // A workgroup holds DVW columns of one state in registers for the whole sequence:
 // 16-byte column chunks over the lanes, R consecutive rows a thread (so its part of
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
     float4_t S[R];
 #pragma unroll
     for (int j = 0; j < R; ++j)
-        S[j] = p.state ? *reinterpret_cast<const float4_t*>(p.state + base + static_cast<int64_t>(j) * p.Dv) : float4_t{0, 0, 0, 0};
+        S[j] = p.state ? __builtin_nontemporal_load(reinterpret_cast<const float4_t*>(p.state + base + static_cast<int64_t>(j) * p.Dv)) : float4_t{0, 0, 0, 0};
     __shared__ float4_t part[2][4][C4][2];
     __shared__ float dots[2][4][3];
     for (int i = t0; i < t1; ++i) {
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
     }
 #pragma unroll
     for (int j = 0; j < R; ++j)
-        *reinterpret_cast<float4_t*>(p.state_out + base + static_cast<int64_t>(j) * p.Dv) = S[j];
+        __builtin_nontemporal_store(S[j], reinterpret_cast<float4_t*>(p.state_out + base + static_cast<int64_t>(j) * p.Dv));
 }
 
 // Where the chunked form is faster than 1.1 us a token of the longest sequence.  MI355X, us a pass, recurrence and chunks
