@@ -198,7 +198,7 @@ int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, 
         if (rc != MCV_OK || a.short_below == 0) return rc;
     }
     // Columns a workgroup holds: 256 bytes of a row at a time unless that leaves most CUs without work.  MI355X, us a
-    // pass of 128 x 128 states, 16 and 64 columns: 16 states 3.8 4.1, 64 5.8 5.2, 256 13.3 9.6, 848 32.7 25.6.
+    // pass of 128 x 128 states, 16 and 64 columns: 16 states 4.2 4.3, 64 5.1 5.2, 256 14.3 7.5, 848 35.5 22.0.
     const int width = Dv % 64 == 0 && B * Hv * (Dv / 64) >= 96 ? 64 : 16;
     const int64_t grid = B * Hv * (Dv / width);
     if (grid > 0x7fffffff) return fail(MCV_ERR_SHAPE, "delta_rule: too many states");

@@ -24,7 +24,7 @@
 // parts joins them in order, and where there are more than kFan the last of those joins
 // the joined, so the bits do not depend on who is last and nobody waits.
 //
-// Long caches are bound by HBM: 8 heads on 2 of 256, 200000 tokens 77.6 us on MI355X, 5.3
+// Long caches are bound by HBM: 8 heads on 2 of 256, 200000 tokens 68.8 us on MI355X, 6.0
 // TB/s (a read-only stream reaches 6.3).  Short ones by round trips that wait for one
 // another (lengths, page numbers, K and V, the part written through, its counter, the
 // other parts: 1100 tokens 8.9 us).
@@ -155,8 +155,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
             const auto whole_steps = [](int n) { return (n + W - 1) / W * W; };
             per = whole_steps((total + p.split - 1) / p.split);
             // Few (sequence, cache head)s: as many parts as CUs at most, so that none has two while others have one.
-            // MI355X, us of 256, 512 and 768 workgroups: 1 x 200000 77 81 87, 1 x 25000 D 128 26 29 30; where there
-            // are many, small parts even out better than one each: 41 x 4096 ragged 37 30 30, 8 x 20000 D 128 64 53 55.
+            // MI355X, us of 256, 512 and 768 workgroups: 1 x 200000 70 72 79, 1 x 25000 D 128 24 27 28; where there
+            // are many, small parts even out better than one each: 41 x 4096 ragged 35 28 28, 8 x 20000 D 128 59 48 51.
             if (p.B * per_seq <= kCus / 8 && total > kCus * W) {
                 per = whole_steps((total + kCus - 1) / kCus);
                 for (int i = 0; i < 4; ++i) {
@@ -461,11 +461,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
 }
 
 // Workgroups to cut the `groups` (sequence, cache head, head tile)s of up to `most` tokens for: what the chip
-// holds at once.  0: nothing to cut.
-int choose_workers(int64_t groups, int64_t most, int64_t D) {
+// holds at once with D = 256, two a CU.  With D = 128 it holds three; MI355X, us of 512, 640 and 768: 16 x 2000 ragged
+// 15.7 15.6 16.2, 8 x 20000 48 51 51, 41 x 4096 (32 heads on 8) 55 49 51, 5 x 60000 48 53 50, 64 x 1000 25.9 25.9 26.4.
+// 0: nothing to cut.
+int choose_workers(int64_t groups, int64_t most) {
     const int64_t tiles = ceil_div(most, kTile);
     if (most <= 4 * kTile || groups * tiles > 0x3fffffff) return 0;
-    return static_cast<int>(std::min<int64_t>(D == 256 ? 512 : 768, groups * ceil_div(tiles, 4)));
+    return static_cast<int>(std::min<int64_t>(512, groups * ceil_div(tiles, 4)));
 }
 int64_t split_bytes(int64_t workers, int64_t rows, int64_t D) {
     return workers == 0 ? 0 : kCounterBytes + (2 * (workers + 2) + 2 * ceil_div(workers + 2, kFan)) * part_bytes(static_cast<int>(rows), static_cast<int>(D));
@@ -482,7 +484,7 @@ int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || B > 0x7fffffff / Hq || D <= 0 || max_seq_len < 0) return 0;
     const int64_t group = Hq / Hkv, groups = B * Hkv * ceil_div(group, kHeads);
     const int64_t most = max_seq_len < kMaxLen ? max_seq_len : kMaxLen;
-    return split_bytes(choose_workers(groups, most, D), group < kHeads ? group : kHeads, D);
+    return split_bytes(choose_workers(groups, most), group < kHeads ? group : kHeads, D);
 }
 
 int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
@@ -518,7 +520,7 @@ int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void
     const int64_t most = max_seq_len < held ? max_seq_len : held;
     const int64_t group = Hq / Hkv, htiles = ceil_div(group, kHeads), groups = B * Hkv * htiles;
     const int64_t rows = group < kHeads ? group : kHeads;
-    int workers = choose_workers(groups, most, D);
+    int workers = choose_workers(groups, most);
     if (workers && (!workspace || workspace_bytes < split_bytes(workers, rows, D))) workers = 0;
     if (workers && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "paged_attention: workspace must be 256-byte aligned");
