@@ -45,6 +45,12 @@ constexpr int64_t kMaxLen = int64_t(1) << 30;   // tokens of one sequence
 // 69.3 77.9, 41 x 4096 27.9 29.8, 1 x 30000 20.4 21.6, 1 x 1100 10.4 9.7 (9.0 both ways where they may be).
 constexpr int kOnce = 2;
 constexpr float kLog2e = 1.44269504088896340736f;
+// The largest weight, of 2^(s - m) at most one.  As an operand a weight is two fp16 parts, the second what the first,
+// cut off, leaves: off by 2^-21 of the weight, or 2^-39 of the largest.  (One part under a largest weight of one is
+// nothing from 2^-25 on, while l counts it: one token far above 4096 others, its v zero, 25 % off.)  l and the sums
+// of v carry the factor alike.  The second part is never of the other sign, nor zero beside a first that is not: an
+// infinite v stays infinite.
+constexpr float kTop = 32768.f;
 
 struct AttnArgs {
     const uint16_t* q;
@@ -74,6 +80,7 @@ __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);       // lane 31 to the upper half
     return v;
 }
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max4(float v) {          // over the four lanes of one column
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -311,15 +318,26 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
                 m = mx;
             }
             const float base = m == -INFINITY ? 0.f : m;         // nothing so far: every weight 2^-inf
-            half8_t w;
+            float e[8];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = exp2_of(s[x][r] - base);
-                    l += e;
-                    w[4 * x + r] = static_cast<_Float16>(e);     // the product's operand: one rounding of each weight
+                    e[4 * x + r] = exp2_of(s[x][r] - base) * kTop;
+                    l += e[4 * x + r];
                 }
+            uint4 w, w_lo;
+            auto parts_of = [&](int i, uint32_t& hi, uint32_t& lo) {
+                const auto h = __builtin_amdgcn_cvt_pkrtz(e[i], e[i + 1]);
+                const half2_t r = {static_cast<_Float16>(e[i] - static_cast<float>(h[0])), static_cast<_Float16>(e[i + 1] - static_cast<float>(h[1]))};
+                hi = __builtin_bit_cast(uint32_t, h);
+                const ushort2_t least = __builtin_elementwise_min(__builtin_bit_cast(ushort2_t, h), ushort2_t{1, 1});
+                lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, r), least));
+            };
+            parts_of(0, w.x, w_lo.x);
+            parts_of(2, w.y, w_lo.y);
+            parts_of(4, w.z, w_lo.z);
+            parts_of(6, w.w, w_lo.w);
             if (!whole)
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
@@ -338,7 +356,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
                     a.y = __builtin_amdgcn_perm(vr[3][n][d / 2], vr[2][n][d / 2], pick);
                     a.z = __builtin_amdgcn_perm(vr[5][n][d / 2], vr[4][n][d / 2], pick);
                     a.w = __builtin_amdgcn_perm(vr[7][n][d / 2], vr[6][n][d / 2], pick);
-                    acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w, acc[n][d], 0, 0, 0);
+                    acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, w), acc[n][d], 0, 0, 0);
+                    acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, w_lo), acc[n][d], 0, 0, 0);
                 }
         }
         load_v(npage, nrow);
