@@ -35,12 +35,22 @@ __device__ __forceinline__ void turn(float a, float b, float c, float s, uint16_
     y = f2h(b * c + a * s);
 }
 
-// Angle i of token t, in turns of less than a half.
+// Angle i of token t: its quarter turns and what is left of it, an eighth of a turn at most, are found in 64 bits, so
+// that the sine and the cosine are both within 32-bit roundings of themselves.  (In 32 bits a turn next to a half or a
+// quarter has lost the last bits of the smaller of the two.)
 __device__ __forceinline__ void angle_of(const RotaryArgs& p, int t, int i, float& c, float& s) {
     int a = p.axis[i];
     a = a < 0 ? 0 : a >= p.axes ? p.axes - 1 : a;
-    const double x = static_cast<double>(p.pos[a * p.pos_axis + t * p.pos_token]) * p.freq[i] * 0.15915494309189533577;
-    sincospif(2.0f * static_cast<float>(x - rint(x)), &s, &c);
+    double x = static_cast<double>(p.pos[a * p.pos_axis + t * p.pos_token]) * p.freq[i] * 0.15915494309189533577;
+    x -= rint(x);
+    const double quarter = rint(4.0 * x);
+    const int n = static_cast<int>(quarter);
+    float sy, cy;
+    sincospif(2.0f * static_cast<float>(fma(quarter, -0.25, x)), &sy, &cy);
+    s = n & 1 ? cy : sy;
+    c = n & 1 ? sy : cy;
+    s = n & 2 ? -s : s;
+    c = (n + 1) & 2 ? -c : c;
 }
 
 // Where token t's k and v go: page and row, or nowhere.
