@@ -40,3 +40,15 @@ def test_rotary_long(mcv, cuda, T, Hq, Hkv, D, rot):
     value = dev[2].clone()
     mcv.rotary_axes(*dev[:2], *where, q_out=dev[0], k_out=dev[1])              # in place
     assert (dev[0] == plain[0]).all() and (dev[1] == plain[1]).all() and (dev[2] == value).all()
+
+
+@pytest.mark.parametrize("long,others,Hq,Hkv,D", [(200000, 39, 2, 1, 64), (70001, 20, 4, 2, 128), (150000, 65, 3, 1, 64)])
+def test_attention_joined_in_rounds(mcv, cuda, long, others, Hq, Hkv, D):
+    """More than 256 parts of one sequence among many that are short or empty."""
+    lens = [i % 3 * 20 for i in range(others)]
+    lens.insert(others // 2, long)
+    q, k, v, table, n, kv = _attn_case(long, lens, Hq, Hkv, D, 64)
+    a = [x.to(cuda) for x in (q, k, v, table, n)]
+    got = mcv.paged_attention_decode(*a)
+    _attn_close(got, _attn_ref(q, kv, Hkv, D ** -0.5))
+    assert (mcv.paged_attention_decode(*a) == got).all()
