@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -100,6 +101,12 @@ void same_device(const char* who, const at::Tensor& t, std::initializer_list<con
     for (const at::Tensor* o : others)
         if (o && o->device() != t.device()) refuse("%s: tensors on %s and %s", who, t.device().str().c_str(), o->device().str().c_str());
 }
+// Kernels read what they are given as device memory.  Asked last, when all tensors are known to be on t's device;
+// the device is then the current one until the call ends, its stream and its memory among them.
+c10::DeviceGuard on_gpu(const char* who, const at::Tensor& t) {
+    if (!t.is_cuda()) refuse("%s: tensors must be on a GPU, got %s", who, t.device().str().c_str());
+    return c10::DeviceGuard(t.device());
+}
 void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
     return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
@@ -107,8 +114,8 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& l
 PyObject* wrapped(const at::Tensor& t) { return THPVariable_Wrap(t); }
 
 // The handle of `stream` (a torch stream, or None: the current one).
-mcv_stream_t handle(PyObject* stream, const at::Tensor& t) {
-    if (stream == Py_None) return t.is_cuda() ? static_cast<mcv_stream_t>(c10::hip::getCurrentHIPStream().stream()) : nullptr;
+mcv_stream_t handle(PyObject* stream) {
+    if (stream == Py_None) return static_cast<mcv_stream_t>(c10::hip::getCurrentHIPStream().stream());
     PyObject* h = PyObject_GetAttrString(stream, "cuda_stream");
     if (!h) throw Failed{};
     void* p = PyLong_AsVoidPtr(h);
@@ -121,7 +128,6 @@ mcv_stream_t handle(PyObject* stream, const at::Tensor& t) {
 // stream use it too, so its first bytes are counters and stay zero.  Held there, by device, stream and
 // size; a reference of that dict is all that is looked up here.
 void* workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
-    if (!t.is_cuda()) return nullptr;
     int64_t size = g_workspace_min;
     if (bytes > size)
         for (size = 1; size < bytes;) size *= 2;
@@ -180,9 +186,10 @@ PyObject* delta(PyObject* const* a) {
     if (given && (given->scalar_type() != at::kHalf || given->sizes() != v.sizes() || !given->is_contiguous()))
         refuse("%s: out must be contiguous fp16 %s", who, shape(v).c_str());
     same_device(who, q, {&k, &v, &g, &beta, state, state_given, index, cu, given});
+    const auto device = on_gpu(who, q);
     out = given ? *given : fresh(v.sizes(), at::kHalf, q);
     state_out = state_given ? *state_given : fresh({B, Hv, Dk, Dv}, at::kFloat, q);
-    const mcv_stream_t h = handle(a[14], q);
+    const mcv_stream_t h = handle(a[14]);
     const int64_t bytes = mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv);
     uint8_t* ws = bytes ? static_cast<uint8_t*>(workspace(g_counter_bytes + bytes, q, a[14], h)) : nullptr;
     check(mcv_delta_rule(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, g.data_ptr(), g.stride(0), beta.data_ptr(),
@@ -215,8 +222,9 @@ PyObject* paged(PyObject* const* a) {
         most = PyLong_AsLongLong(a[6]);
         if (most == -1 && PyErr_Occurred()) throw Failed{};
     }
+    const auto device = on_gpu(who, q);
     const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q);
-    const mcv_stream_t h = handle(a[8], q);
+    const mcv_stream_t h = handle(a[8]);
     const int64_t bytes = mcv_paged_attention_workspace_bytes(B, Hq, Hkv, D, most);
     void* ws = bytes ? workspace(bytes, q, a[8], h) : nullptr;
     check(mcv_paged_attention(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
@@ -246,12 +254,15 @@ PyObject* rotary(PyObject* const* a, bool cached) {
         const at::Tensor* k_given = maybe(who, "k_out", a[6]);
         if (k_given && k_given->sizes() != k.sizes()) refuse("%s: k_out must be %s", who, shape(k).c_str());
         same_device(who, q, {k_given});
+        for (const at::Tensor* t : {given, k_given})
+            if (t) heads(who, t == given ? "q_out" : "k_out", *t, T);
+        const auto device = on_gpu(who, q);
         const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q), k_out = k_given ? *k_given : fresh(k.sizes(), at::kHalf, q);
         const Heads qo = heads(who, "q_out", q_out, T), ko = heads(who, "k_out", k_out, T);
         if (T)
             check(mcv_rotary_axes(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, pos.data_ptr(), pos.stride(0), pos.stride(1), pos.size(0),
                                   freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row, qo.head, ko.p, ko.row, ko.head,
-                                  handle(a[7], q)),
+                                  handle(a[7])),
                   who);
         return Py_BuildValue("(NN)", wrapped(q_out), wrapped(k_out));
     }
@@ -264,13 +275,15 @@ PyObject* rotary(PyObject* const* a, bool cached) {
     const Cache kca = cache(who, "k_cache", kc, kc, Hkv, D), vca = cache(who, "v_cache", vc, kc, Hkv, D);
     same_device(who, q, {&v, &kc, &vc, &slots});
     const Heads va = heads(who, "v", v, T);
+    if (given) heads(who, "q_out", *given, T);
+    const auto device = on_gpu(who, q);
     const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q);
     const Heads qo = heads(who, "q_out", q_out, T);
     if (T)
         check(mcv_rotary_axes_cached(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, pos.data_ptr(), pos.stride(0),
                                      pos.stride(1), pos.size(0), freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row,
                                      qo.head, kca.p, kca.page, kca.token, kca.head, vca.p, vca.page, vca.token, vca.head, kc.size(0),
-                                     kc.size(1), slots.data_ptr(), handle(a[10], q)),
+                                     kc.size(1), slots.data_ptr(), handle(a[10])),
               who);
     return wrapped(q_out);
 }
