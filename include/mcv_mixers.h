@@ -44,7 +44,9 @@ extern "C" {
  * of any content (NULL or too small: the recurrence, however long).  Chunks hold
  * the state in two fp16 parts scaled by the largest |v| and |state| of the
  * sequence: a state that grows past 4096 times that overflows, which a stable
- * rule (beta |k|^2 <= 2) does not do. */
+ * rule (beta |k|^2 <= 2) does not do.  An infinity or NaN in q, k, v, a gate or a
+ * state reaches what it reaches by the formulas, of its own token and later ones;
+ * from there on the chunks may have NaN where the formulas have an infinity. */
 int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                    const void* v, int64_t v_row, int64_t v_head, const void* g, int64_t g_row, const void* beta,
                    int64_t beta_row, const void* state, void* state_out, const void* state_index, int64_t n_states,

@@ -25,6 +25,11 @@
 // two that brings the largest to 8 .. 16, so that they may grow 4096-fold and a part's
 // last bit is 2^-25 at worst.
 //
+// Order in time.  The products T X and P U run over whole tiles, zeros above the diagonal included, and a zero times an
+// infinity or NaN of a later token would be NaN.  So T holds no rows of tokens whose k or gates are not finite (X has
+// NaN there instead), a product that comes out not finite is made again without what is not, NaN put in from the
+// first such token of its column on, and the scale goes by finite values alone.
+//
 // Operand order.  v_mfma_f32_16x16x32_f16 leaves lane (c, j) = (lane % 16, lane / 16) column c
 // and rows 4j .. 4j + 3 of a 16 x 16 tile; as an operand it wants row (or column) c and eight
 // of the 32 summed-over indexes, which may be any eight as long as both operands agree.
@@ -85,6 +90,7 @@ __device__ __forceinline__ int seq_of_slot(const DeltaArgs& p, int slot, int& t0
 
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef float float8_t __attribute__((ext_vector_type(8)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ half8_t as_h8(uint4 v) { return __builtin_bit_cast(half8_t, v); }
 __device__ __forceinline__ uint4 as_u4(half8_t v) { return __builtin_bit_cast(uint4, v); }
@@ -255,18 +261,22 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
         bet[lane] = lane < n ? gate : 0.f;
     }
     if (w < 2) {                                 // the largest |v|, for the scan's scale; these have fewer products
-        half2_t most = {0, 0};                   // (a maximum with NaN is the other)
+        // (of finite ones: as whole numbers from 0x400 on, where what is not finite has wrapped to less)
+        ushort2_t most = {0, 0};
         for (int from = 0;;) {
 #pragma unroll
             for (int i = 0; i < VT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    most = __builtin_elementwise_max(most, as_h2((e == 0 ? vx[i].x : e == 1 ? vx[i].y : e == 2 ? vx[i].z : vx[i].w) & 0x7fff7fffu));
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = e == 0 ? vx[i].x : e == 1 ? vx[i].y : e == 2 ? vx[i].z : vx[i].w;
+                    most = __builtin_elementwise_max(most, __builtin_bit_cast(ushort2_t, ((x & 0x7fff7fffu) + 0x04000400u) & 0x7fff7fffu));
+                }
             from += 128;
             if (from >= p.Dv) break;
             load_v(from);
         }
-        const float big = wave_butterfly(fmaxf(static_cast<float>(most[0]), static_cast<float>(most[1])), [](float x, float y) { return fmaxf(x, y); });
+        const int top = most[0] > most[1] ? most[0] : most[1];
+        const float big = wave_butterfly(top < 0x400 ? 0.f : h2f(static_cast<uint16_t>(top - 0x400)), [](float x, float y) { return fmaxf(x, y); });
         if (lane == 0) sc[kVmax + w] = big;
     }
     __syncthreads();
@@ -278,6 +288,9 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
         for (int e = 0; e < 8; ++e)
             *reinterpret_cast<half2_t*>(kt + turned(8 * ch + e, token_block(t)) + token_in_block(t)) = half2_t{x[e], y[e]};
     }
+    // The first token whose k or gates (g's running sum) are not finite.
+    const unsigned long long odd = __ballot(!(fabsf(kk[lane]) < INFINITY && fabsf(gh[lane]) < INFINITY && fabsf(bet[lane]) < INFINITY));
+    const int clean = odd ? __builtin_ctzll(odd) : kC;
     {
         // Norm factors within a last bit: the same ones enter T, P and the scan's scalars.
         const float k2 = kk[lane], q2 = qq[lane], g_hi = gh[lane], g_lo = gl[lane];
@@ -291,7 +304,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
             const float b = bet[lane];
             kpow[lane] = static_cast<_Float16>(p.normalize ? __uint_as_float(bits & 0x7f800000u) : 1.0f);
             rkn[lane] = rk;
-            sc[kBet + lane] = b;
+            sc[kBet + lane] = lane < clean ? b : NAN;
             sc[kBr + lane] = b * rk * eg;
             sc[kEf + lane] = to_end * (p.normalize ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 1.0f);
             if (lane == kC - 1) sc[kKeep] = eg;
@@ -338,6 +351,10 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
             }
         }
     }
+    if (clean < kC)
+        for (int x = 0; x <= w; ++x)
+            for (int r = 0; r < 4; ++r)
+                if (16 * w + 4 * j + r >= clean) tri[16 * w + 4 * j + r][16 * x + c] = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         if (2 * s > w) continue;
@@ -478,7 +495,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
                     S[m][x][r] = src ? src[at_state(m, r) + x] : 0.f;
-                    big = fmaxf(big, fabsf(S[m][x][r]));
+                    big = fmaxf(big, fabsf(S[m][x][r]) < INFINITY ? fabsf(S[m][x][r]) : 0.f);
                 }
     }
     auto store_state = [&](float by) {
@@ -506,7 +523,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = fmaxf(most, maxes[i]);
-        int ex = most > 0.f && most < INFINITY ? 3 - ilogbf(most) : 0;
+        int ex = most > 0.f ? 3 - ilogbf(most) : 0;
         ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
         up = ldexpf(1.0f, ex);
         down = ldexpf(1.0f, -ex);
@@ -515,6 +532,22 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
     const int n_last = t1 - (first + static_cast<int64_t>(count - 1) * kC) < kC
                            ? static_cast<int>(t1 - (first + static_cast<int64_t>(count - 1) * kC)) : kC;
     auto row = [&](int t, int n) { return static_cast<int64_t>(t < n ? t : n - 1); };
+
+    // An operand of 64 tokens (two steps, two parts) and 16 columns: what is not finite becomes zero; the first such
+    // token of the lane's column, kC if there is none.
+    auto first_of_columns = [&](half8_t (&g)[2][2]) {
+        int bad = kC;
+#pragma unroll
+        for (int k = 1; k >= 0; --k)
+#pragma unroll
+            for (int e = 7; e >= 0; --e)
+                if (!(fabsf(static_cast<float>(g[0][k][e])) < INFINITY)) {
+                    bad = 32 * k + (e < 4 ? 0 : 12) + 4 * j + e;
+                    g[0][k][e] = g[1][k][e] = 0;
+                }
+        bad = min(bad, __shfl_xor(bad, 16));
+        return min(bad, __shfl_xor(bad, 32));
+    };
 
     if (wave < 4) {
         typedef _Float16 vrow __attribute__((ext_vector_type(NT)));
@@ -650,6 +683,26 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
                         for (int part = 0; part < 2; ++part) g[part][k] = as_h8(*reinterpret_cast<const uint4*>(&xf[part][x][k][lane][0]));
                 };
+                // U of column x's tokens before the first X that is not finite, NaN from it on, for the outputs.
+                auto in_order = [&](int x) {
+                    read_x(x);
+                    const int bad = first_of_columns(g);
+                    float4_t u = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if (2 * k > w) continue;
+                        u = mfma16(s.t[k][0], g[0][k], u);
+                        u = mfma16(s.t[k][0], g[1][k], u);
+                        u = mfma16(s.t[k][1], g[0][k], u);
+                    }
+                    half4_t hi, lo;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) u[r] = 16 * w + 4 * j + r >= bad ? NAN : apart(u[r]);
+                    split<4>(u, hi, lo);
+                    uf[0][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, hi);
+                    uf[1][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, lo);
+                };
+                float all = 0.f;
                 read_x(0);
                 lds_first();
                 load_k(s, ahead);
@@ -667,6 +720,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                         z = mfma16(s.t[k][1], g[0][k], z);
                     }
                     u += v + z;
+                    all += (u[0] + u[1]) + (u[2] + u[3]);
                     float4_t eu;
                     half4_t part[4];
 #pragma unroll
@@ -678,6 +732,8 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) uf[e][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, part[e]);
                 }
+                if (__any(!(fabsf(all) < INFINITY)))     // (the state's own parts stay: it has NaN of any token of the chunk)
+                    for (int x = 0; x < NT; ++x) in_order(x);
                 lds_barrier();                   // U is there, S has been read
                 auto read_u = [&](int x) {
 #pragma unroll
@@ -738,9 +794,31 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
         }
         agree_on_scale();
         float4_t o[NT], ol[NT];                  // e^G Q S of a chunk: rows dv, column token
+        // P U of column x, U's first that is not finite and all after it NaN: rows dv, column token
+        auto in_order = [&](const Stage& s, int x) {
+            half8_t g[2][2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int part = 0; part < 2; ++part) g[part][k] = as_h8(*reinterpret_cast<const uint4*>(&uf[part][x][k][lane][0]));
+            const int bad = first_of_columns(g);
+            float4_t y = (o[x] + ol[x]) * s.eq;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (2 * k > w) continue;
+                y = mfma16(g[0][k], s.pf[k][0], y);
+                y = mfma16(g[1][k], s.pf[k][0], y);
+                y = mfma16(g[0][k], s.pf[k][1], y);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (16 * w + c >= __shfl(bad, 4 * j + e)) y[e] = NAN;
+            return y;
+        };
         auto finish = [&](const Stage& s, int i) {
             const int64_t t = first + static_cast<int64_t>(i) * kC + 16 * w + c;
-            uint16_t r[4 * NT];
+            float4_t sum[NT];
+            float all = 0.f;
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 float4_t y = (o[x] + ol[x]) * s.eq, z = {0, 0, 0, 0}, v = {0, 0, 0, 0};
@@ -753,16 +831,29 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                     z = mfma16(lo, s.pf[k][0], z);
                     v = mfma16(hi, s.pf[k][1], v);
                 }
-                const float osc = s.osc * down;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) r[NT * e + x] = f2h((y[e] + (z[e] + v[e])) * osc);
+                sum[x] = y + (z + v);
+                all += (sum[x][0] + sum[x][1]) + (sum[x][2] + sum[x][3]);
             }
-            if (t < t1) {
-                uint2* at_out = reinterpret_cast<uint2*>(p.out + (t * p.Hv + h) * p.Dv + dv0 + 4 * NT * j);
+            auto put = [&]() {
+                const float osc = s.osc * down;
+                uint16_t r[4 * NT];
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
-                    at_out[x] = make_uint2(r[4 * x] | (static_cast<uint32_t>(r[4 * x + 1]) << 16),
-                                           r[4 * x + 2] | (static_cast<uint32_t>(r[4 * x + 3]) << 16));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[NT * e + x] = f2h(sum[x][e] * osc);
+                if (t < t1) {
+                    uint2* at_out = reinterpret_cast<uint2*>(p.out + (t * p.Hv + h) * p.Dv + dv0 + 4 * NT * j);
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+                        at_out[x] = make_uint2(r[4 * x] | (static_cast<uint32_t>(r[4 * x + 1]) << 16),
+                                               r[4 * x + 2] | (static_cast<uint32_t>(r[4 * x + 3]) << 16));
+                }
+            };
+            put();                               // (looked at after it: before, 2.2 us more over 8192 tokens)
+            if (__any(!(fabsf(all) < INFINITY))) {
+#pragma unroll
+                for (int x = 0; x < NT; ++x) sum[x] = in_order(s, x);
+                put();
             }
         };
         for (int i0 = 0; i0 < count; i0 += PD)
