@@ -498,14 +498,19 @@ def gemm_workspace(nbytes: int, device, stream=None):
     ws = _GEMM_WS.get(key)
     if ws is not None:
         return ws
+    return _new_workspace(_GEMM_WS, _GEMM_WS_CAPTURE, key, key[2], _GEMM_COUNTER_BYTES, dev, handle, stream)
+
+
+def _new_workspace(held: dict, of_graphs: dict, key, zeroed: int, zeroed_in_graph: int, dev, handle: int, stream):
+    """The workspace of `key`, (device, stream, bytes), that is not held yet: kept there, or for the graph
+    that is being captured on the stream."""
     capture = lib().mcv_stream_capture_id(handle)
     if capture == 0:
-        return _GEMM_WS.setdefault(key, _workspace_on(key[2], key[2], dev, handle, stream))
-    held = _GEMM_WS_CAPTURE.get(key)
-    if held is None or held[0] != capture:
-        held = (capture, _workspace_on(key[2], _GEMM_COUNTER_BYTES, dev, handle, stream))
-        _GEMM_WS_CAPTURE[key] = held
-    return held[1]
+        return held.setdefault(key, _workspace_on(key[2], zeroed, dev, handle, stream))
+    own = of_graphs.get(key)
+    if own is None or own[0] != capture:
+        own = of_graphs[key] = (capture, _workspace_on(key[2], zeroed_in_graph, dev, handle, stream))
+    return own[1]
 
 
 def _workspace_on(nbytes: int, zeroed: int, dev, handle: int, stream):

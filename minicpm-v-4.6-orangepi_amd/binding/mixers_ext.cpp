@@ -21,8 +21,12 @@
 
 namespace {
 
-PyObject *g_error, *g_workspace, *g_held;        // McvError, gemm_workspace, its dict of buffers
-int64_t g_workspace_min, g_counter_bytes;
+PyObject* g_error;                               // McvError
+// A function of mixers.py or the package that makes workspaces, the dict of those it keeps, by device, stream and size.
+struct Workspaces {
+    PyObject *make, *held;
+} g_gemm, g_delta;
+int64_t g_gemm_least, g_delta_sizes[2];
 
 struct Failed {};                                // a Python error is set
 
@@ -124,26 +128,32 @@ mcv_stream_t handle(PyObject* stream) {
     return static_cast<mcv_stream_t>(p);
 }
 
-// gemm_workspace's buffer of the next power of two: few sizes, whatever the calls'.  Other calls on the
-// stream use it too, so its first bytes are counters and stay zero.  Held there, by device, stream and
-// size; a reference of that dict is all that is looked up here.
-void* workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
-    int64_t size = g_workspace_min;
-    if (bytes > size)
-        for (size = 1; size < bytes;) size *= 2;
+// A buffer of `size` bytes.  Held ones are looked up here, a reference of that dict is all it takes.
+void* workspace(const Workspaces& from, int64_t size, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
     PyObject* key = Py_BuildValue("(iNL)", int(t.device().index()), PyLong_FromVoidPtr(h), (long long)size);
     if (!key) throw Failed{};
-    PyObject* ws = PyDict_GetItemWithError(g_held, key);
+    PyObject* ws = PyDict_GetItemWithError(from.held, key);
     Py_DECREF(key);
     if (ws) return THPVariable_Unpack(ws).data_ptr();
     if (PyErr_Occurred()) throw Failed{};
     PyObject* device = PyUnicode_FromString(t.device().str().c_str());
-    PyObject* made = device ? PyObject_CallFunction(g_workspace, "LOO", (long long)size, device, stream) : nullptr;
+    PyObject* made = device ? PyObject_CallFunction(from.make, "LOO", (long long)size, device, stream) : nullptr;
     Py_XDECREF(device);
     if (!made) throw Failed{};
     void* p = THPVariable_Unpack(made).data_ptr();
-    Py_DECREF(made);                             // gemm_workspace keeps it
+    Py_DECREF(made);                             // (it is kept where it was made)
     return p;
+}
+// gemm_workspace's buffer of the next power of two: few sizes, whatever the calls'.  Other calls on the
+// stream use it too, so its first bytes are counters and stay zero.
+void* gemm_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
+    int64_t size = g_gemm_least;
+    if (bytes > size)
+        for (size = 1; size < bytes;) size *= 2;
+    return workspace(g_gemm, size, t, stream, h);
+}
+void* delta_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
+    return workspace(g_delta, bytes <= g_delta_sizes[0] ? g_delta_sizes[0] : bytes <= g_delta_sizes[1] ? g_delta_sizes[1] : bytes, t, stream, h);
 }
 
 // (who, q, k, v, g, beta, state, cu, step, scale, normalize, state_index, out, state_out, stream) -> (out, state_out)
@@ -191,11 +201,11 @@ PyObject* delta(PyObject* const* a) {
     state_out = state_given ? *state_given : fresh({B, Hv, Dk, Dv}, at::kFloat, q);
     const mcv_stream_t h = handle(a[14]);
     const int64_t bytes = mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv);
-    uint8_t* ws = bytes ? static_cast<uint8_t*>(workspace(g_counter_bytes + bytes, q, a[14], h)) : nullptr;
+    void* ws = bytes ? delta_workspace(bytes, q, a[14], h) : nullptr;
     check(mcv_delta_rule(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, g.data_ptr(), g.stride(0), beta.data_ptr(),
                          beta.stride(0), ptr(state), state_out.data_ptr(), ptr(index), n_states, ptr(cu), B, T, Hk, Hv, Dk, Dv,
                          number(a[9], 1.0 / std::sqrt(static_cast<double>(Dk))), truth(a[10]), out.data_ptr(),
-                         ws ? ws + g_counter_bytes : nullptr, ws ? bytes : 0, h),
+                         ws, ws ? bytes : 0, h),
           who);
     return Py_BuildValue("(NN)", wrapped(out), wrapped(state_out));
 }
@@ -226,7 +236,7 @@ PyObject* paged(PyObject* const* a) {
     const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q);
     const mcv_stream_t h = handle(a[8]);
     const int64_t bytes = mcv_paged_attention_workspace_bytes(B, Hq, Hkv, D, most);
-    void* ws = bytes ? workspace(bytes, q, a[8], h) : nullptr;
+    void* ws = bytes ? gemm_workspace(bytes, q, a[8], h) : nullptr;
     check(mcv_paged_attention(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
                               table.data_ptr(), table.stride(0), table.size(1), lens.data_ptr(), most, B, Hq, Hkv, D,
                               number(a[5], 1.0 / std::sqrt(static_cast<double>(D))), out.data_ptr(), ws, ws ? bytes : 0, h),
@@ -306,19 +316,21 @@ PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 8, [&] { return rotary(a, false); }); }
 PyObject* py_rotary_cached(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 11, [&] { return rotary(a, true); }); }
 
-// (McvError, gemm_workspace, its buffers by (device, stream, bytes), the smallest's bytes, the counters' bytes)
+// (McvError, gemm_workspace, the buffers it keeps, the smallest's bytes, delta_workspace, its, its two sizes)
 PyObject* py_bind(PyObject*, PyObject* args) {
-    PyObject *error, *make, *held;
-    long long least, counters;
-    if (!PyArg_ParseTuple(args, "OOO!LL", &error, &make, &PyDict_Type, &held, &least, &counters)) return nullptr;
-    Py_INCREF(error);
-    Py_INCREF(make);
-    Py_INCREF(held);
+    PyObject* error;
+    Workspaces gemm, delta;
+    long long least, small, large;
+    if (!PyArg_ParseTuple(args, "OOO!LOO!LL", &error, &gemm.make, &PyDict_Type, &gemm.held, &least, &delta.make, &PyDict_Type, &delta.held,
+                          &small, &large))
+        return nullptr;
+    for (PyObject* o : {error, gemm.make, gemm.held, delta.make, delta.held}) Py_INCREF(o);
     g_error = error;
-    g_workspace = make;
-    g_held = held;
-    g_workspace_min = least;
-    g_counter_bytes = counters;
+    g_gemm = gemm;
+    g_delta = delta;
+    g_gemm_least = least;
+    g_delta_sizes[0] = small;
+    g_delta_sizes[1] = large;
     Py_RETURN_NONE;
 }
 

@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import importlib.util
 
-from . import _GEMM_COUNTER_BYTES, _GEMM_WS, GEMM_WORKSPACE_BYTES, PKG_DIR, McvError, _torch, gemm_workspace, lib
+from . import _GEMM_WS, GEMM_WORKSPACE_BYTES, PKG_DIR, McvError, _new_workspace, _stream, _torch, gemm_workspace, lib
 
 # A call's checks and its launch are native (binding/mixers_ext.cpp): the kernels of one
 # decoded token take 3 to 5 us, and a call written here with ctypes took 9 to 12.  MI355X,
@@ -31,9 +31,31 @@ def binding():
         spec = importlib.util.spec_from_file_location("_mcv_mixers", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        mod.bind(McvError, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, _GEMM_COUNTER_BYTES)
+        mod.bind(McvError, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES)
         _BINDING = mod
     return _BINDING
+
+
+# The delta rule's workspace comes in two sizes, for some 800 tokens of 16 heads of 128 and for all that a pass takes of
+# any length, so that a stream holds one of each at most.  Its two launches read what the first has written, and calls
+# that let other threads run launch on the GEMM's: it has buffers of its own.
+DELTA_WORKSPACE_BYTES = (16 << 20, 192 << 20)
+_DELTA_WS: dict = {}            # (device, stream, bytes) -> workspace
+_DELTA_WS_CAPTURE: dict = {}    # the same -> (capture id, workspace of that graph)
+
+
+def delta_workspace(nbytes: int, device, stream=None):
+    """The workspace of gated_delta_rule for calls on one stream, of any content; kept, and recorded by
+    graphs, as gemm_workspace's is."""
+    torch = _torch()
+    dev = torch.device(device)
+    handle = _stream(stream)
+    key = (dev.index if dev.index is not None else torch.cuda.current_device(), handle,
+           next((size for size in DELTA_WORKSPACE_BYTES if nbytes <= size), nbytes))
+    ws = _DELTA_WS.get(key)
+    if ws is not None:
+        return ws
+    return _new_workspace(_DELTA_WS, _DELTA_WS_CAPTURE, key, 0, 0, dev, handle, stream)
 
 
 def gated_delta_rule(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, normalize=False, state_index=None,
