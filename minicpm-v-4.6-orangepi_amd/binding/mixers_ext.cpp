@@ -26,7 +26,7 @@ PyObject* g_error;                               // McvError
 struct Workspaces {
     PyObject *make, *held;
 } g_gemm, g_delta;
-int64_t g_gemm_least, g_delta_sizes[2];
+int64_t g_gemm_sizes[2], g_delta_sizes[2];
 
 struct Failed {};                                // a Python error is set
 
@@ -144,16 +144,15 @@ void* workspace(const Workspaces& from, int64_t size, const at::Tensor& t, PyObj
     Py_DECREF(made);                             // (it is kept where it was made)
     return p;
 }
-// gemm_workspace's buffer of the next power of two: few sizes, whatever the calls'.  Other calls on the
-// stream use it too, so its first bytes are counters and stay zero.
+// One of two sizes: few buffers, whatever the calls'.
+int64_t of(const int64_t (&sizes)[2], int64_t bytes) { return bytes <= sizes[0] ? sizes[0] : bytes <= sizes[1] ? sizes[1] : bytes; }
+// gemm_workspace's buffer, or one that is enough for any call of this kind.  Other calls on the stream use it too, so
+// its first bytes are counters and stay zero.
 void* gemm_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
-    int64_t size = g_gemm_least;
-    if (bytes > size)
-        for (size = 1; size < bytes;) size *= 2;
-    return workspace(g_gemm, size, t, stream, h);
+    return workspace(g_gemm, of(g_gemm_sizes, bytes), t, stream, h);
 }
 void* delta_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
-    return workspace(g_delta, bytes <= g_delta_sizes[0] ? g_delta_sizes[0] : bytes <= g_delta_sizes[1] ? g_delta_sizes[1] : bytes, t, stream, h);
+    return workspace(g_delta, of(g_delta_sizes, bytes), t, stream, h);
 }
 
 // (who, q, k, v, g, beta, state, cu, step, scale, normalize, state_index, out, state_out, stream) -> (out, state_out)
@@ -316,21 +315,22 @@ PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 8, [&] { return rotary(a, false); }); }
 PyObject* py_rotary_cached(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 11, [&] { return rotary(a, true); }); }
 
-// (McvError, gemm_workspace, the buffers it keeps, the smallest's bytes, delta_workspace, its, its two sizes)
+// (McvError, gemm_workspace, the buffers it keeps, two sizes of them, delta_workspace, its, two of them)
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject* error;
     Workspaces gemm, delta;
-    long long least, small, large;
-    if (!PyArg_ParseTuple(args, "OOO!LOO!LL", &error, &gemm.make, &PyDict_Type, &gemm.held, &least, &delta.make, &PyDict_Type, &delta.held,
-                          &small, &large))
+    long long sizes[4];
+    if (!PyArg_ParseTuple(args, "OOO!LLOO!LL", &error, &gemm.make, &PyDict_Type, &gemm.held, &sizes[0], &sizes[1], &delta.make, &PyDict_Type,
+                          &delta.held, &sizes[2], &sizes[3]))
         return nullptr;
     for (PyObject* o : {error, gemm.make, gemm.held, delta.make, delta.held}) Py_INCREF(o);
     g_error = error;
     g_gemm = gemm;
     g_delta = delta;
-    g_gemm_least = least;
-    g_delta_sizes[0] = small;
-    g_delta_sizes[1] = large;
+    for (int i = 0; i < 2; ++i) {
+        g_gemm_sizes[i] = sizes[i];
+        g_delta_sizes[i] = sizes[2 + i];
+    }
     Py_RETURN_NONE;
 }
 

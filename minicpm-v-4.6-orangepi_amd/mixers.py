@@ -31,7 +31,8 @@ def binding():
         spec = importlib.util.spec_from_file_location("_mcv_mixers", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        mod.bind(McvError, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES)
+        most = lib().mcv_paged_attention_workspace_bytes(512, 16, 1, 256, 1 << 20)      # of any call
+        mod.bind(McvError, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, most, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES)
         _BINDING = mod
     return _BINDING
 

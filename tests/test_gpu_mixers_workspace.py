@@ -35,3 +35,48 @@ def test_two_sizes_a_stream(mcv, cuda):
         held = [ws.numel() for (_, stream, _), ws in mcv.mixers._DELTA_WS.items() if stream == side.cuda_stream]
     side.synchronize()
     assert len(held) == 2 and sum(held) <= 208 << 20
+
+
+def test_attention_has_two_sizes_a_stream(mcv, cuda):
+    torch = _torch()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for lens, Hq, Hkv, D in (([300], 2, 2, 64), ([3000], 8, 2, 128), ([20000], 4, 2, 256), ([20000, 7, 0], 16, 1, 256), ([900] * 60, 12, 2, 128)):
+            mcv.paged_attention_decode(*(x.to(cuda) for x in _attn_case(1, lens, Hq, Hkv, D, 32)[:5]))
+        held = [ws.numel() for (_, stream, _), ws in mcv._GEMM_WS.items() if stream == side.cuda_stream]
+    side.synchronize()
+    assert len(held) <= 2 and sum(held) <= 24 << 20
+
+
+def test_calls_allocate_nothing(mcv, cuda):
+    """Given their outputs, and once a stream has its workspaces."""
+    torch = _torch()
+    half = lambda *s: torch.zeros(*s, dtype=torch.float16, device=cuda)      # noqa: E731
+    delta = [(c, half(*c["v"].shape), torch.empty_like(c["state"])) for c in (_delta(cuda, lens) for lens in ([3], [300], [1] * 20, [1] * 20 + [400]))]
+    step = {n: x for n, x in _delta(cuda, [1] * 5).items() if n != "cu_seqlens"}
+    attn = [[x.to(cuda) for x in _attn_case(1, lens, 8, 2, 128, 32)[:5]] for lens in ([9], [700, 0], [20000], [500] * 40)]
+    attn = [(a, torch.empty_like(a[0])) for a in attn]
+    freq, axis = mcv.rotary_axes_table(64, 1e6, (12, 10, 10))
+    pos = torch.arange(3 * 50, device=cuda).view(3, 50)
+    q, k, v, qo, ko = half(50, 8, 128), half(50, 2, 128), half(50, 2, 128), half(50, 8, 128), half(50, 2, 128)
+    kc, vc, slots = half(5, 16, 2, 128), half(5, 16, 2, 128), torch.arange(50, device=cuda)
+    step_out = half(*step["v"].shape)
+
+    def once():
+        for c, out, state in delta:
+            mcv.gated_delta_rule(**c, out=out, state_out=state)
+        mcv.gated_delta_rule_step(**step, out=step_out)
+        for a, out in attn:
+            mcv.paged_attention_decode(*a, out=out)
+        mcv.rotary_axes(q, k, pos, freq, axis, q_out=qo, k_out=ko)
+        mcv.rotary_axes_cached(q, k, v, pos, freq, axis, kc, vc, slots, q_out=qo)
+
+    once()
+    torch.cuda.synchronize()
+    asked = lambda: torch.cuda.memory_stats()["allocation.all.allocated"]    # noqa: E731
+    before = asked()
+    for _ in range(3):
+        once()
+    assert asked() == before
+    torch.cuda.synchronize()
