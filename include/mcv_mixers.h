@@ -71,7 +71,8 @@ int64_t mcv_delta_rule_workspace_bytes(int64_t B, int64_t T, int64_t Hk, int64_t
  * Long caches are split over workgroups, whose parts the last of them joins in
  * order (deterministic): workspace of mcv_paged_attention_workspace_bytes bytes,
  * 256-byte aligned, its first 4 KiB zero before its first use (every call leaves
- * them zero), for one call at a time; NULL or too small: no split. */
+ * them zero), for one call at a time; NULL or too small: no split.  The bytes for
+ * a max_seq_len are enough for any shorter one. */
 int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
                         int64_t k_token, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_token,
                         int64_t v_head, int64_t pages, int64_t page_size, const void* block_table,

@@ -485,7 +485,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
 // 0: nothing to cut.
 int choose_workers(int64_t groups, int64_t most) {
     const int64_t tiles = ceil_div(most, kTile);
-    if (most <= 4 * kTile || groups * tiles > 0x3fffffff) return 0;
+    if (most <= 4 * kTile) return 0;
     return static_cast<int>(std::min<int64_t>(512, groups * ceil_div(tiles, 4)));
 }
 int64_t split_bytes(int64_t workers, int64_t rows, int64_t D) {
@@ -539,7 +539,7 @@ int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void
     const int64_t most = max_seq_len < held ? max_seq_len : held;
     const int64_t group = Hq / Hkv, htiles = ceil_div(group, kHeads), groups = B * Hkv * htiles;
     const int64_t rows = group < kHeads ? group : kHeads;
-    int workers = choose_workers(groups, most);
+    int workers = groups * ceil_div(most, kTile) <= 0x3fffffff ? choose_workers(groups, most) : 0;      // tiles are counted in 32 bits
     if (workers && (!workspace || workspace_bytes < split_bytes(workers, rows, D))) workers = 0;
     if (workers && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "paged_attention: workspace must be 256-byte aligned");
