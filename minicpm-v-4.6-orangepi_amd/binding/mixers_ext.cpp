@@ -198,6 +198,11 @@ PyObject* delta(PyObject* const* a) {
     const auto device = on_gpu(who, q);
     out = given ? *given : fresh(v.sizes(), at::kHalf, q);
     state_out = state_given ? *state_given : fresh({B, Hv, Dk, Dv}, at::kFloat, q);
+    if (B == 0) {                                // nothing to launch, of shapes that a batch would be taken of
+        if (Hk == 0 || Hv == 0 || Hv % Hk != 0 || (Dk != 64 && Dk != 128) || Dv == 0 || Dv % 16 != 0 || Dv > 256)
+            refuse("%s: bad shape q %s, v %s", who, shape(q).c_str(), shape(v).c_str());
+        return Py_BuildValue("(NN)", wrapped(out), wrapped(state_out));
+    }
     const mcv_stream_t h = handle(a[14]);
     const int64_t bytes = mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv);
     void* ws = bytes ? delta_workspace(bytes, q, a[14], h) : nullptr;
@@ -233,6 +238,11 @@ PyObject* paged(PyObject* const* a) {
     }
     const auto device = on_gpu(who, q);
     const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q);
+    if (B == 0) {
+        if (Hq == 0 || Hkv == 0 || Hq % Hkv != 0 || (D != 64 && D != 128 && D != 256) || page == 0 || page % 16 != 0)
+            refuse("%s: bad shape q %s, caches %s", who, shape(q).c_str(), shape(kc).c_str());
+        return wrapped(out);
+    }
     const mcv_stream_t h = handle(a[8]);
     const int64_t bytes = mcv_paged_attention_workspace_bytes(B, Hq, Hkv, D, most);
     void* ws = bytes ? gemm_workspace(bytes, q, a[8], h) : nullptr;

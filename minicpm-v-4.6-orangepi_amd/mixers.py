@@ -78,7 +78,8 @@ def gated_delta_rule(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=Non
 def gated_delta_rule_step(q, k, v, g, beta, state, *, scale=None, normalize=False, state_index=None, out=None,
                           state_out=None, stream=None):
     """gated_delta_rule of one token for each of B sequences: q, k fp16 [B, Hk, Dk], v fp16
-    [B, Hv, Dv], g and beta fp32 [B, Hv]; the state is updated in place unless state_out is given."""
+    [B, Hv, Dv], g and beta fp32 [B, Hv]; the state is updated in place unless state_out is given.
+    B may be 0."""
     return (_BINDING or binding()).delta("gated_delta_rule_step", q, k, v, g, beta, state, None, True, scale, normalize,
                                          state_index, out, state if state_out is None else state_out, stream)
 
@@ -92,7 +93,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale=
 
     Token t lies in row t % page_size of page block_table[b, t // page_size]; a page
     number outside the cache is left out like a masked token, and a sequence of
-    length 0 gives zeros.  max_seq_len, at most width * page_size (the default),
+    length 0 gives zeros (and a batch of none an empty result).  max_seq_len, at most width * page_size (the default),
     bounds the lengths.  Returns out fp16 [B, Hq, D]."""
     return (_BINDING or binding()).paged(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len, out, stream)
 
