@@ -79,6 +79,9 @@ bool truth(PyObject* o) {
     return v != 0;
 }
 
+// The stride of a dimension, none where it has one entry: torch leaves any there.
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 // fp16 [rows][heads][D]: pointer, row stride, head stride.
 struct Heads {
     void* p;
@@ -88,7 +91,7 @@ Heads heads(const char* who, const char* name, const at::Tensor& t, int64_t rows
     if (t.scalar_type() != at::kHalf || t.dim() != 3 || t.stride(2) != 1 || t.size(0) != rows)
         refuse("%s: %s must be fp16 [%lld, heads, D] with contiguous heads, got %s %s", who, name, (long long)rows,
                c10::toString(t.scalar_type()), shape(t).c_str());
-    return {t.data_ptr(), t.stride(0), t.stride(1)};
+    return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1)};
 }
 // fp16 [pages][page_size][Hkv][D] of `like`'s shape.
 struct Cache {
@@ -99,7 +102,7 @@ Cache cache(const char* who, const char* name, const at::Tensor& t, const at::Te
     if (t.scalar_type() != at::kHalf || t.dim() != 4 || t.sizes() != like.sizes() || t.size(2) != Hkv || t.size(3) != D || t.stride(3) != 1)
         refuse("%s: %s must be fp16 [pages, page_size, %lld, %lld] with contiguous heads, both caches of one shape, got %s %s", who,
                name, (long long)Hkv, (long long)D, c10::toString(t.scalar_type()), shape(t).c_str());
-    return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+    return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)};
 }
 void same_device(const char* who, const at::Tensor& t, std::initializer_list<const at::Tensor*> others) {
     for (const at::Tensor* o : others)
@@ -176,7 +179,7 @@ PyObject* delta(PyObject* const* a) {
     if (k.sizes() != q.sizes()) refuse("%s: q %s and k %s must have one shape", who, shape(q).c_str(), shape(k).c_str());
     const Heads qa = heads(who, "q", q, T), ka = heads(who, "k", k, T), va = heads(who, "v", v, T);
     for (const at::Tensor* t : {&g, &beta})
-        if (t->scalar_type() != at::kFloat || !is_shape(*t, {T, Hv}) || t->stride(1) != 1)
+        if (t->scalar_type() != at::kFloat || !is_shape(*t, {T, Hv}) || (Hv > 1 && t->stride(1) != 1))
             refuse("%s: %s must be fp32 [%lld, %lld] with contiguous rows", who, t == &g ? "g" : "beta", (long long)T, (long long)Hv);
     int64_t n_states = B;
     at::Tensor out, state_out;
@@ -206,8 +209,8 @@ PyObject* delta(PyObject* const* a) {
     const mcv_stream_t h = handle(a[14]);
     const int64_t bytes = mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv);
     void* ws = bytes ? delta_workspace(bytes, q, a[14], h) : nullptr;
-    check(mcv_delta_rule(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, g.data_ptr(), g.stride(0), beta.data_ptr(),
-                         beta.stride(0), ptr(state), state_out.data_ptr(), ptr(index), n_states, ptr(cu), B, T, Hk, Hv, Dk, Dv,
+    check(mcv_delta_rule(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, g.data_ptr(), stride_of(g, 0), beta.data_ptr(),
+                         stride_of(beta, 0), ptr(state), state_out.data_ptr(), ptr(index), n_states, ptr(cu), B, T, Hk, Hv, Dk, Dv,
                          number(a[9], 1.0 / std::sqrt(static_cast<double>(Dk))), truth(a[10]), out.data_ptr(),
                          ws, ws ? bytes : 0, h),
           who);
@@ -224,7 +227,7 @@ PyObject* paged(PyObject* const* a) {
     const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), pages = kc.size(0), page = kc.size(1), Hkv = kc.size(2);
     const Heads qa = heads(who, "q", q, B);
     const Cache ka = cache(who, "k_cache", kc, kc, Hkv, D), va = cache(who, "v_cache", vc, kc, Hkv, D);
-    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != B || (table.stride(1) != 1 && table.size(1) != 1))
+    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != B || (table.size(1) > 1 && table.stride(1) != 1))
         refuse("%s: block_table must be int32 [%lld, width] with contiguous rows", who, (long long)B);
     if (lens.scalar_type() != at::kInt || !is_shape(lens, {B}) || !lens.is_contiguous())
         refuse("%s: seq_lens must be contiguous int32 [%lld]", who, (long long)B);
@@ -247,7 +250,7 @@ PyObject* paged(PyObject* const* a) {
     const int64_t bytes = mcv_paged_attention_workspace_bytes(B, Hq, Hkv, D, most);
     void* ws = bytes ? gemm_workspace(bytes, q, a[8], h) : nullptr;
     check(mcv_paged_attention(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
-                              table.data_ptr(), table.stride(0), table.size(1), lens.data_ptr(), most, B, Hq, Hkv, D,
+                              table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), most, B, Hq, Hkv, D,
                               number(a[5], 1.0 / std::sqrt(static_cast<double>(D))), out.data_ptr(), ws, ws ? bytes : 0, h),
           who);
     return wrapped(out);
@@ -279,7 +282,7 @@ PyObject* rotary(PyObject* const* a, bool cached) {
         const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q), k_out = k_given ? *k_given : fresh(k.sizes(), at::kHalf, q);
         const Heads qo = heads(who, "q_out", q_out, T), ko = heads(who, "k_out", k_out, T);
         if (T)
-            check(mcv_rotary_axes(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, pos.data_ptr(), pos.stride(0), pos.stride(1), pos.size(0),
+            check(mcv_rotary_axes(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, pos.data_ptr(), stride_of(pos, 0), stride_of(pos, 1), pos.size(0),
                                   freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row, qo.head, ko.p, ko.row, ko.head,
                                   handle(a[7])),
                   who);
@@ -299,8 +302,8 @@ PyObject* rotary(PyObject* const* a, bool cached) {
     const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q);
     const Heads qo = heads(who, "q_out", q_out, T);
     if (T)
-        check(mcv_rotary_axes_cached(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, pos.data_ptr(), pos.stride(0),
-                                     pos.stride(1), pos.size(0), freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row,
+        check(mcv_rotary_axes_cached(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, pos.data_ptr(), stride_of(pos, 0),
+                                     stride_of(pos, 1), pos.size(0), freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row,
                                      qo.head, kca.p, kca.page, kca.token, kca.head, vca.p, vca.page, vca.token, vca.head, kc.size(0),
                                      kc.size(1), slots.data_ptr(), handle(a[10])),
               who);
