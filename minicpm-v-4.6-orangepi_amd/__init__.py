@@ -522,6 +522,12 @@ def _workspace_on(nbytes: int, zeroed: int, dev, handle: int, stream):
         ws[:zeroed].zero_()
         return ws
 
+    return _made_on(make, dev, handle, stream)
+
+
+def _made_on(make, dev, handle: int, stream):
+    """make(), with that stream as the current one: what it allocates is that stream's memory."""
+    torch = _torch()
     if handle == _stream():
         return make()
     if not isinstance(stream, torch.cuda.Stream):

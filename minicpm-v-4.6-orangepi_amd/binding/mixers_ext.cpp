@@ -21,7 +21,7 @@
 
 namespace {
 
-PyObject* g_error;                               // McvError
+PyObject *g_error, *g_empty_on;                  // McvError, and mixers.py's tensor of another stream
 // A function of mixers.py or the package that makes workspaces, the dict of those it keeps, by device, stream and size.
 struct Workspaces {
     PyObject *make, *held;
@@ -115,9 +115,6 @@ c10::DeviceGuard on_gpu(const char* who, const at::Tensor& t) {
     return c10::DeviceGuard(t.device());
 }
 void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
-at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
-    return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
-}
 PyObject* wrapped(const at::Tensor& t) { return THPVariable_Wrap(t); }
 
 // The handle of `stream` (a torch stream, or None: the current one).
@@ -129,6 +126,19 @@ mcv_stream_t handle(PyObject* stream) {
     Py_DECREF(h);
     if (!p && PyErr_Occurred()) throw Failed{};
     return static_cast<mcv_stream_t>(p);
+}
+
+// An output of a call on `stream`, whose handle is h.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like, PyObject* stream, mcv_stream_t h) {
+    if (h == handle(Py_None)) return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
+    PyObject* shape = PyTuple_New(static_cast<Py_ssize_t>(sizes.size()));
+    if (!shape) throw Failed{};
+    for (size_t i = 0; i < sizes.size(); ++i) PyTuple_SET_ITEM(shape, i, PyLong_FromLongLong(sizes[i]));
+    PyObject* made = PyObject_CallFunction(g_empty_on, "NisO", shape, int(type == at::kFloat), like.device().str().c_str(), stream);
+    if (!made) throw Failed{};
+    const at::Tensor t = THPVariable_Unpack(made);
+    Py_DECREF(made);
+    return t;
 }
 
 // A buffer of `size` bytes.  Held ones are looked up here, a reference of that dict is all it takes.
@@ -199,14 +209,14 @@ PyObject* delta(PyObject* const* a) {
         refuse("%s: out must be contiguous fp16 %s", who, shape(v).c_str());
     same_device(who, q, {&k, &v, &g, &beta, state, state_given, index, cu, given});
     const auto device = on_gpu(who, q);
-    out = given ? *given : fresh(v.sizes(), at::kHalf, q);
-    state_out = state_given ? *state_given : fresh({B, Hv, Dk, Dv}, at::kFloat, q);
+    const mcv_stream_t h = handle(a[14]);
+    out = given ? *given : fresh(v.sizes(), at::kHalf, q, a[14], h);
+    state_out = state_given ? *state_given : fresh({B, Hv, Dk, Dv}, at::kFloat, q, a[14], h);
     if (B == 0) {                                // nothing to launch, of shapes that a batch would be taken of
         if (Hk == 0 || Hv == 0 || Hv % Hk != 0 || (Dk != 64 && Dk != 128) || Dv == 0 || Dv % 16 != 0 || Dv > 256)
             refuse("%s: bad shape q %s, v %s", who, shape(q).c_str(), shape(v).c_str());
         return Py_BuildValue("(NN)", wrapped(out), wrapped(state_out));
     }
-    const mcv_stream_t h = handle(a[14]);
     const int64_t bytes = mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv);
     void* ws = bytes ? delta_workspace(bytes, q, a[14], h) : nullptr;
     check(mcv_delta_rule(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, g.data_ptr(), stride_of(g, 0), beta.data_ptr(),
@@ -240,13 +250,13 @@ PyObject* paged(PyObject* const* a) {
         if (most == -1 && PyErr_Occurred()) throw Failed{};
     }
     const auto device = on_gpu(who, q);
-    const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q);
+    const mcv_stream_t h = handle(a[8]);
+    const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q, a[8], h);
     if (B == 0) {
         if (Hq == 0 || Hkv == 0 || Hq % Hkv != 0 || (D != 64 && D != 128 && D != 256) || page == 0 || page % 16 != 0)
             refuse("%s: bad shape q %s, caches %s", who, shape(q).c_str(), shape(kc).c_str());
         return wrapped(out);
     }
-    const mcv_stream_t h = handle(a[8]);
     const int64_t bytes = mcv_paged_attention_workspace_bytes(B, Hq, Hkv, D, most);
     void* ws = bytes ? gemm_workspace(bytes, q, a[8], h) : nullptr;
     check(mcv_paged_attention(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
@@ -279,12 +289,14 @@ PyObject* rotary(PyObject* const* a, bool cached) {
         for (const at::Tensor* t : {given, k_given})
             if (t) heads(who, t == given ? "q_out" : "k_out", *t, T);
         const auto device = on_gpu(who, q);
-        const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q), k_out = k_given ? *k_given : fresh(k.sizes(), at::kHalf, q);
+        const mcv_stream_t h = handle(a[7]);
+        const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q, a[7], h);
+        const at::Tensor k_out = k_given ? *k_given : fresh(k.sizes(), at::kHalf, q, a[7], h);
         const Heads qo = heads(who, "q_out", q_out, T), ko = heads(who, "k_out", k_out, T);
         if (T)
             check(mcv_rotary_axes(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, pos.data_ptr(), stride_of(pos, 0), stride_of(pos, 1), pos.size(0),
                                   freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row, qo.head, ko.p, ko.row, ko.head,
-                                  handle(a[7])),
+                                  h),
                   who);
         return Py_BuildValue("(NN)", wrapped(q_out), wrapped(k_out));
     }
@@ -299,13 +311,14 @@ PyObject* rotary(PyObject* const* a, bool cached) {
     const Heads va = heads(who, "v", v, T);
     if (given) heads(who, "q_out", *given, T);
     const auto device = on_gpu(who, q);
-    const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q);
+    const mcv_stream_t h = handle(a[10]);
+    const at::Tensor q_out = given ? *given : fresh(q.sizes(), at::kHalf, q, a[10], h);
     const Heads qo = heads(who, "q_out", q_out, T);
     if (T)
         check(mcv_rotary_axes_cached(qa.p, qa.row, qa.head, ka.p, ka.row, ka.head, va.p, va.row, va.head, pos.data_ptr(), stride_of(pos, 0),
                                      stride_of(pos, 1), pos.size(0), freq.data_ptr(), axis.data_ptr(), T, Hq, Hkv, D, 2 * half, qo.p, qo.row,
                                      qo.head, kca.p, kca.page, kca.token, kca.head, vca.p, vca.page, vca.token, vca.head, kc.size(0),
-                                     kc.size(1), slots.data_ptr(), handle(a[10])),
+                                     kc.size(1), slots.data_ptr(), h),
               who);
     return wrapped(q_out);
 }
@@ -328,16 +341,17 @@ PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 8, [&] { return rotary(a, false); }); }
 PyObject* py_rotary_cached(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 11, [&] { return rotary(a, true); }); }
 
-// (McvError, gemm_workspace, the buffers it keeps, two sizes of them, delta_workspace, its, two of them)
+// (McvError, _empty_on, gemm_workspace, the buffers it keeps, two sizes of them, delta_workspace, its, two of them)
 PyObject* py_bind(PyObject*, PyObject* args) {
-    PyObject* error;
+    PyObject *error, *empty_on;
     Workspaces gemm, delta;
     long long sizes[4];
-    if (!PyArg_ParseTuple(args, "OOO!LLOO!LL", &error, &gemm.make, &PyDict_Type, &gemm.held, &sizes[0], &sizes[1], &delta.make, &PyDict_Type,
+    if (!PyArg_ParseTuple(args, "OOOO!LLOO!LL", &error, &empty_on, &gemm.make, &PyDict_Type, &gemm.held, &sizes[0], &sizes[1], &delta.make, &PyDict_Type,
                           &delta.held, &sizes[2], &sizes[3]))
         return nullptr;
-    for (PyObject* o : {error, gemm.make, gemm.held, delta.make, delta.held}) Py_INCREF(o);
+    for (PyObject* o : {error, empty_on, gemm.make, gemm.held, delta.make, delta.held}) Py_INCREF(o);
     g_error = error;
+    g_empty_on = empty_on;
     g_gemm = gemm;
     g_delta = delta;
     for (int i = 0; i < 2; ++i) {

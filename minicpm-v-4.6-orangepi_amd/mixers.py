@@ -5,13 +5,14 @@ key-value cache for the full-attention layers.
 
 Activations and caches are fp16, gates and states fp32.  q, k and v may be
 columns of one projection's output: rows and heads have strides, the elements
-of one head are contiguous.
+of one head are contiguous.  A call with stream= runs there, and what it allocates is that
+stream's, as under torch.cuda.stream(stream).
 """
 from __future__ import annotations
 
 import importlib.util
 
-from . import _GEMM_WS, GEMM_WORKSPACE_BYTES, PKG_DIR, McvError, _new_workspace, _stream, _torch, gemm_workspace, lib
+from . import _GEMM_WS, GEMM_WORKSPACE_BYTES, PKG_DIR, McvError, _made_on, _new_workspace, _stream, _torch, gemm_workspace, lib
 
 # A call's checks and its launch are native (binding/mixers_ext.cpp): the kernels of one
 # decoded token take 3 to 5 us, and a call written here with ctypes took 9 to 12.  MI355X,
@@ -32,9 +33,17 @@ def binding():
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         most = lib().mcv_paged_attention_workspace_bytes(512, 16, 1, 256, 1 << 20)      # of any call
-        mod.bind(McvError, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, most, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES)
+        mod.bind(McvError, _empty_on, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, most, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES)
         _BINDING = mod
     return _BINDING
+
+
+def _empty_on(shape, single: bool, device, stream):
+    """An output, fp32 or fp16, of a call on a stream that is not the current one: its memory, so that it is not handed
+    out anew while that stream still writes to it, nor written while the current stream still uses what it was."""
+    torch = _torch()
+    make = lambda: torch.empty(shape, dtype=torch.float32 if single else torch.float16, device=device)     # noqa: E731
+    return _made_on(make, torch.device(device), _stream(stream), stream)
 
 
 # The delta rule's workspace comes in two sizes, for some 800 tokens of 16 heads of 128 and for all that a pass takes of

@@ -80,3 +80,36 @@ def test_calls_allocate_nothing(mcv, cuda):
         once()
     assert asked() == before
     torch.cuda.synchronize()
+
+
+def test_outputs_of_another_stream(mcv, cuda):
+    """What a call on another stream allocates is that stream's: freed at once, the current stream does not get it."""
+    torch = _torch()
+    side = torch.cuda.Stream()
+    delta, step = _delta(cuda, [300]), {n: x for n, x in _delta(cuda, [1] * 5).items() if n != "cu_seqlens"}
+    attn = [x.to(cuda) for x in _attn_case(1, [5000], 8, 2, 128, 32)[:5]]
+    q, k = torch.randn(50, 8, 128, device=cuda).half(), torch.randn(50, 2, 128, device=cuda).half()
+    freq, axis = mcv.rotary_axes_table(64, 1e6, (12, 10, 10))
+    pos = torch.arange(3 * 50, device=cuda).view(3, 50)
+    cache = [torch.zeros(5, 16, 2, 128, device=cuda).half() for _ in range(2)]
+    slots, state_out = torch.arange(50, device=cuda), torch.empty_like(step["state"])
+    calls = [
+        lambda **on: mcv.gated_delta_rule(**delta, **on),
+        lambda **on: mcv.gated_delta_rule_step(**step, state_out=state_out, **on)[:1],
+        lambda **on: (mcv.paged_attention_decode(*attn, **on),),
+        lambda **on: mcv.rotary_axes(q, k, pos, freq, axis, **on),
+        lambda **on: (mcv.rotary_axes_cached(q, k, k, pos, freq, axis, *cache, slots, **on),),
+    ]
+    for call in calls:
+        want = call()
+        torch.cuda.synchronize()
+        got = call(stream=side)
+        side.synchronize()
+        assert all((x == y).all() for x, y in zip(got, want))
+        where, shapes = {t.data_ptr() for t in got}, [(t.shape, t.dtype) for t in got]
+        del got
+        fresh = [torch.empty(shape, dtype=dtype, device=cuda) for shape, dtype in shapes for _ in range(4)]
+        assert not where & {t.data_ptr() for t in fresh}
+        same = call(stream=torch.cuda.current_stream())
+        assert all((x == y).all() for x, y in zip(same, want))
+    assert torch.cuda.current_stream() != side
