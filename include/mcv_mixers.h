@@ -42,9 +42,10 @@ extern "C" {
  * chunks of 64 tokens on the matrix cores, for which the call needs a workspace
  * of mcv_delta_rule_workspace_bytes(B, T, Hk, Hv, Dk, Dv) bytes, 256-byte aligned,
  * of any content (NULL or too small: the recurrence, however long).  Chunks hold
- * the state in two fp16 parts scaled by the largest |v| and |state| of the
- * sequence: a state that grows past 4096 times that overflows, which a stable
- * rule (beta |k|^2 <= 2) does not do.  An infinity or NaN in q, k, v, a gate or a
+ * values and the state in two fp16 parts scaled by M, the largest |v| of the chunk
+ * and the one before or what decay leaves of the M before (the first: the state's
+ * largest): they are off by 2^-28 M at worst, and overflow where they grow past
+ * 4096 M, which a stable rule (beta |k|^2 <= 2) does not do.  An infinity or NaN in q, k, v, a gate or a
  * state reaches what it reaches by the formulas, of its own token and later ones;
  * from there on the chunks may have NaN where the formulas have an infinity. */
 int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,

@@ -21,9 +21,11 @@
 // bits; T by substitution, in fp32 products).  Operands of products are two fp16 parts,
 // 22 bits, of which only lo x lo is left out; q, k and v are fp16 as they come.  fp16's
 // range: turned k rows are scaled by the power of two next to their norm's factor, q's
-// norm is taken out of P, and the scan works on states and values scaled by a power of
-// two that brings the largest to 8 .. 16, so that they may grow 4096-fold and a part's
-// last bit is 2^-25 at worst.
+// norm is taken out of P, and the scan works on states and values scaled, for each chunk, by
+// a power of two that brings M to 8 .. 16, M = the largest |v| of it and the chunk before or
+// what decay leaves of the M before: they may grow 4096-fold, and a part's last bit is 2^-25
+// at worst, 2^-28 M.  (The state's own largest would be less where the rule takes from it
+// without decay; found by the outputs' waves it cost 0.13 us a chunk.)
 //
 // Order in time.  The products T X and P U run over whole tiles, zeros above the diagonal included, and a zero times an
 // infinity or NaN of a later token would be NaN.  So T holds no rows of tokens whose k or gates are not finite (X has
@@ -46,7 +48,7 @@ namespace {
 constexpr int kC = 64;                           // tokens of a chunk
 constexpr int64_t kSegmentBytes = int64_t(192) << 20;   // workspace of one pass over the chunks
 constexpr int kBet = 0, kBr = 64, kEf = 128, kEq = 192, kOsc = 256;   // of a unit's scalars, 64 each, then:
-constexpr int kKeep = 320, kVmax = 321;          // e^(G_last), largest |v| two waves saw
+constexpr int kKeep = 320, kVmax = 321;          // e^(G_last), largest |v|
 constexpr int kScalars = 352;
 constexpr int kTriBytes = 6 * 2 * 64 * 16;       // a triangle of 16 x 32 blocks, two parts
 
@@ -144,6 +146,14 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Global loads after this stay behind the LDS writes before it, which others wait for.
 __device__ __forceinline__ void lds_first() { asm volatile("" ::: "memory"); }
 
+// For the largest of two fp16 values' magnitudes, of finite ones: whole numbers from 0x400 on, where what is not finite
+// has wrapped to less; and that number's value.
+__device__ __forceinline__ ushort2_t finite_up(uint32_t x) { return __builtin_bit_cast(ushort2_t, ((x & 0x7fff7fffu) + 0x04000400u) & 0x7fff7fffu); }
+__device__ __forceinline__ float largest_of(ushort2_t v) {
+    const int top = v[0] > v[1] ? v[0] : v[1];
+    return top < 0x400 ? 0.f : h2f(static_cast<uint16_t>(top - 0x400));
+}
+
 // Position of token t's value in row d of a transposed tile [D][64] fp16: operand order,
 // 16-byte blocks moved so that neither the pair stores nor the operand loads conflict.
 __device__ __forceinline__ int turned(int d, int block) { return d * 64 + ((block ^ d ^ (d >> 3)) & 7) * 8; }
@@ -170,7 +180,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
     // k and q as rows, 16-byte chunks moved so that operand reads do not conflict; then k turned and L, T
     constexpr int RC = DK / 8;                   // chunks of a row
     __shared__ __attribute__((aligned(16))) uint8_t space[2][kC * PT * 4];
-    __shared__ __attribute__((aligned(16))) float gh[kC], gl[kC], bet[kC], rkn[kC], rqn[kC], kk[kC], qq[kC], lrow[kC], pcol[kC], fall[4][kC];
+    __shared__ __attribute__((aligned(16))) float gh[kC], gl[kC], bet[kC], rkn[kC], rqn[kC], kk[kC], qq[kC], lrow[kC], pcol[kC], fall[4][kC], vmax[2];
     __shared__ __attribute__((aligned(16))) _Float16 kpow[kC];
     half8_t* const kr = reinterpret_cast<half8_t*>(space[0]);
     half8_t* const qr = reinterpret_cast<half8_t*>(space[1]);
@@ -261,7 +271,6 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
         bet[lane] = lane < n ? gate : 0.f;
     }
     if (w < 2) {                                 // the largest |v|, for the scan's scale; these have fewer products
-        // (of finite ones: as whole numbers from 0x400 on, where what is not finite has wrapped to less)
         ushort2_t most = {0, 0};
         for (int from = 0;;) {
 #pragma unroll
@@ -269,15 +278,14 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t x = e == 0 ? vx[i].x : e == 1 ? vx[i].y : e == 2 ? vx[i].z : vx[i].w;
-                    most = __builtin_elementwise_max(most, __builtin_bit_cast(ushort2_t, ((x & 0x7fff7fffu) + 0x04000400u) & 0x7fff7fffu));
+                    most = __builtin_elementwise_max(most, finite_up(x));
                 }
             from += 128;
             if (from >= p.Dv) break;
             load_v(from);
         }
-        const int top = most[0] > most[1] ? most[0] : most[1];
-        const float big = wave_butterfly(top < 0x400 ? 0.f : h2f(static_cast<uint16_t>(top - 0x400)), [](float x, float y) { return fmaxf(x, y); });
-        if (lane == 0) sc[kVmax + w] = big;
+        const float big = wave_butterfly(largest_of(most), [](float x, float y) { return fmaxf(x, y); });
+        if (lane == 0) vmax[w] = big;
     }
     __syncthreads();
     // k turned: a thread packs two tokens of eight d
@@ -308,6 +316,7 @@ __global__ __launch_bounds__(256, 3) void delta_prepare_kernel(ChunkArgs a) {
             sc[kBr + lane] = b * rk * eg;
             sc[kEf + lane] = to_end * (p.normalize ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 1.0f);
             if (lane == kC - 1) sc[kKeep] = eg;
+            if (lane == 0) sc[kVmax] = fmaxf(vmax[0], vmax[1]);
         } else if (w == 1) {
             rqn[lane] = rn;
             sc[kEq + lane] = exp2_of(g_hi + g_lo) * rn;
@@ -475,7 +484,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
     __shared__ __attribute__((aligned(16))) uint2 sf[2][NT][KS][64][2];       // S, two parts, operand order
     __shared__ __attribute__((aligned(16))) uint2 xf[2][NT][2][64][2];        // X, two parts
     __shared__ __attribute__((aligned(16))) uint2 uf[4][NT][2][64][2];        // U and e^(G_last - G) f U, two parts each
-    __shared__ float maxes[8];
+    __shared__ float maxes[4], down_next;
 
     // the state and the scale of this pass
     const int count = c1 > c0 ? c1 - c0 : 0;
@@ -513,20 +522,23 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
     }
     const int slot = s0 + c0 - a.slot0;          // of chunk c0 in this pass
     const int64_t unit0 = static_cast<int64_t>(slot) * p.Hv + h;     // its unit; the next is Hv on
-    for (int i = threadIdx.x; i < (c1 - c0) * 2; i += 512)
-        big = fmaxf(big, a.sc[(unit0 + static_cast<int64_t>(i / 2) * p.Hv) * kScalars + kVmax + i % 2]);
+    float up, down, largest;                     // M, in true size
+    auto scale_for = [](float most, float& up, float& down) {    // (2^126 at most: both are normal numbers)
+        const int ex = min(3 + 127 - static_cast<int>(__float_as_uint(most) >> 23), 126);
+        up = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+        down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+    };
     // Both kinds of waves call this once, with their first operands on the way.
-    float up, down;
+    const float first_vmax = a.sc[unit0 * kScalars + kVmax];
     auto agree_on_scale = [&]() {
         float most = wave_butterfly(big, [](float x, float y) { return fmaxf(x, y); });
-        if (lane == 0) maxes[wave] = most;
+        if (lane == 0 && wave < 4) maxes[wave] = most;
         lds_barrier();
+        most = first_vmax;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, maxes[i]);
-        int ex = most > 0.f ? 3 - ilogbf(most) : 0;
-        ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
-        up = ldexpf(1.0f, ex);
-        down = ldexpf(1.0f, -ex);
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, maxes[i]);
+        largest = most;
+        scale_for(most, up, down);
     };
     const int64_t first = t0 + static_cast<int64_t>(c0) * kC;
     const int n_last = t1 - (first + static_cast<int64_t>(count - 1) * kC) < kC
@@ -554,7 +566,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
         struct Stage {
             half8_t k[KS], kt[MT][2], t[2][2];
             vrow v[4];
-            float bet, br, ef, keep;             // of token 4 j + c % 4 of the wave's tile; e^(G_last)
+            float bet, br, ef, keep, vmax;       // of token 4 j + c % 4 of the wave's tile; e^(G_last); the next chunk's largest |v|
         } st[PD];
         // Loads are unconditional (past the last chunk: the last again), so that a wait counts those in flight exactly.
         int64_t voff[4];
@@ -577,7 +589,10 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 s.v[r] = *reinterpret_cast<const vrow*>(vbase + static_cast<int64_t>(i) * kC * p.v_row + voff[r]);
-            const float* sc = a.sc + (unit0 + static_cast<int64_t>(i) * p.Hv) * kScalars + 16 * w + 4 * j + c % 4;
+            const float* sc = a.sc + (unit0 + static_cast<int64_t>(i) * p.Hv) * kScalars;
+            s.keep = sc[kKeep];
+            s.vmax = sc[(i + 1 < count ? p.Hv * kScalars : 0) + kVmax];
+            sc += 16 * w + 4 * j + c % 4;
             s.bet = sc[kBet];
             s.br = sc[kBr];
         };
@@ -596,7 +611,6 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) s.kt[m][q] = as_h8(at[((MT * w + m) * 2 + q) * 64]);
-            s.keep = a.sc[(unit0 + static_cast<int64_t>(i) * p.Hv) * kScalars + kKeep];
         };
         auto put_state = [&]() {
 #pragma unroll
@@ -629,6 +643,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
             for (int x = 0; x < NT; ++x) S[m][x] *= up;
         put_state();
+        float vmax = first_vmax;                 // of this chunk
         for (int i0 = 0; i0 < count; i0 += PD)
 #pragma unroll
             for (int q = 0; q < PD; ++q) {
@@ -704,6 +719,14 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                 };
                 float all = 0.f;
                 read_x(0);
+                // The next chunk's scale, while X comes (no step of it past 2^64).
+                const float keep = s.keep;
+                largest = fmaxf(fmaxf(largest * (keep < 0x1p60f ? keep : 1.f), 0x1p-60f * down), fmaxf(vmax, s.vmax));
+                vmax = s.vmax;
+                float up_next, down_to;
+                scale_for(largest, up_next, down_to);
+                const float rescale = up_next * down, keep_to = keep * rescale;
+                down_next = down_to;             // (of every lane: a branch for one costs 0.06 us a chunk)
                 lds_first();
                 load_k(s, ahead);
                 load_v(s, ahead);
@@ -721,10 +744,11 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                     }
                     u += v + z;
                     all += (u[0] + u[1]) + (u[2] + u[3]);
+                    const float ef = s.ef * rescale;
                     float4_t eu;
                     half4_t part[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) eu[r] = apart(of_quad(s.ef, r) * u[r]);
+                    for (int r = 0; r < 4; ++r) eu[r] = apart(of_quad(ef, r) * u[r]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] = apart(u[r]);
                     split<4>(eu, part[2], part[3]);
@@ -750,7 +774,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                     if (x) read_u(x);
                     float4_t low[MT] = {};
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) S[m][x] *= s.keep;
+                    for (int m = 0; m < MT; ++m) S[m][x] *= keep_to;
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -761,6 +785,8 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
 #pragma unroll
                     for (int m = 0; m < MT; ++m) S[m][x] += low[m];
                 }
+                up = up_next;
+                down = down_to;
                 put_state();
             }
         store_state(down);
@@ -793,6 +819,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
             asm volatile("" ::: "memory");
         }
         agree_on_scale();
+        float down_to = down;                    // the scales of the chunk to finish next, and of the one after
         float4_t o[NT], ol[NT];                  // e^G Q S of a chunk: rows dv, column token
         // P U of column x, U's first that is not finite and all after it NaN: rows dv, column token
         auto in_order = [&](const Stage& s, int x) {
@@ -877,6 +904,8 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                 lds_barrier();                   // U is there, S has been read
                 load_p(before, next(i - 1 + PD));
                 load_q(s, next(i + PD));
+                down = down_to;
+                down_to = down_next;
             }
 #pragma unroll
         for (int q = 0; q < PD; ++q)
