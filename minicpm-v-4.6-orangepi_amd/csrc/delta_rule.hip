@@ -138,12 +138,17 @@ __global__ __launch_bounds__(kThreads) void delta_recurrent_kernel(DeltaArgs p) 
 // Where the chunked form is faster than 1.1 us a token of the longest sequence.  MI355X, us a pass, recurrence and chunks
 // (16 heads of 128): 1 sequence of 8 tokens 11.7 14.5, of 12 16.3 14.6, of 32 39.0 14.6; 4 of 8 on average 26.4 20.3.
 // Lengths are the device's, and one sequence may have all tokens but a few: 100 of one token and one of 800 take 1083 us
-// by the recurrence and 88 as below.
+// by the recurrence and 88 as below.  Both forms launched cost the recurrence's batches 4 to 9 us (41 of two tokens 19.1
+// 28.1, 8 of five 9.6 13.9) and save what one longer sequence takes: 40 of one token and one of 20 39.0 38.0, of 40 61.9
+// 38.4, of 63 88.2 38.5; 7 and one of 33 41.4 20.3, of 60 72.5 20.4.  From 32 tokens more than sequences on the second
+// is the larger of the two that a wrong guess loses.
 constexpr int kShort = 10;
 bool may_be_long(int64_t B, int64_t T) {
-    const int64_t even = kShort * B, skewed = B + 64;
-    return T >= (B == 1 || (B <= kMixed && even < skewed) ? even : skewed);
+    const int64_t even = kShort * B, skewed = B + 32;
+    return T >= (B == 1 || even < skewed ? even : skewed);
 }
+// Then: whether both forms are launched.  With few sequences not where they may all be long.
+bool mixed(int64_t B, int64_t T) { return B > kMixed || (B > 1 && T < kShort * B && T < B + 64); }
 
 }  // namespace
 }  // namespace mcv
@@ -193,7 +198,7 @@ int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, 
     if (chunks) {
         if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
             return fail(MCV_ERR_INVALID_ARG, "delta_rule: workspace must be 256-byte aligned");
-        a.short_below = cu_seqlens && B > kMixed ? kShort : 0;
+        a.short_below = cu_seqlens && mixed(B, T) ? kShort : 0;
         rc = launch_delta_chunk(a, static_cast<int>(Hk), static_cast<int>(Dk), workspace, workspace_bytes, static_cast<hipStream_t>(stream));
         if (rc != MCV_OK || a.short_below == 0) return rc;
     }
