@@ -10,12 +10,14 @@
 //   delta_scan_kernel     a workgroup per 16 NT columns of one state walks its chunks
 // The scan takes K and V as they come and applies T: three products that wait for one another
 // where T K and T V made ahead would leave two, but K is exact in fp16 where T K takes two
-// parts, and less goes through memory (8192 tokens: 49 + 144 us, with T K and T V 70 + 147).
+// parts, and less goes through memory (8192 tokens: 49 + 144 us, with T K and T V 70 + 147; before the order in
+// time and the scales below were right, 47 + 148 since).
 //
-// The first is bound by memory (8192 tokens, 16 heads of 128: 250 MB in 49 us on MI355X).
-// The second walks in series, 1.1 us a chunk: without its outputs 1.04, without the loads of
-// the state's waves 0.85, without both 0.75, which is three times an LDS write, a barrier,
-// an LDS read and a short chain of products; the loads are 76 KB a chunk and CU.
+// The first is bound by memory (8192 tokens, 16 heads of 128: 250 MB in 47 us on MI355X).
+// The second walks in series, 1.16 us a chunk; 1.12 before every chunk had a scale and a look
+// at what is not finite, and then without its outputs 1.04, without the loads of the state's
+// waves 0.85, without both 0.75, which is three times an LDS write, a barrier, an LDS read and
+// a short chain of products; the loads are 76 KB a chunk and CU.
 //
 // Precision.  The state, G, L, T and all sums are fp32 (G's differences from a sum in 64
 // bits; T by substitution, in fp32 products).  Operands of products are two fp16 parts,
@@ -718,8 +720,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                     uf[1][x][w / 2][lane][w % 2] = __builtin_bit_cast(uint2, lo);
                 };
                 float all = 0.f;
-                read_x(0);
-                // The next chunk's scale, while X comes (no step of it past 2^64).
+                // The next chunk's scale (no step of it past 2^64); behind X's reads 1 us more over 8192 tokens.
                 const float keep = s.keep;
                 largest = fmaxf(fmaxf(largest * (keep < 0x1p60f ? keep : 1.f), 0x1p-60f * down), fmaxf(vmax, s.vmax));
                 vmax = s.vmax;
@@ -727,6 +728,7 @@ __global__ __launch_bounds__(512, 2) void delta_scan_kernel(ChunkArgs a) {
                 scale_for(largest, up_next, down_to);
                 const float rescale = up_next * down, keep_to = keep * rescale;
                 down_next = down_to;             // (of every lane: a branch for one costs 0.06 us a chunk)
+                read_x(0);
                 lds_first();
                 load_k(s, ahead);
                 load_v(s, ahead);

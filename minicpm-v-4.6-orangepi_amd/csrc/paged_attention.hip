@@ -24,10 +24,10 @@
 // parts joins them in order, and where there are more than kFan the last of those joins
 // the joined, so the bits do not depend on who is last and nobody waits.
 //
-// Long caches are bound by HBM: 8 heads on 2 of 256, 200000 tokens 68.8 us on MI355X, 6.0
+// Long caches are bound by HBM: 8 heads on 2 of 256, 200000 tokens 69.0 us on MI355X, 5.9
 // TB/s (a read-only stream reaches 6.3).  Short ones by round trips that wait for one
 // another (lengths, page numbers, K and V, the part written through, its counter, the
-// other parts: 1100 tokens 8.9 us).
+// other parts: 1100 tokens 9.1 us).
 #include <algorithm>
 
 #include "mixers.h"
@@ -481,7 +481,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attention_kernel(AttnArgs p) 
 
 // Workgroups to cut the `groups` (sequence, cache head, head tile)s of up to `most` tokens for: what the chip
 // holds at once with D = 256, two a CU.  With D = 128 it holds three; MI355X, us of 512, 640 and 768: 16 x 2000 ragged
-// 15.7 15.6 16.2, 8 x 20000 48 51 51, 41 x 4096 (32 heads on 8) 55 49 51, 5 x 60000 48 53 50, 64 x 1000 25.9 25.9 26.4.
+// 15.7 15.6 16.2, 8 x 20000 48 51 51, 41 x 4096 (32 heads on 8) 55 49 51, 5 x 60000 48 53 50, 64 x 1000 25.9 25.9 26.4:
+// no number is the best of all, 512 loses once.
 // 0: nothing to cut.
 int choose_workers(int64_t groups, int64_t most) {
     const int64_t tiles = ceil_div(most, kTile);

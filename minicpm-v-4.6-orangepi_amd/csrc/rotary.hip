@@ -6,7 +6,7 @@
 // Bound by memory, so the data is on its way while the angles are made: a thread has 32
 // bytes of the same place in a head (two chunks that turn into one another, or two that
 // are copied) of one or four tokens in registers before the workgroup's angles meet in LDS.
-// MI355X, 8 + 2 heads of 256, 64 turned, with the cache: 8192 tokens 20.7 us, 4.9 TB/s (a
+// MI355X, 8 + 2 heads of 256, 64 turned, with the cache: 8192 tokens 20.9 us, 4.8 TB/s (a
 // copy of 1 GiB 5.2); one token 4.2 us, the host's part of a call.
 #include "mixers.h"
 
@@ -207,8 +207,9 @@ int launch_rotary(RotaryArgs& a, mcv_stream_t stream) {
     }
     const int64_t items = (static_cast<int64_t>(a.Hq) + a.Hkv + (a.v ? a.Hkv : 0)) * (a.D / 16);
     const dim3 threads(static_cast<unsigned>(items < 256 ? ceil_div(items, 64) * 64 : 256));
-    // Four tokens a workgroup once that still fills the chip.  MI355X, us a pass with the cache (8 + 2 heads of 256, 64
-    // turned), one and four tokens: 2048 tokens 9.4 10.7, 4096 15.6 15.2, 8192 27.2 25.0.
+    // Four tokens a workgroup once that still fills the chip.  MI355X, us a pass, one and four tokens: with the cache, 8 + 2
+    // heads of 256, 64 turned, 2048 tokens 7.6 8.7, 4096 12.4 12.2, 8192 24.7 20.9; 16 + 4 of 128 without 6.1 7.8, 10.2 10.5,
+    // 18.0 15.6; 16 + 16 of 64 without 5.1 6.3, 9.3 9.2, 14.4 12.7.
     if (a.T >= 4096)
         hipLaunchKernelGGL(rotary_chunk_kernel<4>, dim3(static_cast<unsigned>(ceil_div(a.T, 4))), threads, 0, static_cast<hipStream_t>(stream), a);
     else

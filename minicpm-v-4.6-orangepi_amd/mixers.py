@@ -16,7 +16,7 @@ from . import _GEMM_WS, GEMM_WORKSPACE_BYTES, PKG_DIR, McvError, _made_on, _new_
 
 # A call's checks and its launch are native (binding/mixers_ext.cpp): the kernels of one
 # decoded token take 3 to 5 us, and a call written here with ctypes took 9 to 12.  MI355X,
-# one token: delta rule 10.8 us a call, now 4.2; rotary with the cache 12.7, now 4.1.
+# one token: delta rule 10.8 us a call, now 4.2; rotary with the cache 12.7, now 4.2.
 _BINDING = None
 
 

@@ -31,12 +31,9 @@ def _check(mcv, cuda, inputs, lens, scale, normalize, state_too=True):
 BAD = [math.inf, -math.inf, math.nan]
 
 
-@pytest.mark.parametrize("n", [9, 64, 65, 200])
-@pytest.mark.parametrize("at", [0, 5, 31, 47, 63, 70, 129])
+@pytest.mark.parametrize("n,at", [(n, at) for n in (9, 64, 65, 200) for at in (0, 5, 31, 47, 63, 70, 129) if at < n])
 @pytest.mark.parametrize("bad", BAD)
 def test_in_v(mcv, cuda, n, at, bad):
-    if at >= n:
-        pytest.skip("past the sequence's end")
     q, k, v, g, beta, state = _delta_case(n + at, [n, 40], 2, 4, 128, 64)
     v[at, 1, 3], v[at, 2, 50] = bad, 1.0
     _check(mcv, cuda, (q, k, v, g, beta, state), [n, 40], 0.1, True)
