@@ -45,9 +45,11 @@ extern "C" {
  * values and the state in two fp16 parts scaled by M, the largest |v| of the chunk
  * and the one before or what decay leaves of the M before (the first: the state's
  * largest): they are off by 2^-28 M at worst, and overflow where they grow past
- * 4096 M, which a stable rule (beta |k|^2 <= 2) does not do.  An infinity or NaN in q, k, v, a gate or a
- * state reaches what it reaches by the formulas, of its own token and later ones;
- * from there on the chunks may have NaN where the formulas have an infinity. */
+ * 4096 M, which a stable rule (beta |k|^2 <= 2) does not do.  An infinity or NaN
+ * in q, k, v, a gate or a state reaches what it reaches by the formulas, of its own
+ * token and later ones; from there on the chunks may have NaN where the formulas
+ * have an infinity.  The call's second launch reads what its first wrote into the
+ * workspace: no other call may use it between them. */
 int mcv_delta_rule(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                    const void* v, int64_t v_row, int64_t v_head, const void* g, int64_t g_row, const void* beta,
                    int64_t beta_row, const void* state, void* state_out, const void* state_index, int64_t n_states,

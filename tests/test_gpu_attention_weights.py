@@ -8,7 +8,7 @@ import math
 
 import pytest
 
-from test_gpu_mixers import H, _attn_case, _attn_ref, _gen
+from test_gpu_mixers import H, _attn_case, _attn_ref
 
 pytestmark = pytest.mark.gpu
 
