@@ -84,6 +84,61 @@ int mcv_paged_attention(const void* q, int64_t q_row, int64_t q_head, const void
                         int64_t workspace_bytes, mcv_stream_t stream);
 int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seq_len);
 
+/* Attention of chunks of new tokens over a paged cache that holds them already:
+ * sequence b has the n = cu[b + 1] - cu[b] rows cu[b] .. of q, its last n tokens.
+ * Its token i, at place seq_lens[b] - n + i, sees the tokens up to and with itself:
+ *   out[row][h] = sum_t softmax_t(scale q[row][h] . K[t][h / (Hq / Hkv)]) V[t][..]
+ *   q, out  fp16 [T][Hq][D] (q: row and head strides; out contiguous)
+ *   caches, block_table, seq_lens, max_seq_len  as for mcv_paged_attention
+ *   cu_seqlens  int32 [B + 1], values clamped to [0, T]; rows of no sequence are left
+ *           as they are.  NULL: T / B rows each (T % B == 0)
+ * A row that sees nothing (seq_lens[b] < n, or its pages are not there) gives zeros.  An
+ * infinity or NaN reaches the rows that see its token and no others.  The softmax is in 32
+ * bits; its weights are rounded to fp16, which leaves those below 2^-39 of a row's
+ * largest out.
+ * Where the rows are few the cache is split over workgroups, whose parts a second
+ * launch joins in order (deterministic): workspace of
+ * mcv_paged_attention_chunk_workspace_bytes bytes, 256-byte aligned, of any content,
+ * that no other call uses between the two launches (NULL or too small: no split).  The
+ * bytes for a T and a max_seq_len are enough for any smaller ones. */
+int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
+                              int64_t k_token, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_token,
+                              int64_t v_head, int64_t pages, int64_t page_size, const void* block_table,
+                              int64_t table_row, int64_t table_width, const void* seq_lens, int64_t max_seq_len,
+                              const void* cu_seqlens, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                              double scale, void* out, void* workspace, int64_t workspace_bytes, mcv_stream_t stream);
+int64_t mcv_paged_attention_chunk_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                                  int64_t max_seq_len);
+
+/* --------------------------------------------------- pages of the sequences -- */
+/* Room for new tokens: sequence b, of seq_lens[b] tokens, gets the n rows cu[b] ..
+ * cu[b + 1] - 1 of a packed batch as its next tokens.
+ *   block_table  int32 [B][width] (row stride): sequence b's pages in order; the
+ *           first ceil(seq_lens[b] / page_size) are there, the new ones are written
+ *   seq_lens  int32 [B], clamped to [0, width * page_size]
+ *   cu_seqlens  int32 [B + 1], ascending; NULL: T / B rows each (T % B == 0)
+ *   free_pages  int32 [free_capacity], free_count int32 [1]: a stack of free pages.  New
+ *           pages come from its top, sequence by sequence.  NULL: every page is in the
+ *           table already
+ *   slots  int64 [T]: page * page_size + place in it (mcv_rotary_axes_cached's); -1 for
+ *           a row of no sequence and for a token that has no room
+ *   positions  int64 [T]: the token's place in its sequence, 0 for a row of none
+ *   seq_lens_out  int32 [B]: lengths with the new tokens that have room (a table row
+ *           is width * page_size tokens); may be seq_lens
+ *   free_count_out  int32 [1]: pages left; below zero: so many were lacking, and the
+ *           last sequences' last tokens have no room.  May be free_count */
+int mcv_paged_append(void* block_table, int64_t table_row, int64_t table_width, const void* seq_lens,
+                     const void* cu_seqlens, int64_t B, int64_t T, int64_t page_size, const void* free_pages,
+                     int64_t free_capacity, const void* free_count, void* slots, void* positions, void* seq_lens_out,
+                     void* free_count_out, mcv_stream_t stream);
+/* The reverse: sequence b keeps its first keep[b] tokens (int32 [B], clamped to [0,
+ * seq_lens[b]]; NULL: none), and the pages behind them go on top of the free list, sequence
+ * by sequence.  Table entries stay.  seq_lens_out may be seq_lens or keep.  free_count_out above free_capacity: so many pages did
+ * not fit and are lost (as when a page is given back twice). */
+int mcv_paged_truncate(const void* block_table, int64_t table_row, int64_t table_width, const void* seq_lens,
+                       const void* keep, int64_t B, int64_t page_size, void* free_pages, int64_t free_capacity,
+                       const void* free_count, void* seq_lens_out, void* free_count_out, mcv_stream_t stream);
+
 /* ------------------------------------------------------- rotary positions -- */
 /* Rotary positions with several axes (time, height, width): the pair (x[i],
  * x[i + rot / 2]) of a head's first `rot` elements turns by

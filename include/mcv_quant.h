@@ -615,6 +615,20 @@ int mcv_argmax_f16(const void* x_dev, int64_t M, int64_t N, int64_t* idx_dev,
 int mcv_rms_norm(const void* x_dev, const void* gamma_dev, int64_t M, int64_t H, double eps, void* out_dev,
                  mcv_stream_t stream);
 
+/* The residual row's addition and the norm behind it in one launch: sum = fp16 RNE(x +
+ * residual), out = mcv_rms_norm of sum, to the bit.
+ *   x, residual, sum  fp16 [M][H] with row strides in elements; sum may be x or residual
+ *   out  fp16 [M][H] contiguous; may be x where x is contiguous and sum is elsewhere
+ * Pointers need fp16's alignment only; 16-byte accesses are used where all rows allow them. */
+int mcv_rms_norm_add(const void* x_dev, int64_t x_row, const void* residual_dev, int64_t residual_row,
+                     const void* gamma_dev, int64_t M, int64_t H, double eps, void* sum_dev, int64_t sum_row,
+                     void* out_dev, mcv_stream_t stream);
+/* The same with the normed row's int8 values and scales, as mcv_rms_norm_w8a8_quantize of sum. */
+int mcv_rms_norm_add_w8a8_quantize(const void* x_dev, int64_t x_row, const void* residual_dev, int64_t residual_row,
+                                   const void* gamma_dev, int64_t M, int64_t H, double eps, void* sum_dev,
+                                   int64_t sum_row, void* normed_dev, int8_t* xq_dev, float* x_scale_f32_dev,
+                                   void* x_scale_f16_dev, mcv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

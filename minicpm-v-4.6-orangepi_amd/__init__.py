@@ -125,6 +125,9 @@ _SIGS = {
     "mcv_argmax_f16": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp]),
     "mcv_rms_norm": (_c_int, [_vp, _vp, _c_i64, _c_i64, ctypes.c_double, _vp, _vp]),
     "mcv_rms_norm_w8a8_quantize": (_c_int, [_vp, _vp, _c_i64, _c_i64, ctypes.c_double, _vp, _vp, _vp, _vp, _vp]),
+    "mcv_rms_norm_add": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, ctypes.c_double, _vp, _c_i64, _vp, _vp]),
+    "mcv_rms_norm_add_w8a8_quantize": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, ctypes.c_double, _vp, _c_i64,
+                                                *[_vp] * 5]),
     # include/mcv_mixers.h; a strided operand is a pointer and its strides
     "mcv_delta_rule": (_c_int, [*[_vp, _c_i64, _c_i64] * 3, *[_vp, _c_i64] * 2, _vp, _vp, _vp, _c_i64, _vp, *[_c_i64] * 6,
                                 ctypes.c_double, _c_int, _vp, _vp, _c_i64, _vp]),
@@ -132,6 +135,12 @@ _SIGS = {
     "mcv_paged_attention": (_c_int, [_vp, _c_i64, _c_i64, *[_vp, _c_i64, _c_i64, _c_i64] * 2, _c_i64, _c_i64,
                                      _vp, _c_i64, _c_i64, _vp, *[_c_i64] * 5, ctypes.c_double, _vp, _vp, _c_i64, _vp]),
     "mcv_paged_attention_workspace_bytes": (_c_i64, [_c_i64] * 5),
+    "mcv_paged_attention_chunk": (_c_int, [_vp, _c_i64, _c_i64, *[_vp, _c_i64, _c_i64, _c_i64] * 2, _c_i64, _c_i64,
+                                           _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, *[_c_i64] * 5, ctypes.c_double, _vp, _vp,
+                                           _c_i64, _vp]),
+    "mcv_paged_attention_chunk_workspace_bytes": (_c_i64, [_c_i64] * 6),
+    "mcv_paged_append": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, *[_vp] * 6]),
+    "mcv_paged_truncate": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, *[_vp] * 4]),
     "mcv_rotary_axes": (_c_int, [*[_vp, _c_i64, _c_i64] * 3, _c_i64, _vp, _vp, *[_c_i64] * 5, *[_vp, _c_i64, _c_i64] * 2,
                                  _vp]),
     "mcv_rotary_axes_cached": (_c_int, [*[_vp, _c_i64, _c_i64] * 4, _c_i64, _vp, _vp, *[_c_i64] * 5, _vp, _c_i64, _c_i64,
@@ -1152,9 +1161,24 @@ def rms_norm_w8a8_quantize(x, gamma, eps: float, normed=None, want_normed: bool 
     return normed, xq, xs, x_scale_f16
 
 
+def rms_norm_add(x, residual, gamma, eps: float, *, out=None, residual_out=None, stream=None):
+    """The residual row's addition and the norm behind it in one launch: residual_out = x + residual (fp16),
+    out = rms_norm(residual_out, gamma, eps), to the bit.  x and residual fp16 [M, H] with contiguous rows of any
+    stride; residual_out may be x or residual.  Returns (out, residual_out)."""
+    return mixers.binding().norm_add(x, residual, gamma, eps, out, residual_out, stream)
+
+
+def rms_norm_add_w8a8_quantize(x, residual, gamma, eps: float, *, normed=None, want_normed: bool = True, x_scale_f16=None,
+                               residual_out=None, stream=None):
+    """rms_norm_add with the normed rows' int8 values and scales, as rms_norm_w8a8_quantize gives them.  Returns
+    (normed fp16 [M, H] or None, x_int8 [M, H], x_scale fp32 [M], x_scale_f16 or None, residual_out)."""
+    return mixers.binding().norm_add_quantize(x, residual, gamma, eps, normed, want_normed, x_scale_f16, residual_out, stream)
+
+
 def version() -> str:
     return lib().mcv_version().decode()
 
 
-from .mixers import (gated_delta_rule, gated_delta_rule_step, paged_attention_decode, rotary_axes,  # noqa: E402,F401
-                     rotary_axes_cached, rotary_axes_table)
+from . import mixers  # noqa: E402
+from .mixers import (gated_delta_rule, gated_delta_rule_step, paged_append, paged_attention_chunk,  # noqa: E402,F401
+                     paged_attention_decode, paged_truncate, rotary_axes, rotary_axes_cached, rotary_axes_table)

@@ -1,4 +1,4 @@
-// mixers_ext.cpp -- the token mixers' Python calls (mixers.py), from torch tensors to the C-ABI.
+// mixers_ext.cpp -- the token mixers' Python calls (mixers.py) and the residual norm's, from torch tensors to the C-ABI.
 //
 // One decoded token's mixers run 3 to 5 us each on the GPU, so the host's part of a call
 // is what counts: the same checks written in Python with a ctypes call of thirty
@@ -134,7 +134,8 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& l
     PyObject* shape = PyTuple_New(static_cast<Py_ssize_t>(sizes.size()));
     if (!shape) throw Failed{};
     for (size_t i = 0; i < sizes.size(); ++i) PyTuple_SET_ITEM(shape, i, PyLong_FromLongLong(sizes[i]));
-    PyObject* made = PyObject_CallFunction(g_empty_on, "NisO", shape, int(type == at::kFloat), like.device().str().c_str(), stream);
+    const int kind = type == at::kHalf ? 0 : type == at::kFloat ? 1 : type == at::kChar ? 2 : 3;
+    PyObject* made = PyObject_CallFunction(g_empty_on, "NisO", shape, kind, like.device().str().c_str(), stream);
     if (!made) throw Failed{};
     const at::Tensor t = THPVariable_Unpack(made);
     Py_DECREF(made);
@@ -266,6 +267,179 @@ PyObject* paged(PyObject* const* a) {
     return wrapped(out);
 }
 
+// Contiguous int32 of n entries.
+void* ints(const char* who, const char* name, const at::Tensor& t, int64_t n) {
+    if (t.scalar_type() != at::kInt || !is_shape(t, {n}) || !t.is_contiguous())
+        refuse("%s: %s must be contiguous int32 [%lld], got %s %s", who, name, (long long)n, c10::toString(t.scalar_type()), shape(t).c_str());
+    return t.data_ptr();
+}
+// int32 [B][width] with contiguous rows.
+void check_table(const char* who, const at::Tensor& t, int64_t B) {
+    if (t.scalar_type() != at::kInt || t.dim() != 2 || t.size(0) != B || (t.size(1) > 1 && t.stride(1) != 1))
+        refuse("%s: block_table must be int32 [%lld, width] with contiguous rows", who, (long long)B);
+}
+int64_t whole(PyObject* o) {
+    const int64_t v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw Failed{};
+    return v;
+}
+
+// (q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, stream) -> out
+PyObject* chunk(PyObject* const* a) {
+    const char* who = "paged_attention_chunk";
+    const at::Tensor &q = tensor(who, "q", a[0]), &kc = tensor(who, "k_cache", a[1]), &vc = tensor(who, "v_cache", a[2]);
+    const at::Tensor &table = tensor(who, "block_table", a[3]), &lens = tensor(who, "seq_lens", a[4]);
+    const at::Tensor *cu = maybe(who, "cu_seqlens", a[5]), *given = maybe(who, "out", a[8]);
+    if (q.dim() != 3 || kc.dim() != 4) refuse("%s: q must be [T, Hq, D] and the caches [pages, page_size, Hkv, D]", who);
+    const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), pages = kc.size(0), page = kc.size(1), Hkv = kc.size(2), B = lens.numel();
+    const Heads qa = heads(who, "q", q, T);
+    const Cache ka = cache(who, "k_cache", kc, kc, Hkv, D), va = cache(who, "v_cache", vc, kc, Hkv, D);
+    ints(who, "seq_lens", lens, B);
+    check_table(who, table, B);
+    if (cu) ints(who, "cu_seqlens", *cu, B + 1);
+    else if (B ? T % B != 0 : T != 0) refuse("%s: %lld rows for %lld sequences need cu_seqlens", who, (long long)T, (long long)B);
+    if (given && (given->scalar_type() != at::kHalf || given->sizes() != q.sizes() || !given->is_contiguous()))
+        refuse("%s: out must be contiguous fp16 %s", who, shape(q).c_str());
+    same_device(who, q, {&kc, &vc, &table, &lens, cu, given});
+    const int64_t most = a[7] == Py_None ? table.size(1) * page : whole(a[7]);
+    const auto device = on_gpu(who, q);
+    const mcv_stream_t h = handle(a[9]);
+    const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q, a[9], h);
+    if (B == 0 || T == 0) {                      // nothing to launch, of shapes that a batch would be taken of
+        if (Hq == 0 || Hkv == 0 || Hq % Hkv != 0 || (D != 64 && D != 128 && D != 256) || page == 0 || page % 16 != 0)
+            refuse("%s: bad shape q %s, caches %s", who, shape(q).c_str(), shape(kc).c_str());
+        return wrapped(out);
+    }
+    const int64_t bytes = mcv_paged_attention_chunk_workspace_bytes(B, T, Hq, Hkv, D, most);
+    void* ws = bytes ? delta_workspace(bytes, q, a[9], h) : nullptr;
+    check(mcv_paged_attention_chunk(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
+                                    table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), most, ptr(cu), B, T, Hq, Hkv, D,
+                                    number(a[6], 1.0 / std::sqrt(static_cast<double>(D))), out.data_ptr(), ws, ws ? bytes : 0, h),
+          who);
+    return wrapped(out);
+}
+
+// (block_table, seq_lens, cu_seqlens, page_size, tokens, free_pages, free_count, seq_lens_out, free_count_out, slots, positions,
+// stream) -> (slots, positions, seq_lens_out)
+PyObject* append(PyObject* const* a) {
+    const char* who = "paged_append";
+    const at::Tensor &table = tensor(who, "block_table", a[0]), &lens = tensor(who, "seq_lens", a[1]);
+    const at::Tensor *cu = maybe(who, "cu_seqlens", a[2]), *free = maybe(who, "free_pages", a[5]), *count = maybe(who, "free_count", a[6]);
+    const at::Tensor *lens_given = maybe(who, "seq_lens_out", a[7]), *count_given = maybe(who, "free_count_out", a[8]);
+    const at::Tensor *slots_given = maybe(who, "slots", a[9]), *positions_given = maybe(who, "positions", a[10]);
+    const int64_t page = whole(a[3]), B = lens.numel();
+    const int64_t T = a[4] != Py_None ? whole(a[4]) : slots_given ? slots_given->numel() : B;
+    if (T < 0) refuse("%s: tokens must not be negative (tokens=%lld)", who, (long long)T);
+    ints(who, "seq_lens", lens, B);
+    check_table(who, table, B);
+    if (cu) ints(who, "cu_seqlens", *cu, B + 1);
+    else if (B ? T % B != 0 : T != 0) refuse("%s: %lld rows for %lld sequences need cu_seqlens", who, (long long)T, (long long)B);
+    if (!free != !count) refuse("%s: free_pages and free_count come together", who);
+    if (free) ints(who, "free_pages", *free, free->numel()), ints(who, "free_count", *count, 1);
+    if (lens_given) ints(who, "seq_lens_out", *lens_given, B);
+    if (count_given) ints(who, "free_count_out", *count_given, 1);
+    for (const at::Tensor* t : {slots_given, positions_given})
+        if (t && (t->scalar_type() != at::kLong || !is_shape(*t, {T}) || !t->is_contiguous()))
+            refuse("%s: %s must be contiguous int64 [%lld]", who, t == slots_given ? "slots" : "positions", (long long)T);
+    same_device(who, table, {&lens, cu, free, count, lens_given, count_given, slots_given, positions_given});
+    const auto device = on_gpu(who, table);
+    const mcv_stream_t h = handle(a[11]);
+    const at::Tensor slots = slots_given ? *slots_given : fresh({T}, at::kLong, table, a[11], h);
+    const at::Tensor positions = positions_given ? *positions_given : fresh({T}, at::kLong, table, a[11], h);
+    const at::Tensor lens_out = lens_given ? *lens_given : lens;
+    if (B == 0) {
+        if (T) refuse("%s: %lld rows of no sequence", who, (long long)T);
+        if (count_given) refuse("%s: no sequences, and a free_count_out to write", who);
+    } else {
+        check(mcv_paged_append(table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), ptr(cu), B, T, page, ptr(free),
+                               free ? free->numel() : 0, ptr(count), slots.data_ptr(), positions.data_ptr(), lens_out.data_ptr(),
+                               ptr(count_given ? count_given : count), h),
+              who);
+    }
+    return Py_BuildValue("(NNN)", wrapped(slots), wrapped(positions), wrapped(lens_out));
+}
+
+// (block_table, seq_lens, keep, page_size, free_pages, free_count, seq_lens_out, free_count_out, stream) -> seq_lens_out
+PyObject* truncate(PyObject* const* a) {
+    const char* who = "paged_truncate";
+    const at::Tensor &table = tensor(who, "block_table", a[0]), &lens = tensor(who, "seq_lens", a[1]);
+    const at::Tensor* keep = maybe(who, "keep", a[2]);
+    const at::Tensor &free = tensor(who, "free_pages", a[4]), &count = tensor(who, "free_count", a[5]);
+    const at::Tensor *lens_given = maybe(who, "seq_lens_out", a[6]), *count_given = maybe(who, "free_count_out", a[7]);
+    const int64_t page = whole(a[3]), B = lens.numel();
+    ints(who, "seq_lens", lens, B);
+    check_table(who, table, B);
+    if (keep) ints(who, "keep", *keep, B);
+    ints(who, "free_pages", free, free.numel());
+    ints(who, "free_count", count, 1);
+    if (lens_given) ints(who, "seq_lens_out", *lens_given, B);
+    if (count_given) ints(who, "free_count_out", *count_given, 1);
+    same_device(who, table, {&lens, keep, &free, &count, lens_given, count_given});
+    const auto device = on_gpu(who, table);
+    const at::Tensor& lens_out = lens_given ? *lens_given : lens;
+    if (B == 0) {
+        if (count_given) refuse("%s: no sequences, and a free_count_out to write", who);
+    } else {
+        check(mcv_paged_truncate(table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), ptr(keep), B, page, free.data_ptr(), free.numel(),
+                                 count.data_ptr(), lens_out.data_ptr(), (count_given ? *count_given : count).data_ptr(), handle(a[8])),
+              who);
+    }
+    return wrapped(lens_out);
+}
+
+// fp16 [M][H] with contiguous rows.
+void check_rows(const char* who, const char* name, const at::Tensor& t, int64_t M, int64_t H, bool contiguous) {
+    if (t.scalar_type() != at::kHalf || !is_shape(t, {M, H}) || (H > 1 && t.stride(1) != 1) || (contiguous && !t.is_contiguous()))
+        refuse("%s: %s must be fp16 [%lld, %lld] %s, got %s %s", who, name, (long long)M, (long long)H, contiguous ? "and contiguous" : "with contiguous rows",
+               c10::toString(t.scalar_type()), shape(t).c_str());
+}
+
+// (x, residual, gamma, eps, out, residual_out, stream) -> (out, residual_out), or
+// (x, residual, gamma, eps, normed, want_normed, x_scale_f16, residual_out, stream) -> (normed, x_int8, x_scale, x_scale_f16, residual_out)
+PyObject* norm_add(PyObject* const* a, bool quantize) {
+    const char* who = quantize ? "rms_norm_add_w8a8_quantize" : "rms_norm_add";
+    const at::Tensor &x = tensor(who, "x", a[0]), &residual = tensor(who, "residual", a[1]), &gamma = tensor(who, "gamma", a[2]);
+    const double eps = number(a[3], 0.0);
+    const at::Tensor* given = maybe(who, quantize ? "normed" : "out", a[4]);
+    const at::Tensor* scale16 = quantize ? maybe(who, "x_scale_f16", a[6]) : nullptr;
+    const at::Tensor* sum_given = maybe(who, "residual_out", a[quantize ? 7 : 5]);
+    PyObject* const stream = a[quantize ? 8 : 6];
+    if (x.dim() != 2) refuse("%s: x must be fp16 [M, H], got %s", who, shape(x).c_str());
+    const int64_t M = x.size(0), H = x.size(1);
+    check_rows(who, "x", x, M, H, false);
+    check_rows(who, "residual", residual, M, H, false);
+    if (sum_given) check_rows(who, "residual_out", *sum_given, M, H, false);
+    if (given) check_rows(who, quantize ? "normed" : "out", *given, M, H, true);
+    if (gamma.scalar_type() != at::kHalf || !is_shape(gamma, {H}) || !gamma.is_contiguous()) refuse("%s: gamma must be contiguous fp16 [%lld]", who, (long long)H);
+    if (scale16 && (scale16->scalar_type() != at::kHalf || scale16->numel() != M || !scale16->is_contiguous()))
+        refuse("%s: x_scale_f16 must be contiguous fp16 [%lld]", who, (long long)M);
+    same_device(who, x, {&residual, &gamma, given, sum_given, scale16});
+    const auto device = on_gpu(who, x);
+    const mcv_stream_t h = handle(stream);
+    const bool want = !quantize || given || truth(a[5]);
+    const at::Tensor out = given ? *given : want ? fresh({M, H}, at::kHalf, x, stream, h) : at::Tensor();
+    const at::Tensor sum = sum_given ? *sum_given : fresh({M, H}, at::kHalf, x, stream, h);
+    if (!quantize) {
+        if (M)
+            check(mcv_rms_norm_add(x.data_ptr(), stride_of(x, 0), residual.data_ptr(), stride_of(residual, 0), gamma.data_ptr(), M, H, eps, sum.data_ptr(),
+                                   stride_of(sum, 0), out.data_ptr(), h),
+                  who);
+        return Py_BuildValue("(NN)", wrapped(out), wrapped(sum));
+    }
+    const at::Tensor q = fresh({M, H}, at::kChar, x, stream, h), scale = fresh({M}, at::kFloat, x, stream, h);
+    if (M)
+        check(mcv_rms_norm_add_w8a8_quantize(x.data_ptr(), stride_of(x, 0), residual.data_ptr(), stride_of(residual, 0), gamma.data_ptr(), M, H, eps,
+                                             sum.data_ptr(), stride_of(sum, 0), want ? out.data_ptr() : nullptr, static_cast<int8_t*>(q.data_ptr()),
+                                             static_cast<float*>(scale.data_ptr()), ptr(scale16), h),
+              who);
+    auto or_none = [](const at::Tensor* t) {
+        if (t) return wrapped(*t);
+        Py_INCREF(Py_None);
+        return Py_None;
+    };
+    return Py_BuildValue("(NNNNN)", or_none(want ? &out : nullptr), wrapped(q), wrapped(scale), or_none(scale16), wrapped(sum));
+}
+
 // (q, k, positions, freq, axis, q_out, k_out, stream) -> (q_out, k_out), or
 // (q, k, positions, freq, axis, q_out, v, k_cache, v_cache, slots, stream) -> q_out
 PyObject* rotary(PyObject* const* a, bool cached) {
@@ -338,6 +512,11 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F f) {
 
 PyObject* py_delta(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 15, [&] { return delta(a); }); }
 PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 9, [&] { return paged(a); }); }
+PyObject* py_chunk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 10, [&] { return chunk(a); }); }
+PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 12, [&] { return append(a); }); }
+PyObject* py_truncate(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 9, [&] { return truncate(a); }); }
+PyObject* py_norm_add(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 7, [&] { return norm_add(a, false); }); }
+PyObject* py_norm_add_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 9, [&] { return norm_add(a, true); }); }
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 8, [&] { return rotary(a, false); }); }
 PyObject* py_rotary_cached(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 11, [&] { return rotary(a, true); }); }
 
@@ -368,6 +547,11 @@ PyCFunction method(F* f) {
 PyMethodDef methods[] = {{"bind", py_bind, METH_VARARGS, nullptr},
                          {"delta", method(py_delta), METH_FASTCALL, nullptr},
                          {"paged", method(py_paged), METH_FASTCALL, nullptr},
+                         {"chunk", method(py_chunk), METH_FASTCALL, nullptr},
+                         {"append", method(py_append), METH_FASTCALL, nullptr},
+                         {"truncate", method(py_truncate), METH_FASTCALL, nullptr},
+                         {"norm_add", method(py_norm_add), METH_FASTCALL, nullptr},
+                         {"norm_add_quantize", method(py_norm_add_quantize), METH_FASTCALL, nullptr},
                          {"rotary", method(py_rotary), METH_FASTCALL, nullptr},
                          {"rotary_cached", method(py_rotary_cached), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

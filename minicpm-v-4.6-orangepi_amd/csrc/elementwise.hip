@@ -174,3 +174,59 @@ extern "C" int mcv_rms_norm(const void* x, const void* gamma, int64_t M, int64_t
                       static_cast<uint16_t*>(out), nullptr, nullptr, nullptr, static_cast<hipStream_t>(stream));
     return check_launch("rms_row_kernel");
 }
+
+namespace mcv {
+namespace {
+
+int check_add(const char* who, const void* x, const void* gamma, int64_t M, int64_t H, double eps, const AddRows& add, const void* normed) {
+    if (!x || !gamma || !add.other || !add.sum) return fail(MCV_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (M <= 0 || H <= 0 || M > 0x7fffffff || H > 0x7fffffff || !(eps >= 0.0))
+        return fail(MCV_ERR_SHAPE, "%s: bad shape M=%lld H=%lld or eps", who, (long long)M, (long long)H);
+    if (add.x_row < 0 || add.other_row < 0 || (M > 1 && add.sum_row < H))
+        return fail(MCV_ERR_SHAPE, "%s: bad row stride x=%lld residual=%lld sum=%lld (H=%lld)", who, (long long)add.x_row, (long long)add.other_row,
+                    (long long)add.sum_row, (long long)H);
+    // a row is read by the workgroup that writes it and by no other
+    auto overlap = [&](const void* a, int64_t a_row, const void* b, int64_t b_row) {
+        const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+        return p < q + 2 * ((M - 1) * b_row + H) && q < p + 2 * ((M - 1) * a_row + H);
+    };
+    auto apart = [&](const void* in, int64_t in_row, const void* out, int64_t out_row) {
+        if (!overlap(in, in_row, out, out_row) || (in == out && (in_row == out_row || M == 1))) return true;
+        // columns beside one another of rows of one width
+        const int64_t bytes = static_cast<int64_t>(reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out));
+        if (in_row != out_row || in_row < 2 * H || bytes % 2 != 0) return false;
+        const int64_t off = (bytes / 2 % in_row + in_row) % in_row;
+        return off >= H && in_row - off >= H;
+    };
+    if (!apart(x, add.x_row, add.sum, add.sum_row) || !apart(add.other, add.other_row, add.sum, add.sum_row))
+        return fail(MCV_ERR_INVALID_ARG, "%s: sum overlaps an input without being it", who);
+    if (normed && (overlap(normed, H, add.sum, add.sum_row) || !apart(x, add.x_row, normed, H) || !apart(add.other, add.other_row, normed, H)))
+        return fail(MCV_ERR_INVALID_ARG, "%s: the normed rows overlap the sum, or an input without being it", who);
+    return require_device();
+}
+
+}  // namespace
+}  // namespace mcv
+
+extern "C" int mcv_rms_norm_add(const void* x, int64_t x_row, const void* residual, int64_t residual_row, const void* gamma, int64_t M, int64_t H,
+                                double eps, void* sum, int64_t sum_row, void* out, mcv_stream_t stream) {
+    const AddRows add{static_cast<const uint16_t*>(residual), static_cast<uint16_t*>(sum), x_row, residual_row, sum_row};
+    if (!out) return fail(MCV_ERR_INVALID_ARG, "rms_norm_add: null pointer");
+    int rc = check_add("rms_norm_add", x, gamma, M, H, eps, add, out);
+    if (rc != MCV_OK) return rc;
+    launch_rms<false, true>(static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(gamma), M, H, static_cast<float>(eps),
+                            static_cast<uint16_t*>(out), nullptr, nullptr, nullptr, static_cast<hipStream_t>(stream), add);
+    return check_launch("rms_row_kernel<add>");
+}
+
+extern "C" int mcv_rms_norm_add_w8a8_quantize(const void* x, int64_t x_row, const void* residual, int64_t residual_row, const void* gamma, int64_t M,
+                                              int64_t H, double eps, void* sum, int64_t sum_row, void* normed, int8_t* xq, float* s32, void* s16,
+                                              mcv_stream_t stream) {
+    const AddRows add{static_cast<const uint16_t*>(residual), static_cast<uint16_t*>(sum), x_row, residual_row, sum_row};
+    if (!xq || (!s32 && !s16)) return fail(MCV_ERR_INVALID_ARG, "rms_norm_add_w8a8_quantize: null pointer");
+    int rc = check_add("rms_norm_add_w8a8_quantize", x, gamma, M, H, eps, add, normed);
+    if (rc != MCV_OK) return rc;
+    launch_rms<true, true>(static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(gamma), M, H, static_cast<float>(eps),
+                           static_cast<uint16_t*>(normed), xq, s32, static_cast<uint16_t*>(s16), static_cast<hipStream_t>(stream), add);
+    return check_launch("rms_row_kernel<add, quantise>");
+}

@@ -1,5 +1,6 @@
 // row_norm.h -- RMSNorm of fp16 rows, alone (elementwise.hip) or followed by
-// the W8A8 activation quantisation (w8a8.hip); one 256-thread workgroup per row.
+// the W8A8 activation quantisation (w8a8.hip), and either of them of the sum of two
+// rows; one 256-thread workgroup per row.
 #pragma once
 
 #include "common.h"
@@ -30,6 +31,23 @@ __device__ __forceinline__ uint4 rms_chunk(const uint4& x, const uint4& g, float
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// fp16 RNE(a + b).  In 32 bits first, whose 24 bits are enough for the second rounding to find what one would.
+__device__ __forceinline__ uint16_t add_f16(uint16_t a, uint16_t b) { return f2h(__fadd_rn(h2f(a), h2f(b))); }
+__device__ __forceinline__ uint4 add_chunk(const uint4& a, const uint4& b) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+        w[e / 2] = add_f16(chunk_get(a, e), chunk_get(b, e)) | (static_cast<uint32_t>(add_f16(chunk_get(a, e + 1), chunk_get(b, e + 1))) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The other row of a sum, and where the sum goes (either row, or a row of its own); elements from row to row.
+struct AddRows {
+    const uint16_t* other;
+    uint16_t* sum;
+    int64_t x_row, other_row, sum_row;
+};
+
 // normed = fp16((x * rstd) * gamma), rstd = 1 / sqrt(mean(x^2) + eps); QUANT:
 // then the row's int8 values and scale, from the same fp16 values.  Every step
 // is an explicitly rounded fp32 operation, and thread t sums the squares of
@@ -45,14 +63,18 @@ __device__ __forceinline__ uint4 rms_chunk(const uint4& x, const uint4& g, float
 // quantisation M=1 H=1024 3.5 / 3.1, H=2048 4.9 / 3.5.  PER = 0: rows longer than
 // 256 * 32, strided loops, each with only the loads and stores it needs (with the
 // store conditional inside: M=1 H=16384 27.8 us, now 26.3, as before PER).
-template <int PER, bool VEC, bool QUANT>
+// ADD: the row is fp16(x + other), which goes to `sum` too; normed and int8 are what
+// they are for a row that holds it.
+template <int PER, bool VEC, bool QUANT, bool ADD = false>
 __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ gamma,
                                                       int H, float eps, uint16_t* __restrict__ normed,
                                                       int8_t* __restrict__ xq, float* __restrict__ s32,
-                                                      uint16_t* __restrict__ s16) {
+                                                      uint16_t* __restrict__ s16, AddRows add) {
     const int row = blockIdx.x;
     const int t = threadIdx.x;
-    const uint16_t* xr = x + static_cast<size_t>(row) * H;
+    const uint16_t* xr = x + (ADD ? row * add.x_row : static_cast<int64_t>(row) * H);
+    const uint16_t* ar = ADD ? add.other + row * add.other_row : nullptr;
+    uint16_t* sr = ADD ? add.sum + row * add.sum_row : nullptr;
     uint16_t* nr = normed ? normed + static_cast<size_t>(row) * H : nullptr;
     int8_t* qr = QUANT ? xq + static_cast<size_t>(row) * H : nullptr;
     float m = 0.f;
@@ -61,10 +83,13 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
         constexpr int NC = VEC ? (PER + 7) / 8 : 1;
         uint16_t xs[PER], gs[VEC ? 1 : PER];
         uint4 xv[NC], gv[NC];
+        uint16_t as[ADD ? PER : 1];
+        uint4 av[ADD ? NC : 1];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = t + 256 * j;
             xs[j] = i < H ? xr[i] : uint16_t(0);
+            if constexpr (ADD) as[j] = i < H ? ar[i] : uint16_t(0);
             if constexpr (!VEC) gs[j] = i < H ? gamma[i] : uint16_t(0);
         }
         if constexpr (VEC)
@@ -72,10 +97,14 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
             for (int c = 0; c < NC; ++c) {
                 const int i = 8 * (t + 256 * c);
                 xv[c] = i < H ? *reinterpret_cast<const uint4*>(xr + i) : make_uint4(0, 0, 0, 0);
+                if constexpr (ADD) av[c] = i < H ? *reinterpret_cast<const uint4*>(ar + i) : make_uint4(0, 0, 0, 0);
                 gv[c] = i < H ? *reinterpret_cast<const uint4*>(gamma + i) : make_uint4(0, 0, 0, 0);
             }
-        // x may be `normed`: no load may be in flight when another thread stores
+        // x may be `normed` (or the sum's place): no load may be in flight when another thread stores
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (ADD)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) xs[j] = add_f16(xs[j], as[j]);
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -87,6 +116,10 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int i = 8 * (t + 256 * c);
+                if constexpr (ADD) {
+                    xv[c] = add_chunk(xv[c], av[c]);
+                    if (i < H) *reinterpret_cast<uint4*>(sr + i) = xv[c];
+                }
                 xv[c] = rms_chunk<QUANT>(xv[c], gv[c], rstd, m);          // now the normed chunk
                 if (i < H && nr) *reinterpret_cast<uint4*>(nr + i) = xv[c];
             }
@@ -94,6 +127,8 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int i = t + 256 * j;
+                if constexpr (ADD)
+                    if (i < H) sr[i] = xs[j];
                 xs[j] = rms_apply(xs[j], rstd, gs[j]);
                 if (i < H && nr) nr[i] = xs[j];
                 if constexpr (QUANT) {
@@ -120,6 +155,10 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
             }
         }
     } else {
+        if constexpr (ADD) {                     // each thread reads back what it has written itself
+            for (int i = t; i < H; i += blockDim.x) sr[i] = add_f16(xr[i], ar[i]);
+            xr = sr;
+        }
         const float rstd = row_rstd(xr, H, eps);
         if constexpr (!QUANT) {
             for (int i = t; i < H; i += blockDim.x) nr[i] = rms_apply(xr[i], rstd, gamma[i]);
@@ -148,27 +187,29 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
     }
 }
 
-using RmsFn = void (*)(const uint16_t*, const uint16_t*, int, float, uint16_t*, int8_t*, float*, uint16_t*);
+using RmsFn = void (*)(const uint16_t*, const uint16_t*, int, float, uint16_t*, int8_t*, float*, uint16_t*, AddRows);
 
 // Launches the kernel for M rows of H; VEC needs whole 16-byte chunks: H a
 // multiple of 8 and aligned rows, and more than one element a thread: up to 256
 // it loads x twice where the strided form has everything in one load each
 // (M=50000 H=128 33.3 us in chunks, 24.3 strided; M=8192 H=256 7.8 / 6.3).  (A wave per row, without barriers, was slower
 // below 8192 rows: M=512 H=1024 3.9 us against 3.1, M=2000 H=2048 13.6 / 7.9.)
-template <bool QUANT>
+template <bool QUANT, bool ADD = false>
 void launch_rms(const uint16_t* x, const uint16_t* gamma, int64_t M, int64_t H, float eps, uint16_t* normed, int8_t* xq,
-                float* s32, uint16_t* s16, hipStream_t stream) {
+                float* s32, uint16_t* s16, hipStream_t stream, const AddRows& add = {}) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(gamma) |
-                         reinterpret_cast<uintptr_t>(normed) | (reinterpret_cast<uintptr_t>(xq) << 1);
+                         reinterpret_cast<uintptr_t>(normed) | (reinterpret_cast<uintptr_t>(xq) << 1) |
+                         reinterpret_cast<uintptr_t>(add.other) | reinterpret_cast<uintptr_t>(add.sum) |
+                         static_cast<uintptr_t>(2 * (add.x_row | add.other_row | add.sum_row));
     const bool vec = H % 8 == 0 && at % 16 == 0;
     const int h = static_cast<int>(H);
-    RmsFn fn = rms_row_kernel<0, false, QUANT>;
-    if (H <= 256) fn = rms_row_kernel<1, false, QUANT>;
-    else if (H <= 1024) fn = vec ? rms_row_kernel<4, true, QUANT> : rms_row_kernel<4, false, QUANT>;
-    else if (H <= 2048) fn = vec ? rms_row_kernel<8, true, QUANT> : rms_row_kernel<8, false, QUANT>;
-    else if (H <= 4096) fn = vec ? rms_row_kernel<16, true, QUANT> : rms_row_kernel<16, false, QUANT>;
-    else if (H <= 8192) fn = vec ? rms_row_kernel<32, true, QUANT> : rms_row_kernel<32, false, QUANT>;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(M)), dim3(256), 0, stream, x, gamma, h, eps, normed, xq, s32, s16);
+    RmsFn fn = rms_row_kernel<0, false, QUANT, ADD>;
+    if (H <= 256) fn = rms_row_kernel<1, false, QUANT, ADD>;
+    else if (H <= 1024) fn = vec ? rms_row_kernel<4, true, QUANT, ADD> : rms_row_kernel<4, false, QUANT, ADD>;
+    else if (H <= 2048) fn = vec ? rms_row_kernel<8, true, QUANT, ADD> : rms_row_kernel<8, false, QUANT, ADD>;
+    else if (H <= 4096) fn = vec ? rms_row_kernel<16, true, QUANT, ADD> : rms_row_kernel<16, false, QUANT, ADD>;
+    else if (H <= 8192) fn = vec ? rms_row_kernel<32, true, QUANT, ADD> : rms_row_kernel<32, false, QUANT, ADD>;
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(M)), dim3(256), 0, stream, x, gamma, h, eps, normed, xq, s32, s16, add);
 }
 
 }  // namespace mcv

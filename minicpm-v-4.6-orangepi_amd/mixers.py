@@ -1,7 +1,8 @@
 """Token mixers that stand between a decoder layer's quantised projections, over
 the C-ABI in include/mcv_mixers.h: the gated delta rule of the linear-attention
-layers, several-axis rotary positions, and one-token attention over a paged
-key-value cache for the full-attention layers.
+layers, several-axis rotary positions, and attention of one new token or of chunks of
+them over a paged key-value cache for the full-attention layers, whose pages are dealt
+out and taken back on the device.
 
 Activations and caches are fp16, gates and states fp32.  q, k and v may be
 columns of one projection's output: rows and heads have strides, the elements
@@ -38,11 +39,12 @@ def binding():
     return _BINDING
 
 
-def _empty_on(shape, single: bool, device, stream):
-    """An output, fp32 or fp16, of a call on a stream that is not the current one: its memory, so that it is not handed
+def _empty_on(shape, kind: int, device, stream):
+    """An output (0 fp16, 1 fp32, 2 int8, 3 int64) of a call on a stream that is not the current one: its memory, so that it is not handed
     out anew while that stream still writes to it, nor written while the current stream still uses what it was."""
     torch = _torch()
-    make = lambda: torch.empty(shape, dtype=torch.float32 if single else torch.float16, device=device)     # noqa: E731
+    dtype = (torch.float16, torch.float32, torch.int8, torch.int64)[kind]
+    make = lambda: torch.empty(shape, dtype=dtype, device=device)     # noqa: E731
     return _made_on(make, torch.device(device), _stream(stream), stream)
 
 
@@ -105,6 +107,41 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale=
     length 0 gives zeros (and a batch of none an empty result).  max_seq_len, at most width * page_size (the default),
     bounds the lengths.  Returns out fp16 [B, Hq, D]."""
     return (_BINDING or binding()).paged(q, k_cache, v_cache, block_table, seq_lens, scale, max_seq_len, out, stream)
+
+
+def paged_attention_chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens=None, *, scale=None, max_seq_len=None,
+                          out=None, stream=None):
+    """Attention of chunks of new tokens over a paged cache that holds them already (rotary_axes_cached): q fp16 [T, Hq, D],
+    sequence b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device; None: T / B rows each) its last
+    tokens.  Each sees the tokens of its sequence up to and with itself.  Caches, block_table, seq_lens int32 [B] (the new
+    tokens among them) and max_seq_len as for paged_attention_decode.
+
+    Prompts, their chunks and single tokens may share a call.  A row that sees nothing gives zeros, a row of no sequence is
+    left as it is, and so is all of `out` that no row writes.  Returns out fp16 [T, Hq, D]."""
+    return (_BINDING or binding()).chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, stream)
+
+
+def paged_append(block_table, seq_lens, cu_seqlens=None, page_size=16, *, tokens=None, free_pages=None, free_count=None,
+                 seq_lens_out=None, free_count_out=None, slots=None, positions=None, stream=None):
+    """Room in a paged cache for new tokens: sequence b, of seq_lens[b] tokens, gets the rows cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1 of a packed batch of `tokens` rows (None: the rows of `slots`, else one each) as its next.
+
+    Pages that a sequence lacks are taken from the top of the stack free_pages int32 [n], free_count int32 [1] and written
+    into block_table int32 [B, width]; without free_pages the table is complete.  Returns (slots int64 [tokens], where
+    rotary_axes_cached writes each token, -1 for a row of no sequence or a token without room; positions int64 [tokens];
+    seq_lens_out).  seq_lens and free_count are updated in place unless seq_lens_out and free_count_out are given; a
+    count below zero says how many pages were lacking, and lengths then end where the room does."""
+    return (_BINDING or binding()).append(block_table, seq_lens, cu_seqlens, page_size, tokens, free_pages, free_count, seq_lens_out,
+                                          free_count_out, slots, positions, stream)
+
+
+def paged_truncate(block_table, seq_lens, keep, page_size, free_pages, free_count, *, seq_lens_out=None, free_count_out=None,
+                   stream=None):
+    """The reverse of paged_append: sequence b keeps its first keep[b] tokens (int32 [B]; None: no sequence keeps any), and its
+    pages behind them go on top of the free list.  seq_lens and free_count are updated in place unless seq_lens_out and
+    free_count_out are given.  Returns seq_lens_out."""
+    return (_BINDING or binding()).truncate(block_table, seq_lens, keep, page_size, free_pages, free_count, seq_lens_out,
+                                            free_count_out, stream)
 
 
 def rotary_axes_table(rot: int, theta: float, sections, interleaved: bool = True, device="cuda"):
