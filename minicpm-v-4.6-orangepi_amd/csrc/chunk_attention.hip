@@ -1,5 +1,6 @@
 // chunk_attention.hip -- attention of chunks of new tokens over a paged cache, gfx950.
 #include <algorithm>
+#include <cmath>
 
 #include "mixers.h"
 
@@ -7,14 +8,13 @@ namespace mcv {
 namespace {
 
 constexpr int kTile = 64;                        // tokens that are staged and taken at a time
-constexpr int kWaves = 4;
-constexpr int kRowsWave = 32;
-constexpr int kRows = kWaves * kRowsWave;        // (token, head) rows of a workgroup
-constexpr int kLeast = 4 * kTile;                // tokens of a part, at least
+constexpr int kLeast = 2 * kTile;                // tokens of a part, at least
 constexpr int kJoinRows = 16;                    // rows that a workgroup joins
 constexpr int64_t kMaxLen = int64_t(1) << 30;    // tokens of one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kTopLog2 = 15.f;
+// A row's reference exponent m is a whole number, so that what it once stood for is brought to another by an exact product,
+// and is raised only when a score passes it by kRoom: the weights 2^(s - m + kTop) end below fp16's 65504.
+constexpr float kRoom = 6.f, kTop = 9.f;
 
 struct ChunkArgs {
     const uint16_t* q;
@@ -27,9 +27,10 @@ struct ChunkArgs {
     uint8_t* ws;
     int64_t q_row, q_head, k_page, k_head, v_page, v_head, table_row;
     int k_token, v_token, pages, page16, max_len, B, T, Hq, Hkv, group;
-    uint32_t page16_inv;                         // ceil(2^32 / page16), page16 > 1
-    float scale_log2;
-    int slots;                                   // parts to cut for; 0: every tile of rows whole
+    uint32_t page16_inv, group_inv;              // ceil(2^32 / n), n > 1
+    float scale_log2;                            // above zero: a score of -inf stays one
+    float q_by;                                  // 1, -1 or 0: the scale's sign
+    int slots_log2;                              // parts to cut for; -1: every tile of rows whole
     int64_t slot_bytes;
 };
 
@@ -45,52 +46,58 @@ __device__ __forceinline__ float sum2(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// What no kernel in flight writes, at an address that a whole wave shares: read through the scalar cache.
-typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
-__device__ __forceinline__ scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)reinterpret_cast<uintptr_t>(p); }
-
 // ---------------------------------------------------------------- who does what --
 struct Seq {
     int first, n, len;                           // first new row, new tokens, tokens in the cache
 };
 __device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b) {
     if (b >= p.B) return {0, 0, 0};
-    auto row = [&](int i) {
-        const int at = p.cu ? p.cu[i] : i * (p.T / p.B);
-        return at < 0 ? 0 : at > p.T ? p.T : at;
-    };
-    const int first = row(b), n = row(b + 1) - first, len = p.lens[b];
-    return {first, n < 0 ? 0 : n, len < 0 ? 0 : len > p.max_len ? p.max_len : len};
+    int first, next;
+    const int held = p.lens[b];
+    if (p.cu) first = p.cu[b], next = p.cu[b + 1];
+    else first = b * (p.T / p.B), next = first + p.T / p.B;
+    auto inside = [](int v, int most) { return v < 0 ? 0 : v > most ? most : v; };
+    first = inside(first, p.T);
+    next = inside(next, p.T);
+    return {first, next > first ? next - first : 0, inside(held, p.max_len)};
 }
+__device__ __forceinline__ int token_of(const ChunkArgs& p, int row) {         // row / group
+    if (p.group == 1) return row;
+    int t = static_cast<int>(__umulhi(static_cast<uint32_t>(row), p.group_inv));      // one too many at most
+    if (t * static_cast<int64_t>(p.group) > row) --t;
+    return t;
+}
+// R: rows of a tile.
+template <int R>
 __device__ __forceinline__ int tiles_of(const ChunkArgs& p, const Seq& s) {
-    return static_cast<int>((static_cast<int64_t>(s.n) * p.group + kRows - 1) / kRows);
+    return static_cast<int>((static_cast<int64_t>(s.n) * p.group + R - 1) / R);
 }
-// Tokens that the first i tiles of rows read, at most (of one cache head), and that tile i reads.
-__device__ __forceinline__ int64_t reads_below(const ChunkArgs& p, const Seq& s, int64_t i) {
-    const int64_t base = s.len > s.n ? s.len - s.n : 0, step = (kRows + p.group - 1) / p.group;
-    return i * (base + kTile) + step * (i * (i + 1) / 2);
+// Tokens that the first i tiles of rows read, at most (of one cache head).
+template <int R>
+__device__ __forceinline__ int64_t reads_below(const ChunkArgs& p, const Seq& s, int i) {
+    const int base = s.len > s.n ? s.len - s.n : 0, step = token_of(p, R + p.group - 1);
+    return static_cast<int64_t>(i) * (base + kTile) + step * (static_cast<int64_t>(i) * (i + 1) / 2);
 }
 // Tiles of rows that have a part p > 0, which begins at token p S: the last ones.
+template <int R>
 __device__ __forceinline__ int tiles_with(const ChunkArgs& p, const Seq& s, int tiles, int64_t begin) {
     const int64_t x = begin - (s.len - s.n);     // the first new token that sees it
-    return x <= 0 ? tiles : x >= s.n ? 0 : tiles - static_cast<int>(x * p.group / kRows);
+    return x <= 0 ? tiles : x >= s.n ? 0 : tiles - static_cast<int>(x * p.group / R);
 }
 
 __device__ __forceinline__ int wave_scan(int v) {
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        const int u = __shfl_up(v, off, 64);
-        v += static_cast<int>(threadIdx.x & 63) >= off ? u : 0;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);       // rows of 16: one to the right, two, four, eight
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);       // a row's last lane to the next row
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);       // lane 31 to the upper half
     return v;
 }
+// Of values below 2^50: 25 bits at a time, whose sums of 64 lanes fit in 32.
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        const int64_t u = __shfl_up(v, off, 64);
-        v += static_cast<int>(threadIdx.x & 63) >= off ? u : 0;
-    }
-    return v;
+    const int lo = wave_scan(static_cast<int>(v & 0x1ffffff)), hi = wave_scan(static_cast<int>(v >> 25));
+    return (static_cast<int64_t>(hi) << 25) + static_cast<uint32_t>(lo);
 }
 __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
     const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
@@ -104,11 +111,11 @@ struct Place {
     int64_t read;                                // reads_below of all sequences before it
     int S;                                       // tokens of a part
 };
-template <class Count>
+template <int R, class Count>
 __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Count count) {
     const int lane = threadIdx.x & 63, span = (p.B + 63) / 64;
     Seq s = seq_of(p, lane);                     // (of span 1)
-    auto reads = [&](const Seq& s) { return p.Hkv * reads_below(p, s, tiles_of(p, s)); };
+    auto reads = [&](const Seq& s) { return p.Hkv * reads_below<R>(p, s, tiles_of<R>(p, s)); };
     int64_t read = 0;
     if (span == 1) read = reads(s);
     else
@@ -116,8 +123,8 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
     int64_t read_upto = wave_scan(read);
     const int64_t total = lane_of(read_upto, 63);
     at.S = 0x40000000;
-    if (p.slots) {
-        const int64_t S = ((total + p.slots - 1) / p.slots + kTile - 1) / kTile * kTile;
+    if (p.slots_log2 >= 0) {
+        const int64_t S = (((total - 1) >> p.slots_log2) + kTile) / kTile * kTile;
         at.S = static_cast<int>(S < kLeast ? kLeast : S < 0x40000000 ? S : 0x40000000);
     }
     int units = 0;
@@ -155,11 +162,14 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
 
 // Where part i of a tile lies in the workspace. `read`: reads_below of all tiles before it. Part i has the id w0 + i, w0
 // the part of an even cut of all reads that the tile's first falls into; a part 0 has slot 2 id + 1, others 2 id: ids of
-// one tile are its own but for its last, which may be the next tile's first.
-__device__ __forceinline__ int64_t slot_of(int64_t read, int S, int i) {
-    const int64_t id = read / S + i;
-    return i == 0 ? 2 * id + 1 : 2 * id;
+// one tile are its own but for its last, which may be the next tile's first. (The quotient in 64-bit floating point, which
+// finds the whole number of any that the workspace is large enough for, and in a tenth of an integer division's time.)
+template <int R>
+__device__ __forceinline__ int first_id(const ChunkArgs& p, const Place& at, int tile, int hk) {
+    const int64_t here = reads_below<R>(p, at.s, tile), read = at.read + p.Hkv * here + hk * (reads_below<R>(p, at.s, tile + 1) - here);
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<double>(read) / static_cast<double>(at.S)));
 }
+__device__ __forceinline__ uint8_t* slot_of(const ChunkArgs& p, int w0, int i) { return p.ws + (2 * (w0 + i) + (i == 0)) * p.slot_bytes; }
 
 __device__ __forceinline__ uint2 halves(const float4_t& v, float by, bool none) {
     uint16_t r[4];
@@ -169,29 +179,32 @@ __device__ __forceinline__ uint2 halves(const float4_t& v, float by, bool none) 
 }
 
 // ---------------------------------------------------------------------- a part --
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkArgs p) {
+// W: waves, each with 32 rows.
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p) {
+    constexpr int R = 32 * W;                    // (token, head) rows of a workgroup
     constexpr int KS = D / 16;                   // steps of the score product
     constexpr int MB = D / 32;                   // blocks of 32 d
     constexpr int RC = D / 8;                    // 16-byte chunks of a row
-    constexpr int RPI = 64 / RC;                 // rows that a wave's copy takes
-    constexpr int CP = 16 / RPI;                 // copies of 16 rows
+    constexpr int RPI = 64 / RC;                 // rows that a copy takes
+    constexpr int CR = W == 8 ? 8 : 16;          // rows of K and of V that a wave copies
     constexpr int ROW = 2 * D;                   // bytes
     constexpr int KM = RC < 16 ? RC - 1 : 15;
+    constexpr int kMfma = 0x008, kDsRead = 0x100, kAhead = 3;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // [2][K, V][kTile][D]
     const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     Place at;
     auto units = [&](const Seq& s, int S) {
-        const int tiles = tiles_of(p, s), base = s.len - s.n, parts = (s.len + S - 1) / S;
+        const int tiles = tiles_of<R>(p, s), base = s.len - s.n, parts = (s.len + S - 1) / S;
         const int whole = base > 0 ? base / S : 0;
-        int64_t sum = static_cast<int64_t>(tiles) * (1 + whole);
-        for (int i = whole + 1; i < parts; ++i) sum += tiles_with(p, s, tiles, static_cast<int64_t>(i) * S);
-        return static_cast<int>(sum) * p.Hkv;
+        int sum = tiles * (1 + whole);
+        for (int i = whole + 1; i < parts; ++i) sum += tiles_with<R>(p, s, tiles, static_cast<int64_t>(i) * S);
+        return sum * p.Hkv;
     };
-    if (!find(p, blockIdx.x, at, units)) return;
-    const int rows = at.s.n * p.group, tiles = tiles_of(p, at.s), base = at.s.len - at.s.n;
+    if (!find<R>(p, blockIdx.x, at, units)) return;
+    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
     const int hk = at.unit % p.Hkv;
     int part, tile;
     {
@@ -202,7 +215,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkAr
             part = whole + 1;
             i = v - tiles * (1 + whole);
             for (;;) {
-                const int have = tiles_with(p, at.s, tiles, static_cast<int64_t>(part) * at.S);
+                const int have = tiles_with<R>(p, at.s, tiles, static_cast<int64_t>(part) * at.S);
                 if (have == 0) return;           // (lengths that changed meanwhile)
                 if (i < have) break;
                 i -= have;
@@ -211,86 +224,102 @@ __global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkAr
         }
         tile = tiles - 1 - i;                    // (the ones that read most first)
     }
-    const int row0 = tile * kRows, last_row = (row0 + kRows < rows ? row0 + kRows : rows) - 1;
+    const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1;
     auto seen_by = [&](int row) {                // tokens that a row sees
-        const int n = base + row / p.group + 1;
+        const int n = base + token_of(p, row) + 1;
         return n < 0 ? 0 : n;
     };
     const int end = seen_by(last_row), parts = end <= at.S ? 1 : (end + at.S - 1) / at.S;
     const int t_begin = part * at.S, t_end = part < parts - 1 ? t_begin + at.S : end;
 
-    const int wrow = row0 + wave * kRowsWave;
+    const int wrow = row0 + wave * 32;
     const bool mine = wrow < rows;               // this wave has rows
-    const int row = wrow + c < rows ? wrow + c : rows - 1;
-    const int seen = seen_by(row), least = mine ? seen_by(wrow) : 0;
-    const int most = mine ? seen_by(wrow + kRowsWave - 1 < rows ? wrow + kRowsWave - 1 : rows - 1) : 0;
-    const int token = row / p.group, head = hk * p.group + row - token * p.group;
-    const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + head * p.q_head;
+    const int least = mine ? seen_by(wrow) : 0, most = mine ? seen_by(wrow + 31 < rows ? wrow + 31 : rows - 1) : 0;
+    const int row = wrow + c < rows ? wrow + c : rows - 1, token = token_of(p, row);      // past the last one: that one again, never stored
+    const int seen = seen_by(row);
     half8_t q[KS];
+    {
+        const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const half8_t*>(qr + 16 * s + 8 * j);
+        for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const half8_t*>(qr + 16 * s + 8 * j);
+        if (p.q_by != 1.f)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) q[s] *= static_cast<_Float16>(p.q_by);
+    }
 
-    const scalar_ints table = as_scalar(p.table + at.b * p.table_row);
+    const int32_t* table = p.table + at.b * p.table_row;
     const uint16_t* kh = p.k + hk * p.k_head;
     const uint16_t* vh = p.v + hk * p.v_head;
-    // Rows of 16 tokens from t on: their page's number (-1: not there, or past the end) and first row in it.
-    auto place = [&](int t, int& page, int& prow) {
-        const uint32_t t16 = static_cast<uint32_t>(t) >> 4;
-        uint32_t i = t16;
+    // The page of the 16 tokens from 16 t16 on (-1: not there, or past the end) and their first row in it.
+    auto place = [&](int t16, int& page, int& prow) {
+        uint32_t i = static_cast<uint32_t>(t16);
         prow = 0;
         if (p.page16 > 1) {
-            i = __umulhi(t16, p.page16_inv);     // one too many at most
-            int r = static_cast<int>(t16 - i * p.page16);
+            i = __umulhi(static_cast<uint32_t>(t16), p.page16_inv);      // one too many at most
+            int r = t16 - static_cast<int>(i * p.page16);
             if (r < 0) --i, r += p.page16;
             prow = 16 * r;
         }
-        page = t < t_end ? table[i] : -1;
-        page = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages) ? page : -1);
+        page = 16 * t16 < t_end ? table[i] : -1;
+        page = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages) ? page : -1;
     };
-    // 16 rows of K or V: as they lie, but a row's chunks in an order of its own, so that reads of a column meet other banks.
+    // A lane holds that of one of the 64 groups of 16 tokens from token `known` on.
+    int my_page = -1, my_row = 0, known = t_begin;
+    place(known / 16 + lane, my_page, my_row);
+    auto turn_of_v = [](int row) { return RC < 16 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); };
+    // Rows of K or V: as they lie, but a row's chunks in an order of its own, so that reads of a column meet other banks.
     const int lr = lane / RC, lc = lane % RC;
-    auto copy16 = [&](const uint16_t* base, int64_t page_stride, int token_stride, int page, int prow, uint8_t* to, bool of_v) {
+    auto copy = [&](const uint16_t* base, int64_t page_stride, int token_stride, int page, int prow, uint8_t* to, bool of_v) {
         const uint16_t* from = base + (page < 0 ? 0 : page) * page_stride + static_cast<int64_t>(page < 0 ? 0 : prow) * token_stride;
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(from), 0, 2 * (15 * token_stride + D), 0x00020000);
+        const int first = wave * CR % 16;        // of the 16 rows
 #pragma unroll
-        for (int i = 0; i < CP; ++i) {
-            const int at_row = i * RPI + lr;
-            const int turn = of_v ? (RC < 16 ? 4 * ((at_row >> 1) & 1) : 4 * (at_row & 3)) : at_row & KM;
+        for (int i = 0; i < CR / RPI; ++i) {
+            const int at_row = first + i * RPI + lr;
+            const int turn = of_v ? turn_of_v(at_row) : at_row & KM;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 2 * lr * token_stride + 16 * (lc ^ turn),
-                                                     2 * i * RPI * token_stride, 0, 0);
+                                                     2 * (first + i * RPI) * token_stride, 0, 0);
         }
     };
-    uint32_t gone[2] = {0, 0};                   // groups of 16 tokens that are not there, of the tiles in the two buffers
+    // Groups of 16 tokens that are not there, of the tile that is being taken and of the one that is on its way.
+    uint32_t gone = 0, gone_next = 0;
     auto stage = [&](int t, int buf) {
-        uint8_t* to = lds + buf * 2 * kTile * ROW + wave * 16 * ROW;
-        uint32_t none = 0;
-        int page = -1, prow = 0;
-#pragma unroll
-        for (int x = 0; x < kTile / 16; ++x) {
-            int pg, pr;
-            place(t + 16 * x, pg, pr);
-            none |= (pg < 0 ? 1u : 0u) << x;
-            if (x == wave) page = pg, prow = pr;
+        uint8_t* to = lds + buf * 2 * kTile * ROW + wave * CR * ROW;
+        const int g = (t - known) / 16, mine = g + wave * CR / 16;
+        gone_next = static_cast<uint32_t>(__ballot(my_page < 0) >> g) & 15u;
+        const int page = __builtin_amdgcn_readlane(my_page, mine), prow = __builtin_amdgcn_readlane(my_row, mine);
+        copy(kh, p.k_page, p.k_token, page, prow, to, false);
+        copy(vh, p.v_page, p.v_token, page, prow, to + kTile * ROW, true);
+        if (g == 64 - kTile / 16) {
+            known += 1024;
+            place(known / 16 + lane, my_page, my_row);
         }
-        gone[buf] = none;
-        copy16(kh, p.k_page, p.k_token, page, prow, to, false);
-        copy16(vh, p.v_page, p.v_token, page, prow, to + kTile * ROW, true);
     };
 
-    float4_t zero4 = {0, 0, 0, 0};
     float16_t acc[MB] = {};
     float m = -INFINITY, l = 0.f;
+    // Operands lie in LDS where a lane's place of the first turns by whole chunks: an exclusive or on the address.
+    const int vrow = 4 * j + ((lane & 15) >> 2);
+    const uint32_t k_at = c * ROW + 16 * (j ^ (c & KM));
+    const uint32_t v_at = kTile * ROW + vrow * ROW + 16 * (turn_of_v(vrow) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    typedef __fp16 half4_b __attribute__((ext_vector_type(4)));
+    typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+    typedef const __attribute__((address_space(3))) half8_t* lds_half8;
+    typedef __attribute__((address_space(3))) half4_b* lds_half4;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+
     if (t_begin < t_end) stage(t_begin, 0);
     int buf = 0;
     for (int t = t_begin; t < t_end; t += kTile, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        uint8_t* const kl = lds + buf * 2 * kTile * ROW;
-        uint8_t* const vl = kl + kTile * ROW;
-        if (t + kTile > t_end || gone[buf]) {
+        uint8_t* const vl = lds + (2 * buf + 1) * kTile * ROW;
+        const uint32_t k_now = lds_at + buf * 2 * kTile * ROW + k_at, v_now = lds_at + buf * 2 * kTile * ROW + v_at;
+        gone = gone_next;
+        if (t + kTile > t_end || gone) {
             // what lies past the end or is not there may be NaN, whose product with a weight of zero is no zero
-            for (int i = lane; i < 16 * RC; i += 64) {
-                const int r = 16 * wave + i / RC;
-                if (t + r >= t_end || (gone[buf] >> wave & 1)) *reinterpret_cast<float4_t*>(vl + r * ROW + 16 * (i % RC)) = zero4;
+            for (int i = lane; i < CR * RC; i += 64) {
+                const int r = CR * wave + i / RC;
+                if (t + r >= t_end || (gone >> (CR * wave / 16) & 1)) *reinterpret_cast<float4_t*>(vl + r * ROW + 16 * (i % RC)) = float4_t{0, 0, 0, 0};
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
@@ -299,68 +328,102 @@ __global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkAr
         __builtin_amdgcn_sched_barrier(0);
         if (t + kTile < t_end) stage(t + kTile, buf ^ 1);
         if (!mine || t >= most) continue;
-        float16_t s[2] = {};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
+        const bool all = t + kTile <= least && gone == 0;
+        // Scores of 32 tokens; the reference exponent of what follows, and its rare change; weights; their products
+        auto scores = [&](int h, float16_t& s) {
+            s = float16_t{};
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
-                const half8_t k = *reinterpret_cast<const half8_t*>(kl + (32 * h + c) * ROW + 16 * ((2 * x + j) ^ (c & KM)));
-                s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], s[h], 0, 0, 0);
+                const half8_t k = *reinterpret_cast<lds_half8>((k_now ^ (32 * x % (16 * (KM + 1)))) + 32 * h * ROW + 32 * x / (16 * (KM + 1)) * (16 * (KM + 1)));
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], s, 0, 0, 0);
             }
-        const bool all = t + kTile <= least && gone[buf] == 0;
-        float mx = -INFINITY;
+            // reads run kAhead products ahead
+            __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float v = s[h][i] * p.scale_log2;
-                if (!all && (t + 32 * h + 8 * (i / 4) + 4 * j + i % 4 >= seen || (gone[buf] >> (2 * h + i / 8) & 1))) v = -INFINITY;
-                s[h][i] = v;
-                mx = fmaxf(mx, v);
+            for (int x = 0; x < KS - kAhead; ++x) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
             }
-        mx = fmaxf(max2(mx), m);
-        if (__any(mx > m)) {
-            const float keep = m == -INFINITY ? 0.f : exp2_of(m - mx);
-            l *= keep;
+            __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto refer = [&](int h, float16_t& s) {
+            if (!all) {
+                const int left = seen - t - 32 * h - 4 * j;
 #pragma unroll
-            for (int b = 0; b < MB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[b][i] *= keep;
-            m = mx;
-        }
-        const float from = m == -INFINITY ? 0.f : m - kTopLog2;
-        half8_t w[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float e = exp2_of(s[x / 2][8 * (x & 1) + i] - from);
-                l += e;
-                w[x][i] = static_cast<_Float16>(e);
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i / 4) + i % 4 >= left || (gone >> (2 * h + i / 8) & 1)) s[i] = -INFINITY;
             }
-        const int vrow = 4 * j + ((lane & 15) >> 2);
-        const int vturn = RC < 16 ? 4 * ((vrow >> 1) & 1) : 4 * (vrow & 3);
-        const int vcol = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        typedef __fp16 half4_b __attribute__((ext_vector_type(4)));
-        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+            float mx = s[0];
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+            mx = max2(mx) * p.scale_log2;
+            if (__any(mx > m + (m == -INFINITY ? 0.f : kRoom))) {
+                const float to = fmaxf(m, ceilf(mx)), keep = m == -INFINITY ? 0.f : exp2_of(m - to);
+                m = to;
+                l *= keep;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                half8_t a;
+                for (int b = 0; b < MB; ++b)
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint8_t* from = vl + (16 * x + 8 * y + vrow) * ROW + 16 * ((4 * b + vcol) ^ vturn) + 8 * (lane & 1);
-                    const auto r = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) half4_b*)(from)));
+                    for (int i = 0; i < 16; ++i) acc[b][i] *= keep;
+            }
+        };
+        auto weigh = [&](const float16_t& s, half8_t (&w)[2]) {
+            const float from = m == -INFINITY ? 0.f : m - kTop;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) a[4 * y + e] = r[e];
+            for (int i = 0; i < 16; i += 2) {
+                const half2_t e = {static_cast<_Float16>(exp2_of(fmaf(s[i], p.scale_log2, -from))),
+                                   static_cast<_Float16>(exp2_of(fmaf(s[i + 1], p.scale_log2, -from)))};
+                l = __builtin_amdgcn_fdot2(e, half2_t{1, 1}, l, false);
+                w[i / 8][i % 8] = e[0];
+                w[i / 8][i % 8 + 1] = e[1];
+            }
+        };
+        auto add = [&](int h, const half8_t (&w)[2]) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int b = 0; b < MB; ++b) {
+                    half8_t a;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        constexpr int TM = RC < 16 ? 2 : 4;      // blocks that turn into one another
+                        const uint32_t from = (v_now ^ (64 * (b % TM))) + (32 * h + 16 * x + 8 * y) * ROW + 64 * TM * (b / TM);
+                        const auto r = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_half4>(from)));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) a[4 * y + e] = r[e];
+                    }
+                    acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[x], acc[b], 0, 0, 0);
                 }
-                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[x], acc[b], 0, 0, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kAhead, 0);
+#pragma unroll
+            for (int x = 0; x < 2 * MB - kAhead; ++x) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
             }
+            __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float16_t s;
+            half8_t w[2];
+            scores(h, s);
+            refer(h, s);
+            weigh(s, w);
+            add(h, w);
+        }
     }
     if (!mine) return;
-    l = sum2(l);
 
+    const int w0 = parts > 1 ? first_id<R>(p, at, tile, hk) : 0;
+    float* const slot = parts > 1 ? reinterpret_cast<float*>(slot_of(p, w0, part)) : nullptr;
+    const int64_t stats = static_cast<int64_t>(p.slot_bytes / (D * 4 + 8)) * D;       // behind the rows
+    auto out_row = [&](int r) {
+        const int tk = token_of(p, r);
+        return p.out + (static_cast<int64_t>(at.s.first + tk) * p.Hq + hk * p.group + r - tk * p.group) * D;
+    };
+    l = sum2(l);
     // acc[b][i]: d = 32 b + 8 (i / 4) + 4 j + i % 4 of this lane's row
     bool odd = !(fabsf(l) < INFINITY);
 #pragma unroll
@@ -369,52 +432,38 @@ __global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkAr
         for (int i = 0; i < 16; ++i) odd |= !(fabsf(acc[b][i]) < INFINITY);
     const unsigned long long odds = __ballot(odd);
     const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
-    float* slot = nullptr;
-    const int64_t read = at.read + p.Hkv * reads_below(p, at.s, tile) + hk * (reads_below(p, at.s, tile + 1) - reads_below(p, at.s, tile));
-    if (parts > 1) slot = reinterpret_cast<float*>(p.ws + slot_of(read, at.S, part) * p.slot_bytes);
-    const int slot_rows = static_cast<int>(p.slot_bytes / (D * 4 + 8));
-    auto out_row = [&](int r) {
-        const int tk = r / p.group;
-        return p.out + (static_cast<int64_t>(at.s.first + tk) * p.Hq + hk * p.group + r - tk * p.group) * D;
-    };
     if (wrow + c < rows && !(bad >> c & 1)) {
-        if (slot) {
-            float* to = slot + static_cast<int64_t>(wave * kRowsWave + c) * D;
+        const float by = l > 0.f ? 1.0f / l : 0.f;
+        float* part_row = slot ? slot + static_cast<int64_t>(wrow + c - row0) * D : nullptr;
+        uint16_t* to = out_row(wrow + c);
 #pragma unroll
-            for (int b = 0; b < MB; ++b)
+        for (int b = 0; b < MB; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<float4_t*>(to + 32 * b + 8 * i + 4 * j) = float4_t{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-            if (j == 0) *reinterpret_cast<float2*>(slot + static_cast<int64_t>(slot_rows) * D + 2 * (wave * kRowsWave + c)) = make_float2(m, l);
-        } else {
-            const float by = l > 0.f ? 1.0f / l : 0.f;
-            uint16_t* to = out_row(wrow + c);
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<uint2*>(to + 32 * b + 8 * i + 4 * j) =
-                        halves(float4_t{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]}, by, l == 0.f);
-        }
+            for (int i = 0; i < 4; ++i) {
+                const float4_t v = {acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+                if (slot) *reinterpret_cast<float4_t*>(part_row + 32 * b + 8 * i + 4 * j) = v;
+                else *reinterpret_cast<uint2*>(to + 32 * b + 8 * i + 4 * j) = halves(v, by, l == 0.f);
+            }
+        if (slot && j == 0) *reinterpret_cast<float2*>(slot + stats + 2 * (wrow + c - row0)) = make_float2(m, l);
     }
     // Rows that are not finite, one at a time and token by token: an infinity or NaN in V reaches the rows that see its
     // token, where above it reaches every row of its tile (zero weights times it are NaN).
     for (uint32_t left = bad; left; left &= left - 1) {
-        const int r = __builtin_ctz(left), rr = wrow + r;
+        const int rr = wrow + __builtin_ctz(left);
         if (rr >= rows) break;
         constexpr int E = D / 64;
-        const int tk = rr / p.group;
-        const uint16_t* from = p.q + static_cast<int64_t>(at.s.first + tk) * p.q_row + (hk * p.group + rr - tk * p.group) * p.q_head + E * lane;
+        const int tk = token_of(p, rr);
+        const uint16_t* from = p.q + static_cast<int64_t>(at.s.first + tk) * p.q_row + static_cast<int64_t>(hk * p.group + rr - tk * p.group) * p.q_head + E * lane;
         float qv[E], sum[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) qv[e] = h2f(from[e]), sum[e] = 0.f;
+        for (int e = 0; e < E; ++e) qv[e] = h2f(from[e]) * p.q_by, sum[e] = 0.f;
         const int upto = seen_by(rr) < t_end ? seen_by(rr) : t_end;
         float top = -INFINITY, tot = 0.f;
         auto tokens = [&](auto use) {
-            for (int t16 = t_begin; t16 < upto; t16 += 16) {
+            for (int t = t_begin; t < upto; t += 16) {
                 int page, prow;
-                place(t16, page, prow);
-                for (int x = 0; page >= 0 && x < 16 && t16 + x < upto; ++x) {
+                place(t / 16, page, prow);
+                for (int x = 0; page >= 0 && x < 16 && t + x < upto; ++x) {
                     const uint16_t* k = kh + page * p.k_page + static_cast<int64_t>(prow + x) * p.k_token + E * lane;
                     float dot = 0.f;
 #pragma unroll
@@ -425,7 +474,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkAr
             }
         };
         tokens([&](float s, const uint16_t*) { top = fmaxf(top, s); });
-        const float less = top == -INFINITY ? 0.f : top - kTopLog2;
+        const float less = top == -INFINITY ? 0.f : top - kTop;
         tokens([&](float s, const uint16_t* v) {
             const float w = exp2_of(s - less);
             tot += w;
@@ -435,25 +484,26 @@ __global__ __launch_bounds__(64 * kWaves, 1) void chunk_attention_kernel(ChunkAr
         const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (slot) slot[static_cast<int64_t>(wave * kRowsWave + r) * D + E * lane + e] = sum[e];
+            if (slot) slot[static_cast<int64_t>(rr - row0) * D + E * lane + e] = sum[e];
             else out_row(rr)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
         }
-        if (slot && lane == 0) *reinterpret_cast<float2*>(slot + static_cast<int64_t>(slot_rows) * D + 2 * (wave * kRowsWave + r)) = make_float2(top, tot);
+        if (slot && lane == 0) *reinterpret_cast<float2*>(slot + stats + 2 * (rr - row0)) = make_float2(top, tot);
     }
 }
 
 // ------------------------------------------------------------------- the parts' sum --
-template <int D>
+template <int D, int W>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
+    constexpr int R = 32 * W;
     Place at;
-    auto cut = [&](const Seq& s, int S) { return s.len > S ? tiles_with(p, s, tiles_of(p, s), S) * p.Hkv : 0; };
-    if (!find(p, blockIdx.x, at, cut)) return;
-    const int rows = at.s.n * p.group, tiles = tiles_of(p, at.s), base = at.s.len - at.s.n;
+    auto cut = [&](const Seq& s, int S) { return s.len > S ? tiles_with<R>(p, s, tiles_of<R>(p, s), S) * p.Hkv : 0; };
+    if (!find<R>(p, blockIdx.x, at, cut)) return;
+    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
     const int hk = at.unit % p.Hkv, tile = tiles - 1 - at.unit / p.Hkv;
-    const int row0 = tile * kRows, last_row = (row0 + kRows < rows ? row0 + kRows : rows) - 1;
-    const int end = base + last_row / p.group + 1, parts = (end + at.S - 1) / at.S;
-    const int64_t read = at.read + p.Hkv * reads_below(p, at.s, tile) + hk * (reads_below(p, at.s, tile + 1) - reads_below(p, at.s, tile));
-    const int slot_rows = static_cast<int>(p.slot_bytes / (D * 4 + 8));
+    const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1;
+    const int end = base + token_of(p, last_row) + 1, parts = (end + at.S - 1) / at.S;
+    const int w0 = first_id<R>(p, at, tile, hk);
+    const int64_t stats = static_cast<int64_t>(p.slot_bytes / (D * 4 + 8)) * D;
     for (int i = threadIdx.x; i < kJoinRows * D / 4; i += 256) {
         const int r = blockIdx.y * kJoinRows + i / (D / 4), d = i % (D / 4) * 4, rr = row0 + r;
         if (rr > last_row) break;
@@ -466,9 +516,9 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
             float most = top;
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                const float* slot = reinterpret_cast<const float*>(p.ws + slot_of(read, at.S, u0 + u < parts ? u0 + u : parts - 1) * p.slot_bytes);
+                const float* slot = reinterpret_cast<const float*>(slot_of(p, w0, u0 + u < parts ? u0 + u : parts - 1));
                 o[u] = *reinterpret_cast<const float4_t*>(slot + static_cast<int64_t>(r) * D + d);
-                st[u] = *reinterpret_cast<const float2*>(slot + static_cast<int64_t>(slot_rows) * D + 2 * r);
+                st[u] = *reinterpret_cast<const float2*>(slot + stats + 2 * r);
             }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) most = fmaxf(most, st[u].x);
@@ -485,16 +535,18 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
                 for (int x = 0; x < 4; ++x) sum[x] = fmaf(o[u][x], by, sum[x]);
             }
         }
-        const int tk = rr / p.group;
+        const int tk = token_of(p, rr);
         const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
         *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(at.s.first + tk) * p.Hq + hk * p.group + rr - tk * p.group) * D + d) = halves(sum, by, tot == 0.f);
     }
 }
 
-// Parts to cut for, of rows that read up to `most` tokens: what the chip holds at once.  0: nothing to cut.
-int choose_slots(int64_t most, int64_t D) { return most <= kLeast ? 0 : D == 256 ? 256 : 512; }
-int64_t slot_rows_of(int64_t T, int64_t group) { return std::min<int64_t>(kRows, T * group); }
-int64_t split_bytes(int64_t slots, int64_t rows, int64_t D) { return slots == 0 ? 0 : 2 * (slots + 2) * part_bytes(rows, D); }
+// Waves of a workgroup.
+int choose_waves(int64_t D) { return D == 256 ? 8 : 4; }
+// Parts to cut for, of rows that read up to `most` tokens: what the chip holds at once.  -1: nothing to cut.
+int choose_slots_log2(int64_t most, int64_t D) { return most <= kLeast ? -1 : D == 256 ? 8 : 9; }
+int64_t slot_rows_of(int64_t T, int64_t group, int64_t D) { return std::min<int64_t>(32 * choose_waves(D), T * group); }
+int64_t split_bytes(int slots_log2, int64_t rows, int64_t D) { return slots_log2 < 0 ? 0 : 2 * ((int64_t(1) << slots_log2) + 2) * part_bytes(rows, D); }
 
 }  // namespace
 }  // namespace mcv
@@ -505,7 +557,7 @@ extern "C" {
 
 int64_t mcv_paged_attention_chunk_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seq_len) {
     if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || T > 0x7fffffff / Hq || D <= 0 || max_seq_len < 0) return 0;
-    return split_bytes(choose_slots(std::min(max_seq_len, kMaxLen), D), slot_rows_of(T, Hq / Hkv), D);
+    return split_bytes(choose_slots_log2(std::min(max_seq_len, kMaxLen), D), slot_rows_of(T, Hq / Hkv, D), D);
 }
 
 int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
@@ -535,29 +587,34 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     // (width counted in pages first: width * page_size could pass 64 bits)
     const int64_t held = table_width > kMaxLen / page_size ? kMaxLen : table_width * page_size;
     const int64_t most = max_seq_len < held ? max_seq_len : held;
-    const int64_t group = Hq / Hkv, rows = slot_rows_of(T, group);
-    const int64_t tiles = std::min(T * group / kRows + B, T * group);
-    int slots = choose_slots(most, D);
-    if (slots && (!workspace || workspace_bytes < split_bytes(slots, rows, D))) slots = 0;
-    if (slots && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    const int64_t group = Hq / Hkv;
+    const int64_t rows = slot_rows_of(T, group, D), tiles = std::min(T * group / (32 * choose_waves(D)) + B, T * group);
+    int slots_log2 = choose_slots_log2(most, D);
+    if (slots_log2 >= 0 && (!workspace || workspace_bytes < split_bytes(slots_log2, rows, D))) slots_log2 = -1;
+    if (slots_log2 >= 0 && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", who);
+    const int64_t slots = slots_log2 < 0 ? 0 : int64_t(1) << slots_log2;
     if (tiles * Hkv + slots > 0x7fffffff) return fail(MCV_ERR_SHAPE, "%s: too many rows B=%lld T=%lld Hq=%lld", who, (long long)B, (long long)T, (long long)Hq);
     const uint32_t page16 = static_cast<uint32_t>(page_size / 16);
+    auto inverse = [](uint64_t n) { return n > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + n - 1) / n) : 0; };
     const ChunkArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache),
                       static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(seq_lens), static_cast<const int32_t*>(cu_seqlens),
                       static_cast<uint16_t*>(out), static_cast<uint8_t*>(workspace), q_row, q_head, k_page, k_head, v_page, v_head, table_row,
                       static_cast<int>(k_token), static_cast<int>(v_token), static_cast<int>(pages), static_cast<int>(page16), static_cast<int>(most),
                       static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
-                      page16 > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + page16 - 1) / page16) : 0, static_cast<float>(scale) * kLog2e,
-                      slots, part_bytes(rows, D)};
+                      inverse(page16), inverse(group), scale == 0.0 ? 1.f : std::fabs(static_cast<float>(scale) * kLog2e), scale < 0.0 ? -1.f : scale == 0.0 ? 0.f : 1.f,
+                      slots_log2, part_bytes(rows, D)};
     const auto s = static_cast<hipStream_t>(stream);
-    auto fn = D == 64 ? chunk_attention_kernel<64> : D == 128 ? chunk_attention_kernel<128> : chunk_attention_kernel<256>;
-    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(tiles * Hkv + slots)), dim3(64 * kWaves), static_cast<unsigned>(4 * kTile * 2 * D), s, a);
-    rc = check_launch("chunk_attention_kernel");
-    if (rc != MCV_OK || !slots) return rc;
-    auto join = D == 64 ? chunk_join_kernel<64> : D == 128 ? chunk_join_kernel<128> : chunk_join_kernel<256>;
-    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min<int64_t>(tiles * Hkv, slots)), static_cast<unsigned>(ceil_div(rows, kJoinRows))), dim3(256), 0, s, a);
-    return check_launch("chunk_join_kernel");
+    const dim3 grid(static_cast<unsigned>(tiles * Hkv + slots)), joins(static_cast<unsigned>(std::min(tiles * Hkv, slots)), static_cast<unsigned>(ceil_div(rows, kJoinRows)));
+    auto launch = [&](auto part, auto join) {
+        hipLaunchKernelGGL(part, grid, dim3(static_cast<unsigned>(64 * choose_waves(D))), static_cast<unsigned>(4 * kTile * 2 * D), s, a);
+        const int rc = check_launch("chunk_attention_kernel");
+        if (rc != MCV_OK || !slots) return rc;
+        hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
+        return check_launch("chunk_join_kernel");
+    };
+    return D == 64 ? launch(chunk_attention_kernel<64, 4>, chunk_join_kernel<64, 4>) :
+           D == 128 ? launch(chunk_attention_kernel<128, 4>, chunk_join_kernel<128, 4>) : launch(chunk_attention_kernel<256, 8>, chunk_join_kernel<256, 8>);
 }
 
 }  // extern "C"
