@@ -25,8 +25,8 @@ PyObject *g_error, *g_empty_on;                  // McvError, and mixers.py's te
 // A function of mixers.py or the package that makes workspaces, the dict of those it keeps, by device, stream and size.
 struct Workspaces {
     PyObject *make, *held;
-} g_gemm, g_delta;
-int64_t g_gemm_sizes[2], g_delta_sizes[2];
+} g_gemm, g_delta, g_chunk;
+int64_t g_gemm_sizes[2], g_delta_sizes[2], g_chunk_size;
 
 struct Failed {};                                // a Python error is set
 
@@ -167,6 +167,10 @@ void* gemm_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_s
 }
 void* delta_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
     return workspace(g_delta, of(g_delta_sizes, bytes), t, stream, h);
+}
+
+void* chunk_workspace(int64_t bytes, const at::Tensor& t, PyObject* stream, mcv_stream_t h) {
+    return workspace(g_chunk, bytes < g_chunk_size ? g_chunk_size : bytes, t, stream, h);
 }
 
 // (who, q, k, v, g, beta, state, cu, step, scale, normalize, state_index, out, state_out, stream) -> (out, state_out)
@@ -311,7 +315,7 @@ PyObject* chunk(PyObject* const* a) {
         return wrapped(out);
     }
     const int64_t bytes = mcv_paged_attention_chunk_workspace_bytes(B, T, Hq, Hkv, D, most);
-    void* ws = bytes ? delta_workspace(bytes, q, a[9], h) : nullptr;
+    void* ws = bytes ? chunk_workspace(bytes, q, a[9], h) : nullptr;
     check(mcv_paged_attention_chunk(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
                                     table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), most, ptr(cu), B, T, Hq, Hkv, D,
                                     number(a[6], 1.0 / std::sqrt(static_cast<double>(D))), out.data_ptr(), ws, ws ? bytes : 0, h),
@@ -520,19 +524,21 @@ PyObject* py_norm_add_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) { re
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 8, [&] { return rotary(a, false); }); }
 PyObject* py_rotary_cached(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 11, [&] { return rotary(a, true); }); }
 
-// (McvError, _empty_on, gemm_workspace, the buffers it keeps, two sizes of them, delta_workspace, its, two of them)
+// (McvError, _empty_on, gemm_workspace, the buffers it keeps, two sizes of them, delta_workspace, its, two of them, chunk_workspace, its, one)
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject *error, *empty_on;
-    Workspaces gemm, delta;
-    long long sizes[4];
-    if (!PyArg_ParseTuple(args, "OOOO!LLOO!LL", &error, &empty_on, &gemm.make, &PyDict_Type, &gemm.held, &sizes[0], &sizes[1], &delta.make, &PyDict_Type,
-                          &delta.held, &sizes[2], &sizes[3]))
+    Workspaces gemm, delta, chunk;
+    long long sizes[5];
+    if (!PyArg_ParseTuple(args, "OOOO!LLOO!LLOO!L", &error, &empty_on, &gemm.make, &PyDict_Type, &gemm.held, &sizes[0], &sizes[1], &delta.make, &PyDict_Type,
+                          &delta.held, &sizes[2], &sizes[3], &chunk.make, &PyDict_Type, &chunk.held, &sizes[4]))
         return nullptr;
-    for (PyObject* o : {error, empty_on, gemm.make, gemm.held, delta.make, delta.held}) Py_INCREF(o);
+    for (PyObject* o : {error, empty_on, gemm.make, gemm.held, delta.make, delta.held, chunk.make, chunk.held}) Py_INCREF(o);
     g_error = error;
     g_empty_on = empty_on;
     g_gemm = gemm;
     g_delta = delta;
+    g_chunk = chunk;
+    g_chunk_size = sizes[4];
     for (int i = 0; i < 2; ++i) {
         g_gemm_sizes[i] = sizes[i];
         g_delta_sizes[i] = sizes[2 + i];

@@ -7,9 +7,8 @@
 namespace mcv {
 namespace {
 
-constexpr int kTile = 64;                        // tokens that are staged and taken at a time
+constexpr int kTile = 64;                        // a part has whole ones of so many tokens
 constexpr int kLeast = 2 * kTile;                // tokens of a part, at least
-constexpr int kJoinRows = 16;                    // rows that a workgroup joins
 constexpr int64_t kMaxLen = int64_t(1) << 30;    // tokens of one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's reference exponent m is a whole number, so that what it once stood for is brought to another by an exact product,
@@ -31,10 +30,16 @@ struct ChunkArgs {
     float scale_log2;                            // above zero: a score of -inf stays one
     float q_by;                                  // 1, -1 or 0: the scale's sign
     int slots_log2;                              // parts to cut for; -1: every tile of rows whole
+    int near_log2;                               // units side by side on one XCD
     int64_t slot_bytes;
 };
 
-__host__ __device__ constexpr int64_t part_bytes(int64_t rows, int64_t D) { return rows * (D * 4 + 8); }
+
+constexpr int kFan = 4;                          // parts that one of them joins
+constexpr int64_t kCounterBytes = 24576;         // five levels of joining, a counter for each part
+
+// Bytes of a wave's part: a lane's sums, and its reference exponent and sum of weights, as they are in registers.
+__host__ __device__ constexpr int64_t part_bytes(int64_t D) { return 64 * (2 * D + 8); }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max2(float v) {          // over the two lanes of one column
@@ -160,6 +165,14 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
     return true;
 }
 
+// The number of the unit that workgroup b takes. Workgroup b runs on XCD b % 8: runs of `near` units, which read the same K
+// and V, go to one XCD, whose L2 they share; every other round of eight runs goes to them in reverse, as the first of a
+// sequence read most.
+__device__ __forceinline__ int unit_of(const ChunkArgs& p, int b) {
+    const int x = b & 7, i = (b >> 3) & ((1 << p.near_log2) - 1), round = b >> (3 + p.near_log2);
+    return (((round << 3) + (round & 1 ? 7 - x : x)) << p.near_log2) + i;
+}
+
 // Where part i of a tile lies in the workspace. `read`: reads_below of all tiles before it. Part i has the id w0 + i, w0
 // the part of an even cut of all reads that the tile's first falls into; a part 0 has slot 2 id + 1, others 2 id: ids of
 // one tile are its own but for its last, which may be the next tile's first. (The quotient in 64-bit floating point, which
@@ -169,7 +182,21 @@ __device__ __forceinline__ int first_id(const ChunkArgs& p, const Place& at, int
     const int64_t here = reads_below<R>(p, at.s, tile), read = at.read + p.Hkv * here + hk * (reads_below<R>(p, at.s, tile + 1) - here);
     return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<double>(read) / static_cast<double>(at.S)));
 }
-__device__ __forceinline__ uint8_t* slot_of(const ChunkArgs& p, int w0, int i) { return p.ws + (2 * (w0 + i) + (i == 0)) * p.slot_bytes; }
+__device__ __forceinline__ uint8_t* slot_of(const ChunkArgs& p, int w0, int i) { return p.ws + kCounterBytes + (2 * (w0 + i) + (i == 0)) * p.slot_bytes; }
+
+// Counts this workgroup in; true in every thread of the one that is the last of n.
+__device__ __forceinline__ bool last_in(unsigned* counter, int n, int* flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this thread's part is written through
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned old = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int last = old == static_cast<unsigned>(n - 1);
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = last;
+    }
+    __syncthreads();
+    return *flag != 0;
+}
 
 __device__ __forceinline__ uint2 halves(const float4_t& v, float by, bool none) {
     uint16_t r[4];
@@ -179,19 +206,23 @@ __device__ __forceinline__ uint2 halves(const float4_t& v, float by, bool none) 
 }
 
 // ---------------------------------------------------------------------- a part --
-// W: waves, each with 32 rows.
-template <int D, int W>
+// W: waves, each with 32 rows. KT: tokens that are staged and taken at a time.
+template <int D, int W, int KT>
 __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p) {
     constexpr int R = 32 * W;                    // (token, head) rows of a workgroup
     constexpr int KS = D / 16;                   // steps of the score product
     constexpr int MB = D / 32;                   // blocks of 32 d
     constexpr int RC = D / 8;                    // 16-byte chunks of a row
     constexpr int RPI = 64 / RC;                 // rows that a copy takes
-    constexpr int CR = W == 8 ? 8 : 16;          // rows of K and of V that a wave copies
+    constexpr int CR = KT / W;          // rows of K and of V that a wave copies
     constexpr int ROW = 2 * D;                   // bytes
     constexpr int KM = RC < 16 ? RC - 1 : 15;
+    constexpr int QL = D == 256 ? 2 : 0;         // of q's operands, those that lie in LDS: the registers are one or two short
+    constexpr int VA = D == 256 ? 0 : 3;         // operands of V read before the softmax, where there are registers
     constexpr int kMfma = 0x008, kDsRead = 0x100, kAhead = 3;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // [2][K, V][kTile][D]
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // [2][K, V][KT][D]
+    __shared__ int flag;
+    constexpr int kThrough = 16;                 // accesses that all XCDs see
     const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -203,26 +234,30 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         for (int i = whole + 1; i < parts; ++i) sum += tiles_with<R>(p, s, tiles, static_cast<int64_t>(i) * S);
         return sum * p.Hkv;
     };
-    if (!find<R>(p, blockIdx.x, at, units)) return;
+    if (!find<R>(p, unit_of(p, blockIdx.x), at, units)) return;
     const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
-    const int hk = at.unit % p.Hkv;
-    int part, tile;
+    // Part by part; in one, `near` tiles of a cache head after another, those that read most first.
+    int part, tile, hk;
     {
-        const int v = at.unit / p.Hkv, whole = base > 0 ? base / at.S : 0;
-        part = v / tiles;
-        int i = v - part * tiles;
-        if (part > whole) {
+        const int whole = base > 0 ? base / at.S : 0;
+        int i = at.unit, have = tiles;
+        part = i / (tiles * p.Hkv);
+        if (part <= whole) i -= part * tiles * p.Hkv;
+        else {
             part = whole + 1;
-            i = v - tiles * (1 + whole);
+            i -= part * tiles * p.Hkv;
             for (;;) {
-                const int have = tiles_with<R>(p, at.s, tiles, static_cast<int64_t>(part) * at.S);
+                have = tiles_with<R>(p, at.s, tiles, static_cast<int64_t>(part) * at.S);
                 if (have == 0) return;           // (lengths that changed meanwhile)
-                if (i < have) break;
-                i -= have;
+                if (i < have * p.Hkv) break;
+                i -= have * p.Hkv;
                 ++part;
             }
         }
-        tile = tiles - 1 - i;                    // (the ones that read most first)
+        const int near = 1 << p.near_log2, first = i / (near * p.Hkv) * near, of = have - first < near ? have - first : near;
+        i -= first * p.Hkv;
+        hk = i / of;
+        tile = tiles - 1 - first - (i - hk * of);
     }
     const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1;
     auto seen_by = [&](int row) {                // tokens that a row sees
@@ -237,21 +272,12 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     const int least = mine ? seen_by(wrow) : 0, most = mine ? seen_by(wrow + 31 < rows ? wrow + 31 : rows - 1) : 0;
     const int row = wrow + c < rows ? wrow + c : rows - 1, token = token_of(p, row);      // past the last one: that one again, never stored
     const int seen = seen_by(row);
-    half8_t q[KS];
-    {
-        const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const half8_t*>(qr + 16 * s + 8 * j);
-        if (p.q_by != 1.f)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) q[s] *= static_cast<_Float16>(p.q_by);
-    }
 
     const int32_t* table = p.table + at.b * p.table_row;
     const uint16_t* kh = p.k + hk * p.k_head;
     const uint16_t* vh = p.v + hk * p.v_head;
     // The page of the 16 tokens from 16 t16 on (-1: not there, or past the end) and their first row in it.
-    auto place = [&](int t16, int& page, int& prow) {
+    auto place = [&](int t16, int upto, int& page, int& prow) {
         uint32_t i = static_cast<uint32_t>(t16);
         prow = 0;
         if (p.page16 > 1) {
@@ -260,62 +286,93 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             if (r < 0) --i, r += p.page16;
             prow = 16 * r;
         }
-        page = 16 * t16 < t_end ? table[i] : -1;
+        page = 16 * t16 < upto ? table[i] : -1;
         page = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages) ? page : -1;
     };
     // A lane holds that of one of the 64 groups of 16 tokens from token `known` on.
     int my_page = -1, my_row = 0, known = t_begin;
-    place(known / 16 + lane, my_page, my_row);
-    auto turn_of_v = [](int row) { return RC < 16 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); };
-    // Rows of K or V: as they lie, but a row's chunks in an order of its own, so that reads of a column meet other banks.
-    const int lr = lane / RC, lc = lane % RC;
-    auto copy = [&](const uint16_t* base, int64_t page_stride, int token_stride, int page, int prow, uint8_t* to, bool of_v) {
-        const uint16_t* from = base + (page < 0 ? 0 : page) * page_stride + static_cast<int64_t>(page < 0 ? 0 : prow) * token_stride;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(from), 0, 2 * (15 * token_stride + D), 0x00020000);
-        const int first = wave * CR % 16;        // of the 16 rows
-#pragma unroll
-        for (int i = 0; i < CR / RPI; ++i) {
-            const int at_row = first + i * RPI + lr;
-            const int turn = of_v ? turn_of_v(at_row) : at_row & KM;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 2 * lr * token_stride + 16 * (lc ^ turn),
-                                                     2 * (first + i * RPI) * token_stride, 0, 0);
-        }
-    };
+    place(known / 16 + lane, t_end, my_page, my_row);
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    // A tile's copies. Rows lie in LDS as they do in memory, but a row's chunks in an order of its own, so that reads of a
+    // column meet other banks. Each wave has CP copies of K and CP of V to make, spread over the products of the tile before:
+    // in one go they would hold all waves up, and with them the matrix cores.
+    auto turn_of_v = [](uint32_t row) { return RC < 16 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); };
+    constexpr int CP = CR / RPI;
+    const int first_row = wave * CR % 16;        // of its 16 rows
+    int4_t k_from, v_from;                       // buffer descriptors
+    uint32_t copy_to;
     // Groups of 16 tokens that are not there, of the tile that is being taken and of the one that is on its way.
     uint32_t gone = 0, gone_next = 0;
-    auto stage = [&](int t, int buf) {
-        uint8_t* to = lds + buf * 2 * kTile * ROW + wave * CR * ROW;
-        const int g = (t - known) / 16, mine = g + wave * CR / 16;
-        gone_next = static_cast<uint32_t>(__ballot(my_page < 0) >> g) & 15u;
-        const int page = __builtin_amdgcn_readlane(my_page, mine), prow = __builtin_amdgcn_readlane(my_row, mine);
-        copy(kh, p.k_page, p.k_token, page, prow, to, false);
-        copy(vh, p.v_page, p.v_token, page, prow, to + kTile * ROW, true);
-        if (g == 64 - kTile / 16) {
+    auto aim = [&](int t, int buf) {
+        copy_to = lds_at + buf * 2 * KT * ROW + wave * CR * ROW;
+        const int g = (t - known) / 16, own = g + wave * CR / 16;
+        gone_next = static_cast<uint32_t>(__ballot(my_page < 0) >> g) & (KT == 64 ? 15u : 3u);
+        const int page = __builtin_amdgcn_readlane(my_page, own), prow = __builtin_amdgcn_readlane(my_row, own);
+        auto rows16 = [&](const uint16_t* base, int64_t page_stride, int token_stride) {
+            const uint16_t* at = base + (page < 0 ? 0 : page) * page_stride + static_cast<int64_t>(prow) * token_stride;
+            const uintptr_t a = reinterpret_cast<uintptr_t>(at);
+            return int4_t{static_cast<int>(a), static_cast<int>(a >> 32 & 0xffff), page < 0 ? 0 : 2 * (15 * token_stride + D), 0x00020000};
+        };
+        k_from = rows16(kh, p.k_page, p.k_token);
+        v_from = rows16(vh, p.v_page, p.v_token);
+        if (g == 64 - KT / 16) {
             known += 1024;
-            place(known / 16 + lane, my_page, my_row);
+            place(known / 16 + lane, t_end, my_page, my_row);
         }
     };
-
+    // (Written out: the compiler would have every read of V in LDS wait for all copies on their way, whatever buffer they go
+    // to. The loop waits for them where it takes the tile.)
+    auto copy = [&](int i) {                     // 0 .. CP - 1: of K, then of V
+        uint32_t opaque = lane;                  // (offsets made from it would be kept through the loop)
+        asm volatile("" : "+v"(opaque));
+        const uint32_t lr = opaque / RC, lc = opaque % RC;
+        const bool of_v = i >= CP;
+        const int row = first_row + (of_v ? i - CP : i) * RPI, stride = of_v ? p.v_token : p.k_token;
+        const uint32_t turn = of_v ? turn_of_v(row + lr) : (row + lr) & KM;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(copy_to + (of_v ? KT * ROW + (i - CP) * 1024 : i * 1024)),
+                     "v"(2 * lr * stride + 16 * (lc ^ turn)), "s"(of_v ? v_from : k_from), "s"(2 * row * stride));
+    };
+    if (t_begin < t_end) {
+        aim(t_begin, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * CP; ++i) copy(i);
+    }
+    half8_t q[KS - QL], *const q_held = reinterpret_cast<half8_t*>(lds + 4 * KT * ROW) + threadIdx.x;
+    if (mine) {
+        const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head;
+        half8_t all[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) all[s] = *reinterpret_cast<const half8_t*>(qr + 16 * s + 8 * j);
+        if (p.q_by != 1.f)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) all[s] *= static_cast<_Float16>(p.q_by);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            asm volatile("" : "+v"(all[s]));     // (waited for here: a wait in the loop would be one for its copies too)
+            if (s < KS - QL) q[s] = all[s];
+            else q_held[(s - KS + QL) * 64 * W] = all[s];
+        }
+    }
     float16_t acc[MB] = {};
     float m = -INFINITY, l = 0.f;
     // Operands lie in LDS where a lane's place of the first turns by whole chunks: an exclusive or on the address.
     const int vrow = 4 * j + ((lane & 15) >> 2);
     const uint32_t k_at = c * ROW + 16 * (j ^ (c & KM));
-    const uint32_t v_at = kTile * ROW + vrow * ROW + 16 * (turn_of_v(vrow) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    const uint32_t v_at = (KT + vrow) * ROW + 16 * (turn_of_v(vrow) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
     typedef __fp16 half4_b __attribute__((ext_vector_type(4)));
     typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
     typedef const __attribute__((address_space(3))) half8_t* lds_half8;
     typedef __attribute__((address_space(3))) half4_b* lds_half4;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    typedef uint32_t uint2_v __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) uint2_v* lds_uint2;
 
-    if (t_begin < t_end) stage(t_begin, 0);
     int buf = 0;
-    for (int t = t_begin; t < t_end; t += kTile, buf ^= 1) {
+    for (int t = t_begin; t < t_end; t += KT, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        uint8_t* const vl = lds + (2 * buf + 1) * kTile * ROW;
-        const uint32_t k_now = lds_at + buf * 2 * kTile * ROW + k_at, v_now = lds_at + buf * 2 * kTile * ROW + v_at;
+        uint8_t* const vl = lds + (2 * buf + 1) * KT * ROW;
+        const uint32_t k_now = lds_at + buf * 2 * KT * ROW + k_at, v_now = lds_at + buf * 2 * KT * ROW + v_at;
         gone = gone_next;
-        if (t + kTile > t_end || gone) {
+        if (t + KT > t_end || gone) {
             // what lies past the end or is not there may be NaN, whose product with a weight of zero is no zero
             for (int i = lane; i < CR * RC; i += 64) {
                 const int r = CR * wave + i / RC;
@@ -326,16 +383,19 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        if (t + kTile < t_end) stage(t + kTile, buf ^ 1);
+        aim(t + KT, buf ^ 1);                 // (past the end: copies of nothing)
+#pragma unroll
+        for (int i = 0; i < 2 * CP; ++i) copy(i);
         if (!mine || t >= most) continue;
-        const bool all = t + kTile <= least && gone == 0;
+        const bool all = t + KT <= least && gone == 0;
         // Scores of 32 tokens; the reference exponent of what follows, and its rare change; weights; their products
         auto scores = [&](int h, float16_t& s) {
             s = float16_t{};
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
                 const half8_t k = *reinterpret_cast<lds_half8>((k_now ^ (32 * x % (16 * (KM + 1)))) + 32 * h * ROW + 32 * x / (16 * (KM + 1)) * (16 * (KM + 1)));
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[x], s, 0, 0, 0);
+                const half8_t qx = x < KS - QL ? q[x < KS - QL ? x : 0] : q_held[(x - KS + QL) * 64 * W];
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qx, s, 0, 0, 0);
             }
             // reads run kAhead products ahead
             __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
@@ -343,6 +403,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             for (int x = 0; x < KS - kAhead; ++x) {
                 __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+                if (x + kAhead >= KS - QL) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
             }
             __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
             __builtin_amdgcn_sched_barrier(0);
@@ -350,9 +411,10 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         auto refer = [&](int h, float16_t& s) {
             if (!all) {
                 const int left = seen - t - 32 * h - 4 * j;
+                const uint32_t none = gone >> (2 * h);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (8 * (i / 4) + i % 4 >= left || (gone >> (2 * h + i / 8) & 1)) s[i] = -INFINITY;
+                    if (8 * (i / 4) + i % 4 >= left || (none >> (i / 8) & 1)) s[i] = -INFINITY;
             }
             float mx = s[0];
 #pragma unroll
@@ -379,25 +441,26 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
                 w[i / 8][i % 8 + 1] = e[1];
             }
         };
-        auto add = [&](int h, const half8_t (&w)[2]) {
+        auto v_read = [&](int h, int y) {        // product y: block y % MB of d, 16 tokens
+            half8_t a;
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int z = 0; z < 2; ++z) {
+                constexpr int TM = RC < 16 ? 2 : 4;      // blocks that turn into one another
+                const int b = y % MB;
+                const uint32_t from = (v_now ^ (64 * (b % TM))) + (32 * h + 16 * (y / MB) + 8 * z) * ROW + 64 * TM * (b / TM);
+                const auto r = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_half4>(from)));
 #pragma unroll
-                for (int b = 0; b < MB; ++b) {
-                    half8_t a;
+                for (int e = 0; e < 4; ++e) a[4 * z + e] = r[e];
+            }
+            return a;
+        };
+        auto add = [&](int h, const half8_t (&w)[2], const half8_t (&first)[VA + 1]) {
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        constexpr int TM = RC < 16 ? 2 : 4;      // blocks that turn into one another
-                        const uint32_t from = (v_now ^ (64 * (b % TM))) + (32 * h + 16 * x + 8 * y) * ROW + 64 * TM * (b / TM);
-                        const auto r = __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16(reinterpret_cast<lds_half4>(from)));
+            for (int y = 0; y < 2 * MB; ++y)
+                acc[y % MB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y < VA ? first[y < VA ? y : 0] : v_read(h, y), w[y / MB], acc[y % MB], 0, 0, 0);
+            if constexpr (VA == 0) __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kAhead, 0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) a[4 * y + e] = r[e];
-                    }
-                    acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[x], acc[b], 0, 0, 0);
-                }
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kAhead, 0);
-#pragma unroll
-            for (int x = 0; x < 2 * MB - kAhead; ++x) {
+            for (int y = 0; y < 2 * MB - kAhead; ++y) {
                 __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
             }
@@ -405,46 +468,113 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             __builtin_amdgcn_sched_barrier(0);
         };
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < KT / 32; ++h) {
             float16_t s;
-            half8_t w[2];
+            half8_t w[2], first[VA + 1];
             scores(h, s);
+#pragma unroll
+            for (int y = 0; y < VA; ++y) first[y] = v_read(h, y);
             refer(h, s);
             weigh(s, w);
-            add(h, w);
+            add(h, w, first);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                // K and V have been read, no copy is on its way
+    asm volatile("" ::: "memory");
+
+    // Parts meet four by four, the last of four to arrive takes their sum on; always (0 + 1) + (2 + 3), so that the bits do
+    // not depend on who is last: scaling by powers of two is exact, and a sum of two has one value.
+    if (parts > 1) {
+        const int w0 = first_id<R>(p, at, tile, hk), ids = (1 << p.slots_log2) + 2;
+        const int mine_at = wave * static_cast<int>(part_bytes(D)) + 16 * lane, stat_at = wave * static_cast<int>(part_bytes(D)) + 128 * D + 8 * lane;
+        typedef unsigned u2 __attribute__((ext_vector_type(2)));
+        unsigned* counters = reinterpret_cast<unsigned*>(p.ws) + w0;
+        for (int n = parts, me = part, step = 1; n > 1; n = (n + kFan - 1) / kFan, me /= kFan, step *= kFan, counters += ids) {
+            const int first = me / kFan * kFan, of = n - first < kFan ? n - first : kFan;
+            if (of == 1) continue;
+            auto slot = [&](int i) {             // of the first's i-th neighbour; of nothing where there is none
+                return __builtin_amdgcn_make_buffer_rsrc(slot_of(p, w0, (first + i) * step), 0, i < of ? static_cast<int>(p.slot_bytes) : 0, 0x00020000);
+            };
+            if (mine) {
+                const auto to = slot(me - first);
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        __builtin_amdgcn_raw_buffer_store_b128(int4_t{__float_as_int(acc[b][4 * i]), __float_as_int(acc[b][4 * i + 1]), __float_as_int(acc[b][4 * i + 2]),
+                                                                      __float_as_int(acc[b][4 * i + 3])},
+                                                               to, mine_at + 1024 * (4 * b + i), 0, kThrough);
+                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(m), __float_as_uint(l)}, to, stat_at, 0, kThrough);
+            }
+            if (!last_in(counters + first * step, of, &flag)) return;
+            if (!mine) continue;
+            const int k = me - first, others = (k ^ 2) & ~1;
+            const __amdgpu_buffer_rsrc_t from[3] = {slot(k ^ 1), slot(others), slot(others + 1)};
+            const bool there[3] = {(k ^ 1) < of, others < of, others + 1 < of};
+            float om[3], ol[3], by[3], top = m;
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                const auto st = __builtin_amdgcn_raw_buffer_load_b64(from[x], stat_at, 0, kThrough);
+                om[x] = there[x] ? __uint_as_float(st[0]) : -INFINITY;
+                ol[x] = __uint_as_float(st[1]);
+                top = fmaxf(top, om[x]);
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) by[x] = om[x] == -INFINITY ? 0.f : exp2_of(om[x] - top);
+            const float keep = m == -INFINITY ? 0.f : exp2_of(m - top);
+            m = top;
+            l = (l * keep + ol[0] * by[0]) + (ol[1] * by[1] + ol[2] * by[2]);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                int4_t o[3][4];
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[x][i] = __builtin_amdgcn_raw_buffer_load_b128(from[x], mine_at + 1024 * (4 * b + i), 0, kThrough);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    acc[b][i] = (acc[b][i] * keep + __int_as_float(o[0][i / 4][i % 4]) * by[0]) +
+                                (__int_as_float(o[1][i / 4][i % 4]) * by[1] + __int_as_float(o[2][i / 4][i % 4]) * by[2]);
+            }
         }
     }
     if (!mine) return;
 
-    const int w0 = parts > 1 ? first_id<R>(p, at, tile, hk) : 0;
-    float* const slot = parts > 1 ? reinterpret_cast<float*>(slot_of(p, w0, part)) : nullptr;
-    const int64_t stats = static_cast<int64_t>(p.slot_bytes / (D * 4 + 8)) * D;       // behind the rows
+    l = sum2(l);
+    // acc[b][i]: d = 32 b + 8 (i / 4) + 4 j + i % 4 of this lane's row
+    float none = 0.f * l;                        // NaN where anything is not finite
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) none = fmaf(acc[b][i], 0.f, none);
+    const unsigned long long odds = __ballot(none != 0.f);
+    const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
     auto out_row = [&](int r) {
         const int tk = token_of(p, r);
         return p.out + (static_cast<int64_t>(at.s.first + tk) * p.Hq + hk * p.group + r - tk * p.group) * D;
     };
-    l = sum2(l);
-    // acc[b][i]: d = 32 b + 8 (i / 4) + 4 j + i % 4 of this lane's row
-    bool odd = !(fabsf(l) < INFINITY);
-#pragma unroll
-    for (int b = 0; b < MB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) odd |= !(fabsf(acc[b][i]) < INFINITY);
-    const unsigned long long odds = __ballot(odd);
-    const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
-    if (wrow + c < rows && !(bad >> c & 1)) {
+    // Whole rows go out, turned in LDS, a wave in its own part of it: a row's 16-byte chunks in an order of its own, so that
+    // what a lane has of its row meets other banks. (A loop, not its body over and over: code that runs once is fetched from
+    // memory.)
+    {
+        constexpr int CH = D / 8, CM = CH < 16 ? CH - 1 : 15;
+        uint8_t* const turn = lds + wave * 64 * D;
         const float by = l > 0.f ? 1.0f / l : 0.f;
-        float* part_row = slot ? slot + static_cast<int64_t>(wrow + c - row0) * D : nullptr;
-        uint16_t* to = out_row(wrow + c);
+        const uint32_t to = lds_at + wave * 64 * D + 16 * (c * CH + (c & CM)) + 8 * j;
 #pragma unroll
         for (int b = 0; b < MB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4_t v = {acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-                if (slot) *reinterpret_cast<float4_t*>(part_row + 32 * b + 8 * i + 4 * j) = v;
-                else *reinterpret_cast<uint2*>(to + 32 * b + 8 * i + 4 * j) = halves(v, by, l == 0.f);
+                const uint2 h = halves(float4_t{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]}, by, l == 0.f);
+                *reinterpret_cast<lds_uint2>((to ^ (64 * (b % ((CM + 1) / 4)) + 16 * i)) + 16 * (CM + 1) * (b / ((CM + 1) / 4))) = uint2_v{h.x, h.y};
             }
-        if (slot && j == 0) *reinterpret_cast<float2*>(slot + stats + 2 * (wrow + c - row0)) = make_float2(m, l);
+#pragma unroll 1
+        for (int i = lane; i < 32 * CH; i += 64) {
+            const int r = i / CH, ch = i % CH;
+            const uint4 v = *reinterpret_cast<const uint4*>(turn + 16 * (r * CH + (ch ^ (r & CM))));
+            if (wrow + r < rows && !(bad >> r & 1)) *reinterpret_cast<uint4*>(out_row(wrow + r) + 8 * ch) = v;
+        }
     }
     // Rows that are not finite, one at a time and token by token: an infinity or NaN in V reaches the rows that see its
     // token, where above it reaches every row of its tile (zero weights times it are NaN).
@@ -457,12 +587,12 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         float qv[E], sum[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) qv[e] = h2f(from[e]) * p.q_by, sum[e] = 0.f;
-        const int upto = seen_by(rr) < t_end ? seen_by(rr) : t_end;
+        const int upto = seen_by(rr);
         float top = -INFINITY, tot = 0.f;
         auto tokens = [&](auto use) {
-            for (int t = t_begin; t < upto; t += 16) {
+            for (int t = 0; t < upto; t += 16) {
                 int page, prow;
-                place(t / 16, page, prow);
+                place(t / 16, upto, page, prow);
                 for (int x = 0; page >= 0 && x < 16 && t + x < upto; ++x) {
                     const uint16_t* k = kh + page * p.k_page + static_cast<int64_t>(prow + x) * p.k_token + E * lane;
                     float dot = 0.f;
@@ -474,7 +604,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             }
         };
         tokens([&](float s, const uint16_t*) { top = fmaxf(top, s); });
-        const float less = top == -INFINITY ? 0.f : top - kTop;
+        const float less = top == -INFINITY ? 0.f : top;
         tokens([&](float s, const uint16_t* v) {
             const float w = exp2_of(s - less);
             tot += w;
@@ -483,70 +613,19 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         });
         const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (slot) slot[static_cast<int64_t>(rr - row0) * D + E * lane + e] = sum[e];
-            else out_row(rr)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
-        }
-        if (slot && lane == 0) *reinterpret_cast<float2*>(slot + stats + 2 * (rr - row0)) = make_float2(top, tot);
+        for (int e = 0; e < E; ++e) out_row(rr)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
     }
 }
 
-// ------------------------------------------------------------------- the parts' sum --
-template <int D, int W>
-__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
-    constexpr int R = 32 * W;
-    Place at;
-    auto cut = [&](const Seq& s, int S) { return s.len > S ? tiles_with<R>(p, s, tiles_of<R>(p, s), S) * p.Hkv : 0; };
-    if (!find<R>(p, blockIdx.x, at, cut)) return;
-    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
-    const int hk = at.unit % p.Hkv, tile = tiles - 1 - at.unit / p.Hkv;
-    const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1;
-    const int end = base + token_of(p, last_row) + 1, parts = (end + at.S - 1) / at.S;
-    const int w0 = first_id<R>(p, at, tile, hk);
-    const int64_t stats = static_cast<int64_t>(p.slot_bytes / (D * 4 + 8)) * D;
-    for (int i = threadIdx.x; i < kJoinRows * D / 4; i += 256) {
-        const int r = blockIdx.y * kJoinRows + i / (D / 4), d = i % (D / 4) * 4, rr = row0 + r;
-        if (rr > last_row) break;
-        float4_t sum = {0, 0, 0, 0};
-        float top = -INFINITY, tot = 0.f;
-        constexpr int kBatch = 8;                // loads of a batch go out together
-        for (int u0 = 0; u0 < parts; u0 += kBatch) {
-            float4_t o[kBatch];
-            float2 st[kBatch];
-            float most = top;
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const float* slot = reinterpret_cast<const float*>(slot_of(p, w0, u0 + u < parts ? u0 + u : parts - 1));
-                o[u] = *reinterpret_cast<const float4_t*>(slot + static_cast<int64_t>(r) * D + d);
-                st[u] = *reinterpret_cast<const float2*>(slot + stats + 2 * r);
-            }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) most = fmaxf(most, st[u].x);
-            const float keep = top == -INFINITY ? 0.f : exp2_of(top - most);
-            tot *= keep;
-            sum *= keep;
-            top = most;
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                if (u0 + u >= parts) continue;
-                const float by = st[u].x == -INFINITY ? 0.f : exp2_of(st[u].x - top);
-                tot = fmaf(st[u].y, by, tot);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) sum[x] = fmaf(o[u][x], by, sum[x]);
-            }
-        }
-        const int tk = token_of(p, rr);
-        const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
-        *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(at.s.first + tk) * p.Hq + hk * p.group + rr - tk * p.group) * D + d) = halves(sum, by, tot == 0.f);
-    }
-}
-
-// Waves of a workgroup.
-int choose_waves(int64_t D) { return D == 256 ? 8 : 4; }
+// Units side by side on one XCD: of as many tiles as a sequence has on average.
+int choose_near_log2(int64_t tiles, int64_t B) { return 2; }
+// Rows of a workgroup, and tokens that it takes at a time.
+constexpr int kRows = 128;
+constexpr int tokens_of(int64_t D) { return D == 256 ? 32 : 64; }
 // Parts to cut for, of rows that read up to `most` tokens: what the chip holds at once.  -1: nothing to cut.
-int choose_slots_log2(int64_t most, int64_t D) { return most <= kLeast ? -1 : D == 256 ? 8 : 9; }
-int64_t slot_rows_of(int64_t T, int64_t group, int64_t D) { return std::min<int64_t>(32 * choose_waves(D), T * group); }
-int64_t split_bytes(int slots_log2, int64_t rows, int64_t D) { return slots_log2 < 0 ? 0 : 2 * ((int64_t(1) << slots_log2) + 2) * part_bytes(rows, D); }
+int choose_slots_log2(int64_t most, int64_t D) { return most <= kLeast ? -1 : D == 64 ? 10 : 9; }
+int64_t slot_bytes_of(int64_t T, int64_t group, int64_t D) { return ceil_div(std::min<int64_t>(kRows, T * group), 32) * part_bytes(D); }
+int64_t split_bytes(int slots_log2, int64_t slot_bytes) { return slots_log2 < 0 ? 0 : kCounterBytes + 2 * ((int64_t(1) << slots_log2) + 2) * slot_bytes; }
 
 }  // namespace
 }  // namespace mcv
@@ -557,7 +636,7 @@ extern "C" {
 
 int64_t mcv_paged_attention_chunk_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seq_len) {
     if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || T > 0x7fffffff / Hq || D <= 0 || max_seq_len < 0) return 0;
-    return split_bytes(choose_slots_log2(std::min(max_seq_len, kMaxLen), D), slot_rows_of(T, Hq / Hkv, D), D);
+    return split_bytes(choose_slots_log2(std::min(max_seq_len, kMaxLen), D), slot_bytes_of(T, Hq / Hkv, D));
 }
 
 int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
@@ -588,13 +667,14 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     const int64_t held = table_width > kMaxLen / page_size ? kMaxLen : table_width * page_size;
     const int64_t most = max_seq_len < held ? max_seq_len : held;
     const int64_t group = Hq / Hkv;
-    const int64_t rows = slot_rows_of(T, group, D), tiles = std::min(T * group / (32 * choose_waves(D)) + B, T * group);
+    const int64_t slot_bytes = slot_bytes_of(T, group, D), tiles = std::min(T * group / kRows + B, T * group);
     int slots_log2 = choose_slots_log2(most, D);
-    if (slots_log2 >= 0 && (!workspace || workspace_bytes < split_bytes(slots_log2, rows, D))) slots_log2 = -1;
+    if (slots_log2 >= 0 && (!workspace || workspace_bytes < split_bytes(slots_log2, slot_bytes))) slots_log2 = -1;
     if (slots_log2 >= 0 && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", who);
+    const int near_log2 = choose_near_log2(tiles, B);
     const int64_t slots = slots_log2 < 0 ? 0 : int64_t(1) << slots_log2;
-    if (tiles * Hkv + slots > 0x7fffffff) return fail(MCV_ERR_SHAPE, "%s: too many rows B=%lld T=%lld Hq=%lld", who, (long long)B, (long long)T, (long long)Hq);
+    if (tiles * Hkv + slots > 0x7fffff00) return fail(MCV_ERR_SHAPE, "%s: too many rows B=%lld T=%lld Hq=%lld", who, (long long)B, (long long)T, (long long)Hq);
     const uint32_t page16 = static_cast<uint32_t>(page_size / 16);
     auto inverse = [](uint64_t n) { return n > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + n - 1) / n) : 0; };
     const ChunkArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache),
@@ -603,18 +683,12 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
                       static_cast<int>(k_token), static_cast<int>(v_token), static_cast<int>(pages), static_cast<int>(page16), static_cast<int>(most),
                       static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
                       inverse(page16), inverse(group), scale == 0.0 ? 1.f : std::fabs(static_cast<float>(scale) * kLog2e), scale < 0.0 ? -1.f : scale == 0.0 ? 0.f : 1.f,
-                      slots_log2, part_bytes(rows, D)};
+                      slots_log2, near_log2, slot_bytes};
     const auto s = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(tiles * Hkv + slots)), joins(static_cast<unsigned>(std::min(tiles * Hkv, slots)), static_cast<unsigned>(ceil_div(rows, kJoinRows)));
-    auto launch = [&](auto part, auto join) {
-        hipLaunchKernelGGL(part, grid, dim3(static_cast<unsigned>(64 * choose_waves(D))), static_cast<unsigned>(4 * kTile * 2 * D), s, a);
-        const int rc = check_launch("chunk_attention_kernel");
-        if (rc != MCV_OK || !slots) return rc;
-        hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
-        return check_launch("chunk_join_kernel");
-    };
-    return D == 64 ? launch(chunk_attention_kernel<64, 4>, chunk_join_kernel<64, 4>) :
-           D == 128 ? launch(chunk_attention_kernel<128, 4>, chunk_join_kernel<128, 4>) : launch(chunk_attention_kernel<256, 8>, chunk_join_kernel<256, 8>);
+    const dim3 grid(static_cast<unsigned>(ceil_div(tiles * Hkv + slots, 8 << near_log2) * (8 << near_log2)));
+    auto fn = D == 64 ? chunk_attention_kernel<64, 4, tokens_of(64)> : D == 128 ? chunk_attention_kernel<128, 4, tokens_of(128)> : chunk_attention_kernel<256, 4, tokens_of(256)>;
+    hipLaunchKernelGGL(fn, grid, dim3(2 * kRows), static_cast<unsigned>(8 * tokens_of(D) * D + (D == 256 ? 2 * 32 * kRows : 0)), s, a);
+    return check_launch("chunk_attention_kernel");
 }
 
 }  // extern "C"

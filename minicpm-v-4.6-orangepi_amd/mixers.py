@@ -34,7 +34,8 @@ def binding():
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         most = lib().mcv_paged_attention_workspace_bytes(512, 16, 1, 256, 1 << 20)      # of any call
-        mod.bind(McvError, _empty_on, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, most, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES)
+        mod.bind(McvError, _empty_on, gemm_workspace, _GEMM_WS, GEMM_WORKSPACE_BYTES, most, delta_workspace, _DELTA_WS, *DELTA_WORKSPACE_BYTES,
+                 chunk_workspace, _CHUNK_WS, CHUNK_WORKSPACE_BYTES)
         _BINDING = mod
     return _BINDING
 
@@ -68,6 +69,27 @@ def delta_workspace(nbytes: int, device, stream=None):
     if ws is not None:
         return ws
     return _new_workspace(_DELTA_WS, _DELTA_WS_CAPTURE, key, 0, 0, dev, handle, stream)
+
+
+# The chunks' parts of a long cache meet in a workspace that is as large for any call as for the largest, so that a stream
+# holds one; its counters start and end at zero.
+CHUNK_WORKSPACE_BYTES = 144 << 20
+_CHUNK_COUNTER_BYTES = 24576
+_CHUNK_WS: dict = {}            # (device, stream, bytes) -> workspace
+_CHUNK_WS_CAPTURE: dict = {}    # the same -> (capture id, workspace of that graph)
+
+
+def chunk_workspace(nbytes: int, device, stream=None):
+    """The workspace of paged_attention_chunk for calls on one stream; kept, and recorded by graphs, as
+    gemm_workspace's is."""
+    torch = _torch()
+    dev = torch.device(device)
+    handle = _stream(stream)
+    key = (dev.index if dev.index is not None else torch.cuda.current_device(), handle, max(nbytes, CHUNK_WORKSPACE_BYTES))
+    ws = _CHUNK_WS.get(key)
+    if ws is not None:
+        return ws
+    return _new_workspace(_CHUNK_WS, _CHUNK_WS_CAPTURE, key, _CHUNK_COUNTER_BYTES, _CHUNK_COUNTER_BYTES, dev, handle, stream)
 
 
 def gated_delta_rule(q, k, v, g, beta, state=None, *, cu_seqlens=None, scale=None, normalize=False, state_index=None,
