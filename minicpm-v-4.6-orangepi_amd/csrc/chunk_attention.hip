@@ -35,8 +35,8 @@ struct ChunkArgs {
 };
 
 
-constexpr int kFan = 4;                          // parts that one of them joins
-constexpr int64_t kCounterBytes = 24576;         // five levels of joining, a counter for each part
+constexpr int kFan = 4;                          // parts of a tile that the last of them to arrive joins; where there are more, a launch of its own does
+constexpr int64_t kCounterBytes = 8192;          // a counter for each part
 
 // Bytes of a wave's part: a lane's sums, and its reference exponent and sum of weights, as they are in registers.
 __host__ __device__ constexpr int64_t part_bytes(int64_t D) { return 64 * (2 * D + 8); }
@@ -51,21 +51,27 @@ __device__ __forceinline__ float sum2(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// What no kernel in flight writes, at an address that a whole wave shares: read through the scalar cache.
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ __forceinline__ scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)reinterpret_cast<uintptr_t>(p); }
+
 // ---------------------------------------------------------------- who does what --
 struct Seq {
     int first, n, len;                           // first new row, new tokens, tokens in the cache
 };
-__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b) {
+template <class Ints>
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b, Ints lens, Ints cu) {
     if (b >= p.B) return {0, 0, 0};
     int first, next;
-    const int held = p.lens[b];
-    if (p.cu) first = p.cu[b], next = p.cu[b + 1];
+    const int held = lens[b];
+    if (cu) first = cu[b], next = cu[b + 1];
     else first = b * (p.T / p.B), next = first + p.T / p.B;
     auto inside = [](int v, int most) { return v < 0 ? 0 : v > most ? most : v; };
     first = inside(first, p.T);
     next = inside(next, p.T);
     return {first, next > first ? next - first : 0, inside(held, p.max_len)};
 }
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b) { return seq_of(p, b, p.lens, p.cu); }
 __device__ __forceinline__ int token_of(const ChunkArgs& p, int row) {         // row / group
     if (p.group == 1) return row;
     int t = static_cast<int>(__umulhi(static_cast<uint32_t>(row), p.group_inv));      // one too many at most
@@ -118,6 +124,19 @@ struct Place {
 };
 template <int R, class Count>
 __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Count count) {
+    auto part_of = [&](int64_t total) {
+        if (p.slots_log2 < 0) return 0x40000000;
+        const int64_t S = (((total - 1) >> p.slots_log2) + kTile) / kTile * kTile;
+        return static_cast<int>(S < kLeast ? kLeast : S < 0x40000000 ? S : 0x40000000);
+    };
+    if (p.B == 1) {                              // (nothing to look for)
+        at.s = seq_of(p, 0, as_scalar(p.lens), as_scalar(p.cu));
+        at.b = 0;
+        at.unit = me;
+        at.read = 0;
+        at.S = part_of(p.Hkv * reads_below<R>(p, at.s, tiles_of<R>(p, at.s)));
+        return me < count(at.s, at.S);
+    }
     const int lane = threadIdx.x & 63, span = (p.B + 63) / 64;
     Seq s = seq_of(p, lane);                     // (of span 1)
     auto reads = [&](const Seq& s) { return p.Hkv * reads_below<R>(p, s, tiles_of<R>(p, s)); };
@@ -126,12 +145,7 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
     else
         for (int i = 0; i < span; ++i) read += reads(seq_of(p, lane * span + i));
     int64_t read_upto = wave_scan(read);
-    const int64_t total = lane_of(read_upto, 63);
-    at.S = 0x40000000;
-    if (p.slots_log2 >= 0) {
-        const int64_t S = (((total - 1) >> p.slots_log2) + kTile) / kTile * kTile;
-        at.S = static_cast<int>(S < kLeast ? kLeast : S < 0x40000000 ? S : 0x40000000);
-    }
+    at.S = part_of(lane_of(read_upto, 63));
     int units = 0;
     if (span == 1) units = count(s, at.S);
     else
@@ -196,6 +210,67 @@ __device__ __forceinline__ bool last_in(unsigned* counter, int n, int* flag) {
     }
     __syncthreads();
     return *flag != 0;
+}
+
+// The page of the 16 tokens from 16 t16 on (-1: not there, or from `upto` on) and their first row in it.
+__device__ __forceinline__ void page_of(const ChunkArgs& p, const int32_t* table, int t16, int upto, int& page, int& row) {
+    uint32_t i = static_cast<uint32_t>(t16);
+    row = 0;
+    if (p.page16 > 1) {
+        i = __umulhi(static_cast<uint32_t>(t16), p.page16_inv);  // one too many at most
+        int r = t16 - static_cast<int>(i * p.page16);
+        if (r < 0) --i, r += p.page16;
+        row = 16 * r;
+    }
+    page = 16 * t16 < upto ? table[i] : -1;
+    page = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages) ? page : -1;
+}
+__device__ __forceinline__ uint16_t* out_row(const ChunkArgs& p, const Place& at, int hk, int row, int D) {
+    const int token = token_of(p, row);
+    return p.out + (static_cast<int64_t>(at.s.first + token) * p.Hq + hk * p.group + row - token * p.group) * D;
+}
+
+// A row that is not finite, token by token, its d from d0 to d1: an infinity or NaN in V reaches the rows that see its token,
+// where on the matrix cores it reaches every row of its tile (zero weights times it are NaN).
+template <int D>
+__device__ __forceinline__ void slow_row(const ChunkArgs& p, const Place& at, int hk, int row, int d0, int d1) {
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63, token = token_of(p, row);
+    const uint16_t* from = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head + E * lane;
+    float q[E], sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] = h2f(from[e]) * p.q_by, sum[e] = 0.f;
+    const int upto = at.s.len - at.s.n + token + 1;
+    float top = -INFINITY, tot = 0.f;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {       // the largest score; the weights
+        const float less = top == -INFINITY ? 0.f : top;
+        for (int t = 0; t < upto; t += 16) {
+            int page, first;
+            page_of(p, p.table + at.b * p.table_row, t / 16, upto, page, first);
+#pragma unroll 1
+            for (int x = 0; page >= 0 && x < 16 && t + x < upto; ++x) {
+                const uint16_t* k = p.k + hk * p.k_head + page * p.k_page + static_cast<int64_t>(first + x) * p.k_token + E * lane;
+                float dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) dot = fmaf(q[e], h2f(k[e]), dot);
+                const float s = wave_butterfly(dot, [](float a, float b) { return a + b; }) * p.scale_log2;
+                if (pass == 0) {
+                    top = fmaxf(top, s);
+                    continue;
+                }
+                const uint16_t* v = p.v + hk * p.v_head + page * p.v_page + static_cast<int64_t>(first + x) * p.v_token + E * lane;
+                const float w = exp2_of(s - less);
+                tot += w;
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[e] = fmaf(w, h2f(v[e]), sum[e]);
+            }
+        }
+    }
+    const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (E * lane + e >= d0 && E * lane + e < d1) out_row(p, at, hk, row, D)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
 }
 
 __device__ __forceinline__ uint2 halves(const float4_t& v, float by, bool none) {
@@ -276,22 +351,15 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     const int32_t* table = p.table + at.b * p.table_row;
     const uint16_t* kh = p.k + hk * p.k_head;
     const uint16_t* vh = p.v + hk * p.v_head;
-    // The page of the 16 tokens from 16 t16 on (-1: not there, or past the end) and their first row in it.
-    auto place = [&](int t16, int upto, int& page, int& prow) {
-        uint32_t i = static_cast<uint32_t>(t16);
-        prow = 0;
-        if (p.page16 > 1) {
-            i = __umulhi(static_cast<uint32_t>(t16), p.page16_inv);      // one too many at most
-            int r = t16 - static_cast<int>(i * p.page16);
-            if (r < 0) --i, r += p.page16;
-            prow = 16 * r;
-        }
-        page = 16 * t16 < upto ? table[i] : -1;
-        page = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages) ? page : -1;
-    };
     // A lane holds that of one of the 64 groups of 16 tokens from token `known` on.
     int my_page = -1, my_row = 0, known = t_begin;
-    place(known / 16 + lane, t_end, my_page, my_row);
+    page_of(p, table, known / 16 + lane, t_end, my_page, my_row);
+    half8_t all[KS];
+    if (mine) {
+        const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) all[s] = *reinterpret_cast<const half8_t*>(qr + 16 * s + 8 * j);
+    }
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
     // A tile's copies. Rows lie in LDS as they do in memory, but a row's chunks in an order of its own, so that reads of a
     // column meet other banks. Each wave has CP copies of K and CP of V to make, spread over the products of the tile before:
@@ -317,20 +385,20 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         v_from = rows16(vh, p.v_page, p.v_token);
         if (g == 64 - KT / 16) {
             known += 1024;
-            place(known / 16 + lane, t_end, my_page, my_row);
+            page_of(p, table, known / 16 + lane, t_end, my_page, my_row);
         }
     };
+    const uint32_t lr = static_cast<uint32_t>(lane) / RC, lc = static_cast<uint32_t>(lane) % RC;
+    const uint32_t k_row = 2 * lr * p.k_token, v_row = 2 * lr * p.v_token, k_chunk = 16 * (lc ^ (lr & KM)), v_chunk = 16 * (lc ^ turn_of_v(lr));
     // (Written out: the compiler would have every read of V in LDS wait for all copies on their way, whatever buffer they go
     // to. The loop waits for them where it takes the tile.)
     auto copy = [&](int i) {                     // 0 .. CP - 1: of K, then of V
-        uint32_t opaque = lane;                  // (offsets made from it would be kept through the loop)
-        asm volatile("" : "+v"(opaque));
-        const uint32_t lr = opaque / RC, lc = opaque % RC;
         const bool of_v = i >= CP;
-        const int row = first_row + (of_v ? i - CP : i) * RPI, stride = of_v ? p.v_token : p.k_token;
-        const uint32_t turn = of_v ? turn_of_v(row + lr) : (row + lr) & KM;
+        const int row = first_row + (of_v ? i - CP : i) * RPI;
+        uint32_t chunk = of_v ? v_chunk : k_chunk;       // (opaque: what is made from it would be kept through the loop)
+        asm volatile("" : "+v"(chunk));
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(copy_to + (of_v ? KT * ROW + (i - CP) * 1024 : i * 1024)),
-                     "v"(2 * lr * stride + 16 * (lc ^ turn)), "s"(of_v ? v_from : k_from), "s"(2 * row * stride));
+                     "v"((chunk ^ (16 * (of_v ? turn_of_v(row) : row & KM))) + (of_v ? v_row : k_row)), "s"(of_v ? v_from : k_from), "s"(2 * row * (of_v ? p.v_token : p.k_token)));
     };
     if (t_begin < t_end) {
         aim(t_begin, 0);
@@ -339,10 +407,6 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     }
     half8_t q[KS - QL], *const q_held = reinterpret_cast<half8_t*>(lds + 4 * KT * ROW) + threadIdx.x;
     if (mine) {
-        const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head;
-        half8_t all[KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) all[s] = *reinterpret_cast<const half8_t*>(qr + 16 * s + 8 * j);
         if (p.q_by != 1.f)
 #pragma unroll
             for (int s = 0; s < KS; ++s) all[s] *= static_cast<_Float16>(p.q_by);
@@ -483,60 +547,55 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     __builtin_amdgcn_s_barrier();                // K and V have been read, no copy is on its way
     asm volatile("" ::: "memory");
 
-    // Parts meet four by four, the last of four to arrive takes their sum on; always (0 + 1) + (2 + 3), so that the bits do
-    // not depend on who is last: scaling by powers of two is exact, and a sum of two has one value.
+    // Up to four parts meet in the last of them to arrive; always (0 + 1) + (2 + 3), so that the bits do not depend on who is
+    // last: scaling by powers of two is exact, and a sum of two has one value.
     if (parts > 1) {
-        const int w0 = first_id<R>(p, at, tile, hk), ids = (1 << p.slots_log2) + 2;
+        const int w0 = first_id<R>(p, at, tile, hk);
         const int mine_at = wave * static_cast<int>(part_bytes(D)) + 16 * lane, stat_at = wave * static_cast<int>(part_bytes(D)) + 128 * D + 8 * lane;
         typedef unsigned u2 __attribute__((ext_vector_type(2)));
-        unsigned* counters = reinterpret_cast<unsigned*>(p.ws) + w0;
-        for (int n = parts, me = part, step = 1; n > 1; n = (n + kFan - 1) / kFan, me /= kFan, step *= kFan, counters += ids) {
-            const int first = me / kFan * kFan, of = n - first < kFan ? n - first : kFan;
-            if (of == 1) continue;
-            auto slot = [&](int i) {             // of the first's i-th neighbour; of nothing where there is none
-                return __builtin_amdgcn_make_buffer_rsrc(slot_of(p, w0, (first + i) * step), 0, i < of ? static_cast<int>(p.slot_bytes) : 0, 0x00020000);
-            };
-            if (mine) {
-                const auto to = slot(me - first);
+        auto slot = [&](int i) {                 // of nothing where there is no such part
+            return __builtin_amdgcn_make_buffer_rsrc(slot_of(p, w0, i), 0, i < parts ? static_cast<int>(p.slot_bytes) : 0, 0x00020000);
+        };
+        if (mine) {
+            const auto to = slot(part);
 #pragma unroll
-                for (int b = 0; b < MB; ++b)
+            for (int b = 0; b < MB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        __builtin_amdgcn_raw_buffer_store_b128(int4_t{__float_as_int(acc[b][4 * i]), __float_as_int(acc[b][4 * i + 1]), __float_as_int(acc[b][4 * i + 2]),
-                                                                      __float_as_int(acc[b][4 * i + 3])},
-                                                               to, mine_at + 1024 * (4 * b + i), 0, kThrough);
-                __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(m), __float_as_uint(l)}, to, stat_at, 0, kThrough);
-            }
-            if (!last_in(counters + first * step, of, &flag)) return;
-            if (!mine) continue;
-            const int k = me - first, others = (k ^ 2) & ~1;
-            const __amdgpu_buffer_rsrc_t from[3] = {slot(k ^ 1), slot(others), slot(others + 1)};
-            const bool there[3] = {(k ^ 1) < of, others < of, others + 1 < of};
-            float om[3], ol[3], by[3], top = m;
+                for (int i = 0; i < 4; ++i)
+                    __builtin_amdgcn_raw_buffer_store_b128(int4_t{__float_as_int(acc[b][4 * i]), __float_as_int(acc[b][4 * i + 1]), __float_as_int(acc[b][4 * i + 2]),
+                                                                  __float_as_int(acc[b][4 * i + 3])},
+                                                           to, mine_at + 1024 * (4 * b + i), 0, kThrough);
+            __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(m), __float_as_uint(l)}, to, stat_at, 0, kThrough);
+        }
+        if (parts > kFan) return;
+        if (!last_in(reinterpret_cast<unsigned*>(p.ws) + w0, parts, &flag) || !mine) return;
+        const int others = (part ^ 2) & ~1, with[3] = {part ^ 1, others, others + 1};
+        __amdgpu_buffer_rsrc_t from[3];
+        float om[3], ol[3], by[3], top = m;
 #pragma unroll
-            for (int x = 0; x < 3; ++x) {
-                const auto st = __builtin_amdgcn_raw_buffer_load_b64(from[x], stat_at, 0, kThrough);
-                om[x] = there[x] ? __uint_as_float(st[0]) : -INFINITY;
-                ol[x] = __uint_as_float(st[1]);
-                top = fmaxf(top, om[x]);
-            }
+        for (int x = 0; x < 3; ++x) {
+            from[x] = slot(with[x]);
+            const auto st = __builtin_amdgcn_raw_buffer_load_b64(from[x], stat_at, 0, kThrough);
+            om[x] = with[x] < parts ? __uint_as_float(st[0]) : -INFINITY;
+            ol[x] = __uint_as_float(st[1]);
+            top = fmaxf(top, om[x]);
+        }
 #pragma unroll
-            for (int x = 0; x < 3; ++x) by[x] = om[x] == -INFINITY ? 0.f : exp2_of(om[x] - top);
-            const float keep = m == -INFINITY ? 0.f : exp2_of(m - top);
-            m = top;
-            l = (l * keep + ol[0] * by[0]) + (ol[1] * by[1] + ol[2] * by[2]);
+        for (int x = 0; x < 3; ++x) by[x] = om[x] == -INFINITY ? 0.f : exp2_of(om[x] - top);
+        const float keep = m == -INFINITY ? 0.f : exp2_of(m - top);
+        m = top;
+        l = (l * keep + ol[0] * by[0]) + (ol[1] * by[1] + ol[2] * by[2]);
 #pragma unroll
-            for (int b = 0; b < MB; ++b) {
-                int4_t o[3][4];
+        for (int b = 0; b < MB; ++b) {
+            int4_t o[3][4];
 #pragma unroll
-                for (int x = 0; x < 3; ++x)
+            for (int x = 0; x < 3; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[x][i] = __builtin_amdgcn_raw_buffer_load_b128(from[x], mine_at + 1024 * (4 * b + i), 0, kThrough);
+                for (int i = 0; i < 4; ++i) o[x][i] = __builtin_amdgcn_raw_buffer_load_b128(from[x], mine_at + 1024 * (4 * b + i), 0, kThrough);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    acc[b][i] = (acc[b][i] * keep + __int_as_float(o[0][i / 4][i % 4]) * by[0]) +
-                                (__int_as_float(o[1][i / 4][i % 4]) * by[1] + __int_as_float(o[2][i / 4][i % 4]) * by[2]);
-            }
+            for (int i = 0; i < 16; ++i)
+                acc[b][i] = (acc[b][i] * keep + __int_as_float(o[0][i / 4][i % 4]) * by[0]) +
+                            (__int_as_float(o[1][i / 4][i % 4]) * by[1] + __int_as_float(o[2][i / 4][i % 4]) * by[2]);
         }
     }
     if (!mine) return;
@@ -550,10 +609,6 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         for (int i = 0; i < 16; ++i) none = fmaf(acc[b][i], 0.f, none);
     const unsigned long long odds = __ballot(none != 0.f);
     const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
-    auto out_row = [&](int r) {
-        const int tk = token_of(p, r);
-        return p.out + (static_cast<int64_t>(at.s.first + tk) * p.Hq + hk * p.group + r - tk * p.group) * D;
-    };
     // Whole rows go out, turned in LDS, a wave in its own part of it: a row's 16-byte chunks in an order of its own, so that
     // what a lane has of its row meets other banks. (A loop, not its body over and over: code that runs once is fetched from
     // memory.)
@@ -573,47 +628,82 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         for (int i = lane; i < 32 * CH; i += 64) {
             const int r = i / CH, ch = i % CH;
             const uint4 v = *reinterpret_cast<const uint4*>(turn + 16 * (r * CH + (ch ^ (r & CM))));
-            if (wrow + r < rows && !(bad >> r & 1)) *reinterpret_cast<uint4*>(out_row(wrow + r) + 8 * ch) = v;
+            if (wrow + r < rows && !(bad >> r & 1)) *reinterpret_cast<uint4*>(out_row(p, at, hk, wrow + r, D) + 8 * ch) = v;
         }
     }
-    // Rows that are not finite, one at a time and token by token: an infinity or NaN in V reaches the rows that see its
-    // token, where above it reaches every row of its tile (zero weights times it are NaN).
+#pragma unroll 1
     for (uint32_t left = bad; left; left &= left - 1) {
         const int rr = wrow + __builtin_ctz(left);
-        if (rr >= rows) break;
-        constexpr int E = D / 64;
-        const int tk = token_of(p, rr);
-        const uint16_t* from = p.q + static_cast<int64_t>(at.s.first + tk) * p.q_row + static_cast<int64_t>(hk * p.group + rr - tk * p.group) * p.q_head + E * lane;
-        float qv[E], sum[E];
+        if (rr < rows) slow_row<D>(p, at, hk, rr, 0, D);
+    }
+}
+
+// ------------------------------------------------------------------- many parts' sum --
+// Of the tiles that are in more than kFan parts: a wave has 32 rows and 32 d, as one of their parts has them in its registers.
+template <int D, int R>
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
+    constexpr int MB = D / 32;
+    Place at;
+    auto many = [&](const Seq& s, int S) { return s.len > kFan * static_cast<int64_t>(S) ? tiles_with<R>(p, s, tiles_of<R>(p, s), kFan * static_cast<int64_t>(S)) * p.Hkv : 0; };
+    if (!find<R>(p, blockIdx.x, at, many)) return;
+    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
+    const int hk = at.unit % p.Hkv, tile = tiles - 1 - at.unit / p.Hkv;
+    const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5;
+    const int piece = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = piece / MB, b = piece % MB;
+    const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1, wrow = row0 + 32 * wave;
+    if (wrow > last_row) return;
+    const int parts = (base + token_of(p, last_row) + at.S) / at.S;      // ceil(what the last row sees / S)
+    const int w0 = first_id<R>(p, at, tile, hk);
+    float4_t sum[4] = {};
+    float top = -INFINITY, l = 0.f;
+    constexpr int kBatch = 4;                    // loads of a batch go out together
+    for (int u0 = 0; u0 < parts; u0 += kBatch) {
+        float4_t o[kBatch][4];
+        float2 st[kBatch];
+        float most = top;
 #pragma unroll
-        for (int e = 0; e < E; ++e) qv[e] = h2f(from[e]) * p.q_by, sum[e] = 0.f;
-        const int upto = seen_by(rr);
-        float top = -INFINITY, tot = 0.f;
-        auto tokens = [&](auto use) {
-            for (int t = 0; t < upto; t += 16) {
-                int page, prow;
-                place(t / 16, upto, page, prow);
-                for (int x = 0; page >= 0 && x < 16 && t + x < upto; ++x) {
-                    const uint16_t* k = kh + page * p.k_page + static_cast<int64_t>(prow + x) * p.k_token + E * lane;
-                    float dot = 0.f;
+        for (int u = 0; u < kBatch; ++u) {
+            const uint8_t* slot = slot_of(p, w0, u0 + u < parts ? u0 + u : parts - 1) + wave * part_bytes(D);
+            st[u] = *reinterpret_cast<const float2*>(slot + 128 * D + 8 * lane);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) dot = fmaf(qv[e], h2f(k[e]), dot);
-                    use(wave_butterfly(dot, [](float a, float b) { return a + b; }) * p.scale_log2,
-                        vh + page * p.v_page + static_cast<int64_t>(prow + x) * p.v_token + E * lane);
-                }
-            }
-        };
-        tokens([&](float s, const uint16_t*) { top = fmaxf(top, s); });
-        const float less = top == -INFINITY ? 0.f : top;
-        tokens([&](float s, const uint16_t* v) {
-            const float w = exp2_of(s - less);
-            tot += w;
+            for (int i = 0; i < 4; ++i) o[u][i] = *reinterpret_cast<const float4_t*>(slot + 1024 * (4 * b + i) + 16 * lane);
+        }
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] = fmaf(w, h2f(v[e]), sum[e]);
-        });
-        const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
+        for (int u = 0; u < kBatch; ++u) most = fmaxf(most, st[u].x);
+        const float keep = top == -INFINITY ? 0.f : exp2_of(top - most);
+        l *= keep;
 #pragma unroll
-        for (int e = 0; e < E; ++e) out_row(rr)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
+        for (int i = 0; i < 4; ++i) sum[i] *= keep;
+        top = most;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (u0 + u >= parts) continue;
+            const float by = st[u].x == -INFINITY ? 0.f : exp2_of(st[u].x - top);
+            l = fmaf(st[u].y, by, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[i][e] = fmaf(o[u][i][e], by, sum[i][e]);
+        }
+    }
+    l = sum2(l);
+    float none = 0.f * l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) none = fmaf(sum[i][e], 0.f, none);
+    const unsigned long long odds = __ballot(none != 0.f);
+    const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
+    if (wrow + c <= last_row && !(bad >> c & 1)) {
+        uint16_t* to = out_row(p, at, hk, wrow + c, D) + 32 * b + 4 * j;
+        const float by = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(to + 8 * i) = halves(sum[i], by, l == 0.f);
+    }
+#pragma unroll 1
+    for (uint32_t left = bad; left; left &= left - 1) {
+        const int rr = wrow + __builtin_ctz(left);
+        if (rr <= last_row) slow_row<D>(p, at, hk, rr, 32 * b, 32 * b + 32);
     }
 }
 
@@ -688,7 +778,12 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     const dim3 grid(static_cast<unsigned>(ceil_div(tiles * Hkv + slots, 8 << near_log2) * (8 << near_log2)));
     auto fn = D == 64 ? chunk_attention_kernel<64, 4, tokens_of(64)> : D == 128 ? chunk_attention_kernel<128, 4, tokens_of(128)> : chunk_attention_kernel<256, 4, tokens_of(256)>;
     hipLaunchKernelGGL(fn, grid, dim3(2 * kRows), static_cast<unsigned>(8 * tokens_of(D) * D + (D == 256 ? 2 * 32 * kRows : 0)), s, a);
-    return check_launch("chunk_attention_kernel");
+    rc = check_launch("chunk_attention_kernel");
+    if (rc != MCV_OK || most <= kFan * kLeast || !slots) return rc;
+    const dim3 joins(static_cast<unsigned>(std::min(tiles * Hkv, slots / kFan)), static_cast<unsigned>(ceil_div(ceil_div(std::min<int64_t>(kRows, T * group), 32) * D, 128)));
+    auto join = D == 64 ? chunk_join_kernel<64, kRows> : D == 128 ? chunk_join_kernel<128, kRows> : chunk_join_kernel<256, kRows>;
+    hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
+    return check_launch("chunk_join_kernel");
 }
 
 }  // extern "C"

@@ -74,7 +74,7 @@ def delta_workspace(nbytes: int, device, stream=None):
 # The chunks' parts of a long cache meet in a workspace that is as large for any call as for the largest, so that a stream
 # holds one; its counters start and end at zero.
 CHUNK_WORKSPACE_BYTES = 144 << 20
-_CHUNK_COUNTER_BYTES = 24576
+_CHUNK_COUNTER_BYTES = 8192
 _CHUNK_WS: dict = {}            # (device, stream, bytes) -> workspace
 _CHUNK_WS_CAPTURE: dict = {}    # the same -> (capture id, workspace of that graph)
 
