@@ -639,7 +639,8 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
 }
 
 // ------------------------------------------------------------------- many parts' sum --
-// Of the tiles that are in more than kFan parts: a wave has 32 rows and 32 d, as one of their parts has them in its registers.
+// Of the tiles that are in more than kFan parts: a workgroup has 32 rows and 32 d, as their parts have them in a wave's
+// registers, each of its waves a quarter of the parts.
 template <int D, int R>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     constexpr int MB = D / 32;
@@ -648,22 +649,22 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     if (!find<R>(p, blockIdx.x, at, many)) return;
     const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
     const int hk = at.unit % p.Hkv, tile = tiles - 1 - at.unit / p.Hkv;
-    const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5;
-    const int piece = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = piece / MB, b = piece % MB;
+    const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5, quarter = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = blockIdx.y / MB, b = blockIdx.y % MB;
     const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1, wrow = row0 + 32 * wave;
     if (wrow > last_row) return;
     const int parts = (base + token_of(p, last_row) + at.S) / at.S;      // ceil(what the last row sees / S)
-    const int w0 = first_id<R>(p, at, tile, hk);
+    const int w0 = first_id<R>(p, at, tile, hk), per = (parts + 3) / 4, end = (quarter + 1) * per < parts ? (quarter + 1) * per : parts;
     float4_t sum[4] = {};
     float top = -INFINITY, l = 0.f;
     constexpr int kBatch = 4;                    // loads of a batch go out together
-    for (int u0 = 0; u0 < parts; u0 += kBatch) {
+    for (int u0 = quarter * per; u0 < end; u0 += kBatch) {
         float4_t o[kBatch][4];
         float2 st[kBatch];
         float most = top;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const uint8_t* slot = slot_of(p, w0, u0 + u < parts ? u0 + u : parts - 1) + wave * part_bytes(D);
+            const uint8_t* slot = slot_of(p, w0, u0 + u < end ? u0 + u : end - 1) + wave * part_bytes(D);
             st[u] = *reinterpret_cast<const float2*>(slot + 128 * D + 8 * lane);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[u][i] = *reinterpret_cast<const float4_t*>(slot + 1024 * (4 * b + i) + 16 * lane);
@@ -677,13 +678,47 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
         top = most;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            if (u0 + u >= parts) continue;
+            if (u0 + u >= end) continue;
             const float by = st[u].x == -INFINITY ? 0.f : exp2_of(st[u].x - top);
             l = fmaf(st[u].y, by, l);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[i][e] = fmaf(o[u][i][e], by, sum[i][e]);
+        }
+    }
+    // the quarters' sums meet in the first wave
+    __shared__ float4_t meet[3][4][64];
+    __shared__ float2 stat[3][64];
+    if (quarter) {
+        stat[quarter - 1][lane] = make_float2(top, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) meet[quarter - 1][i][lane] = sum[i];
+    }
+    __syncthreads();
+    if (quarter) return;
+    {
+        const float own = top;
+        float2 st[3];
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            st[u] = stat[u][lane];
+            top = fmaxf(top, st[u].x);
+        }
+        const float keep = own == -INFINITY ? 0.f : exp2_of(own - top);
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] *= keep;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            const float by = st[u].x == -INFINITY ? 0.f : exp2_of(st[u].x - top);
+            l = fmaf(st[u].y, by, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4_t o = meet[u][i][lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[i][e] = fmaf(o[e], by, sum[i][e]);
+            }
         }
     }
     l = sum2(l);
@@ -780,7 +815,7 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     hipLaunchKernelGGL(fn, grid, dim3(2 * kRows), static_cast<unsigned>(8 * tokens_of(D) * D + (D == 256 ? 2 * 32 * kRows : 0)), s, a);
     rc = check_launch("chunk_attention_kernel");
     if (rc != MCV_OK || most <= kFan * kLeast || !slots) return rc;
-    const dim3 joins(static_cast<unsigned>(std::min(tiles * Hkv, slots / kFan)), static_cast<unsigned>(ceil_div(ceil_div(std::min<int64_t>(kRows, T * group), 32) * D, 128)));
+    const dim3 joins(static_cast<unsigned>(std::min(tiles * Hkv, slots / kFan)), static_cast<unsigned>(ceil_div(std::min<int64_t>(kRows, T * group), 32) * D / 32));
     auto join = D == 64 ? chunk_join_kernel<64, kRows> : D == 128 ? chunk_join_kernel<128, kRows> : chunk_join_kernel<256, kRows>;
     hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
     return check_launch("chunk_join_kernel");
