@@ -9,6 +9,7 @@ namespace {
 
 constexpr int kTile = 64;                        // a part has whole ones of so many tokens
 constexpr int kLeast = 2 * kTile;                // tokens of a part, at least
+constexpr int kNearLog2 = 2;                     // 1 << kNearLog2 units side by side on one XCD
 constexpr int64_t kMaxLen = int64_t(1) << 30;    // tokens of one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's reference exponent m is a whole number, so that what it once stood for is brought to another by an exact product,
@@ -30,7 +31,7 @@ struct ChunkArgs {
     float scale_log2;                            // above zero: a score of -inf stays one
     float q_by;                                  // 1, -1 or 0: the scale's sign
     int slots_log2;                              // parts to cut for; -1: every tile of rows whole
-    int near_log2;                               // units side by side on one XCD
+    int least;                                   // tokens of a part, at least
     int64_t slot_bytes;
 };
 
@@ -127,7 +128,7 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
     auto part_of = [&](int64_t total) {
         if (p.slots_log2 < 0) return 0x40000000;
         const int64_t S = (((total - 1) >> p.slots_log2) + kTile) / kTile * kTile;
-        return static_cast<int>(S < kLeast ? kLeast : S < 0x40000000 ? S : 0x40000000);
+        return static_cast<int>(S < p.least ? p.least : S < 0x40000000 ? S : 0x40000000);
     };
     if (p.B == 1) {                              // (nothing to look for)
         at.s = seq_of(p, 0, as_scalar(p.lens), as_scalar(p.cu));
@@ -182,9 +183,9 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
 // The number of the unit that workgroup b takes. Workgroup b runs on XCD b % 8: runs of `near` units, which read the same K
 // and V, go to one XCD, whose L2 they share; every other round of eight runs goes to them in reverse, as the first of a
 // sequence read most.
-__device__ __forceinline__ int unit_of(const ChunkArgs& p, int b) {
-    const int x = b & 7, i = (b >> 3) & ((1 << p.near_log2) - 1), round = b >> (3 + p.near_log2);
-    return (((round << 3) + (round & 1 ? 7 - x : x)) << p.near_log2) + i;
+__device__ __forceinline__ int unit_of(int b) {
+    const int x = b & 7, i = (b >> 3) & ((1 << kNearLog2) - 1), round = b >> (3 + kNearLog2);
+    return (((round << 3) + (round & 1 ? 7 - x : x)) << kNearLog2) + i;
 }
 
 // Where part i of a tile lies in the workspace. `read`: reads_below of all tiles before it. Part i has the id w0 + i, w0
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         for (int i = whole + 1; i < parts; ++i) sum += tiles_with<R>(p, s, tiles, static_cast<int64_t>(i) * S);
         return sum * p.Hkv;
     };
-    if (!find<R>(p, unit_of(p, blockIdx.x), at, units)) return;
+    if (!find<R>(p, unit_of(blockIdx.x), at, units)) return;
     const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
     // Part by part; in one, `near` tiles of a cache head after another, those that read most first.
     int part, tile, hk;
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
                 ++part;
             }
         }
-        const int near = 1 << p.near_log2, first = i / (near * p.Hkv) * near, of = have - first < near ? have - first : near;
+        const int near = 1 << kNearLog2, first = i / (near * p.Hkv) * near, of = have - first < near ? have - first : near;
         i -= first * p.Hkv;
         hk = i / of;
         tile = tiles - 1 - first - (i - hk * of);
@@ -742,13 +743,20 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     }
 }
 
-// Units side by side on one XCD: of as many tiles as a sequence has on average.
-int choose_near_log2(int64_t tiles, int64_t B) { return 2; }
 // Rows of a workgroup, and tokens that it takes at a time.
 constexpr int kRows = 128;
 constexpr int tokens_of(int64_t D) { return D == 256 ? 32 : 64; }
 // Parts to cut for, of rows that read up to `most` tokens: what the chip holds at once.  -1: nothing to cut.
 int choose_slots_log2(int64_t most, int64_t D) { return most <= kLeast ? -1 : D == 64 ? 10 : 9; }
+// Tokens of a part, at least. Where there are tiles enough for the chip, a quarter of the longest sequence's: no tile is then in
+// more parts than the last of them joins, and no launch follows for those that are. Measured with a quarter and with kLeast, us:
+// 1100 new tokens, heads 8/2 of 256 (70 tiles) 31.2, 37.0; 2048 47.6, 54.1; 3000 70.0, 78.3; 16 x 32 over 1000, heads 32/8 of
+// 128 (128 tiles) 15.1, 18.8. Otherwise 300 over 800 (20 tiles) 30.0, 25.2; 16 x 32 over 2000 (32 tiles) 30.7, 22.6; 1000 over
+// 3000 (64 tiles) 61.2, 57.3.
+int choose_least(int64_t most, int64_t tiles) {
+    if (tiles < 40 || most > std::min<int64_t>(50 * tiles, 4096)) return kLeast;
+    return static_cast<int>(std::max<int64_t>(ceil_div(most, kFan * kTile) * kTile, kLeast));
+}
 int64_t slot_bytes_of(int64_t T, int64_t group, int64_t D) { return ceil_div(std::min<int64_t>(kRows, T * group), 32) * part_bytes(D); }
 int64_t split_bytes(int slots_log2, int64_t slot_bytes) { return slots_log2 < 0 ? 0 : kCounterBytes + 2 * ((int64_t(1) << slots_log2) + 2) * slot_bytes; }
 
@@ -797,7 +805,7 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     if (slots_log2 >= 0 && (!workspace || workspace_bytes < split_bytes(slots_log2, slot_bytes))) slots_log2 = -1;
     if (slots_log2 >= 0 && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", who);
-    const int near_log2 = choose_near_log2(tiles, B);
+    const int least = choose_least(most, tiles * Hkv);
     const int64_t slots = slots_log2 < 0 ? 0 : int64_t(1) << slots_log2;
     if (tiles * Hkv + slots > 0x7fffff00) return fail(MCV_ERR_SHAPE, "%s: too many rows B=%lld T=%lld Hq=%lld", who, (long long)B, (long long)T, (long long)Hq);
     const uint32_t page16 = static_cast<uint32_t>(page_size / 16);
@@ -808,13 +816,13 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
                       static_cast<int>(k_token), static_cast<int>(v_token), static_cast<int>(pages), static_cast<int>(page16), static_cast<int>(most),
                       static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
                       inverse(page16), inverse(group), scale == 0.0 ? 1.f : std::fabs(static_cast<float>(scale) * kLog2e), scale < 0.0 ? -1.f : scale == 0.0 ? 0.f : 1.f,
-                      slots_log2, near_log2, slot_bytes};
+                      slots_log2, least, slot_bytes};
     const auto s = static_cast<hipStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(ceil_div(tiles * Hkv + slots, 8 << near_log2) * (8 << near_log2)));
+    const dim3 grid(static_cast<unsigned>(ceil_div(tiles * Hkv + slots, 8 << kNearLog2) * (8 << kNearLog2)));
     auto fn = D == 64 ? chunk_attention_kernel<64, 4, tokens_of(64)> : D == 128 ? chunk_attention_kernel<128, 4, tokens_of(128)> : chunk_attention_kernel<256, 4, tokens_of(256)>;
     hipLaunchKernelGGL(fn, grid, dim3(2 * kRows), static_cast<unsigned>(8 * tokens_of(D) * D + (D == 256 ? 2 * 32 * kRows : 0)), s, a);
     rc = check_launch("chunk_attention_kernel");
-    if (rc != MCV_OK || most <= kFan * kLeast || !slots) return rc;
+    if (rc != MCV_OK || most <= kFan * least || !slots) return rc;
     const dim3 joins(static_cast<unsigned>(std::min(tiles * Hkv, slots / kFan)), static_cast<unsigned>(ceil_div(std::min<int64_t>(kRows, T * group), 32) * D / 32));
     auto join = D == 64 ? chunk_join_kernel<64, kRows> : D == 128 ? chunk_join_kernel<128, kRows> : chunk_join_kernel<256, kRows>;
     hipLaunchKernelGGL(join, joins, dim3(256), 0, s, a);
