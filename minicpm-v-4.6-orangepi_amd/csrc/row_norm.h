@@ -84,7 +84,28 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
         uint16_t xs[PER], gs[VEC ? 1 : PER];
         uint4 xv[NC], gv[NC];
         uint16_t as[ADD ? PER : 1];
-        uint4 av[ADD ? NC : 1];
+        if constexpr (ADD && VEC) {
+            // each element is loaded once, by the thread that stores its chunk: rows and sum may be one
+            __shared__ uint4 sums[256 * NC];
+            uint4 av[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int i = 8 * (t + 256 * c);
+                xv[c] = i < H ? *reinterpret_cast<const uint4*>(xr + i) : make_uint4(0, 0, 0, 0);
+                av[c] = i < H ? *reinterpret_cast<const uint4*>(ar + i) : make_uint4(0, 0, 0, 0);
+                gv[c] = i < H ? *reinterpret_cast<const uint4*>(gamma + i) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int i = 8 * (t + 256 * c);
+                xv[c] = add_chunk(xv[c], av[c]);
+                sums[t + 256 * c] = xv[c];
+                if (i < H) *reinterpret_cast<uint4*>(sr + i) = xv[c];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j) xs[j] = reinterpret_cast<const uint16_t*>(sums)[t + 256 * j];      // (zero past the row)
+        } else
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = t + 256 * j;
@@ -92,17 +113,16 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
             if constexpr (ADD) as[j] = i < H ? ar[i] : uint16_t(0);
             if constexpr (!VEC) gs[j] = i < H ? gamma[i] : uint16_t(0);
         }
-        if constexpr (VEC)
+        if constexpr (VEC && !ADD)
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int i = 8 * (t + 256 * c);
                 xv[c] = i < H ? *reinterpret_cast<const uint4*>(xr + i) : make_uint4(0, 0, 0, 0);
-                if constexpr (ADD) av[c] = i < H ? *reinterpret_cast<const uint4*>(ar + i) : make_uint4(0, 0, 0, 0);
                 gv[c] = i < H ? *reinterpret_cast<const uint4*>(gamma + i) : make_uint4(0, 0, 0, 0);
             }
         // x may be `normed` (or the sum's place): no load may be in flight when another thread stores
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if constexpr (ADD)
+        if constexpr (!(ADD && VEC)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (ADD && !VEC)
 #pragma unroll
             for (int j = 0; j < PER; ++j) xs[j] = add_f16(xs[j], as[j]);
         float ss = 0.f;
@@ -116,10 +136,6 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int i = 8 * (t + 256 * c);
-                if constexpr (ADD) {
-                    xv[c] = add_chunk(xv[c], av[c]);
-                    if (i < H) *reinterpret_cast<uint4*>(sr + i) = xv[c];
-                }
                 xv[c] = rms_chunk<QUANT>(xv[c], gv[c], rstd, m);          // now the normed chunk
                 if (i < H && nr) *reinterpret_cast<uint4*>(nr + i) = xv[c];
             }
