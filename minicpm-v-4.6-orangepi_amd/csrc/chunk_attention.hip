@@ -293,9 +293,8 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     constexpr int CR = KT / W;          // rows of K and of V that a wave copies
     constexpr int ROW = 2 * D;                   // bytes
     constexpr int KM = RC < 16 ? RC - 1 : 15;
-    constexpr int QL = D == 256 ? 2 : 0;         // of q's operands, those that lie in LDS: the registers are one or two short
-    constexpr int VA = D == 256 ? 0 : 3;         // operands of V read before the softmax, where there are registers
-    constexpr int kMfma = 0x008, kDsRead = 0x100, kAhead = 3;
+    constexpr int QL = D == 256 ? 3 : 0;         // of q's operands, those that lie in LDS: the registers are one or two short
+    constexpr int kAhead = 3;                    // operands on their way from LDS while a product runs
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // [2][K, V][KT][D]
     __shared__ int flag;
     constexpr int kThrough = 16;                 // accesses that all XCDs see
@@ -370,12 +369,13 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     const int first_row = wave * CR % 16;        // of its 16 rows
     int4_t k_from, v_from;                       // buffer descriptors
     uint32_t copy_to;
-    // Groups of 16 tokens that are not there, of the tile that is being taken and of the one that is on its way.
-    uint32_t gone = 0, gone_next = 0;
+    // Groups of 16 tokens that are not there, of the tile that is being taken, of the one that is on its way and
+    // of the one after it.
+    uint32_t gone = 0, gone_next = 0, gone_then = 0;
     auto aim = [&](int t, int buf) {
         copy_to = lds_at + buf * 2 * KT * ROW + wave * CR * ROW;
         const int g = (t - known) / 16, own = g + wave * CR / 16;
-        gone_next = static_cast<uint32_t>(__ballot(my_page < 0) >> g) & (KT == 64 ? 15u : 3u);
+        gone_then = static_cast<uint32_t>(__ballot(my_page < 0) >> g) & (KT == 64 ? 15u : 3u);
         const int page = __builtin_amdgcn_readlane(my_page, own), prow = __builtin_amdgcn_readlane(my_row, own);
         auto rows16 = [&](const uint16_t* base, int64_t page_stride, int token_stride) {
             const uint16_t* at = base + (page < 0 ? 0 : page) * page_stride + static_cast<int64_t>(prow) * token_stride;
@@ -384,10 +384,6 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         };
         k_from = rows16(kh, p.k_page, p.k_token);
         v_from = rows16(vh, p.v_page, p.v_token);
-        if (g == 64 - KT / 16) {
-            known += 1024;
-            page_of(p, table, known / 16 + lane, t_end, my_page, my_row);
-        }
     };
     const uint32_t lr = static_cast<uint32_t>(lane) / RC, lc = static_cast<uint32_t>(lane) % RC;
     const uint32_t k_row = 2 * lr * p.k_token, v_row = 2 * lr * p.v_token, k_chunk = 16 * (lc ^ (lr & KM)), v_chunk = 16 * (lc ^ turn_of_v(lr));
@@ -403,8 +399,10 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     };
     if (t_begin < t_end) {
         aim(t_begin, 0);
+        gone_next = gone_then;
 #pragma unroll
         for (int i = 0; i < 2 * CP; ++i) copy(i);
+        aim(t_begin + KT, 1);                    // (past the end: copies of nothing)
     }
     half8_t q[KS - QL], *const q_held = reinterpret_cast<half8_t*>(lds + 4 * KT * ROW) + threadIdx.x;
     if (mine) {
@@ -437,6 +435,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         uint8_t* const vl = lds + (2 * buf + 1) * KT * ROW;
         const uint32_t k_now = lds_at + buf * 2 * KT * ROW + k_at, v_now = lds_at + buf * 2 * KT * ROW + v_at;
         gone = gone_next;
+        gone_next = gone_then;
         if (t + KT > t_end || gone) {
             // what lies past the end or is not there may be NaN, whose product with a weight of zero is no zero
             for (int i = lane; i < CR * RC; i += 64) {
@@ -448,30 +447,33 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        aim(t + KT, buf ^ 1);                 // (past the end: copies of nothing)
+        if (t + 2 * KT - known >= 1024) {        // (before the copies: it is waited for)
+            known += 1024;
+            page_of(p, table, known / 16 + lane, t_end, my_page, my_row);
+        }
+        // (Copies and what aims the next ones go out before the products: between them they cost more than they hide, 8192 new
+        // tokens 307 us against 286.)
 #pragma unroll
         for (int i = 0; i < 2 * CP; ++i) copy(i);
+        aim(t + 2 * KT, buf);
         if (!mine || t >= most) continue;
         const bool all = t + KT <= least && gone == 0;
         // Scores of 32 tokens; the reference exponent of what follows, and its rare change; weights; their products
+        auto k_read = [&](int h, int x) {
+            return *reinterpret_cast<lds_half8>((k_now ^ (32 * x % (16 * (KM + 1)))) + 32 * h * ROW + 32 * x / (16 * (KM + 1)) * (16 * (KM + 1)));
+        };
         auto scores = [&](int h, float16_t& s) {
+            half8_t k[kAhead];
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x) k[x] = k_read(h, x);
             s = float16_t{};
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
-                const half8_t k = *reinterpret_cast<lds_half8>((k_now ^ (32 * x % (16 * (KM + 1)))) + 32 * h * ROW + 32 * x / (16 * (KM + 1)) * (16 * (KM + 1)));
                 const half8_t qx = x < KS - QL ? q[x < KS - QL ? x : 0] : q_held[(x - KS + QL) * 64 * W];
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qx, s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[x % kAhead], qx, s, 0, 0, 0);
+                if (x + kAhead < KS) k[x % kAhead] = k_read(h, x + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // reads run kAhead products ahead
-            __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
-#pragma unroll
-            for (int x = 0; x < KS - kAhead; ++x) {
-                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-                if (x + kAhead >= KS - QL) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
-            __builtin_amdgcn_sched_barrier(0);
         };
         auto refer = [&](int h, float16_t& s) {
             if (!all) {
@@ -519,29 +521,32 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             }
             return a;
         };
-        auto add = [&](int h, const half8_t (&w)[2], const half8_t (&first)[VA + 1]) {
-#pragma unroll
-            for (int y = 0; y < 2 * MB; ++y)
-                acc[y % MB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y < VA ? first[y < VA ? y : 0] : v_read(h, y), w[y / MB], acc[y % MB], 0, 0, 0);
-            if constexpr (VA == 0) __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * kAhead, 0);
-#pragma unroll
-            for (int y = 0; y < 2 * MB - kAhead; ++y) {
-                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+        auto add = [&](int h, const half8_t (&w)[2], half8_t (&v)[kAhead]) {
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 2 * MB; ++y) {
+                acc[y % MB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[y % kAhead], w[y / MB], acc[y % MB], 0, 0, 0);
+                if (y + kAhead < 2 * MB) v[y % kAhead] = v_read(h, y + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
 #pragma unroll
         for (int h = 0; h < KT / 32; ++h) {
             float16_t s;
-            half8_t w[2], first[VA + 1];
+            half8_t w[2], v[kAhead];
             scores(h, s);
+            auto v_first = [&]() {
 #pragma unroll
-            for (int y = 0; y < VA; ++y) first[y] = v_read(h, y);
+                for (int y = 0; y < kAhead; ++y) v[y] = v_read(h, y);
+            };
+            if (D < 256) v_first();              // (before the softmax where there are registers)
             refer(h, s);
             weigh(s, w);
-            add(h, w, first);
+            if (D == 256) {
+                __builtin_amdgcn_sched_barrier(0);
+                v_first();
+            }
+            add(h, w, v);
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -820,7 +825,7 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     const auto s = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(ceil_div(tiles * Hkv + slots, 8 << kNearLog2) * (8 << kNearLog2)));
     auto fn = D == 64 ? chunk_attention_kernel<64, 4, tokens_of(64)> : D == 128 ? chunk_attention_kernel<128, 4, tokens_of(128)> : chunk_attention_kernel<256, 4, tokens_of(256)>;
-    hipLaunchKernelGGL(fn, grid, dim3(2 * kRows), static_cast<unsigned>(8 * tokens_of(D) * D + (D == 256 ? 2 * 32 * kRows : 0)), s, a);
+    hipLaunchKernelGGL(fn, grid, dim3(2 * kRows), static_cast<unsigned>(8 * tokens_of(D) * D + (D == 256 ? 3 * 32 * kRows : 0)), s, a);
     rc = check_launch("chunk_attention_kernel");
     if (rc != MCV_OK || most <= kFan * least || !slots) return rc;
     const dim3 joins(static_cast<unsigned>(std::min(tiles * Hkv, slots / kFan)), static_cast<unsigned>(ceil_div(std::min<int64_t>(kRows, T * group), 32) * D / 32));
