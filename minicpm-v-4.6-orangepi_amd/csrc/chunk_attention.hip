@@ -429,6 +429,9 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     typedef uint32_t uint2_v __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) uint2_v* lds_uint2;
 
+    // Of a SIMD's two waves the one in the odd slot goes first: alike, they share the matrix cores and come to their softmaxes at
+    // one time. 9 prompts of 1 to 1501 tokens, heads 32/8 of 128: 81.6 us, 86.9 without; with heads of 256 within 3% either way.
+    if (D < 256 && (__builtin_amdgcn_s_getreg((3 << 11) | 4) & 1)) __builtin_amdgcn_s_setprio(2);
     int buf = 0;
     for (int t = t_begin; t < t_end; t += KT, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
