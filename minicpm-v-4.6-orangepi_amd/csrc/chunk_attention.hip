@@ -274,11 +274,9 @@ __device__ __forceinline__ void slow_row(const ChunkArgs& p, const Place& at, in
         if (E * lane + e >= d0 && E * lane + e < d1) out_row(p, at, hk, row, D)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
 }
 
-__device__ __forceinline__ uint2 halves(const float4_t& v, float by, bool none) {
-    uint16_t r[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) r[x] = f2h(none ? 0.f : v[x] * by);
-    return make_uint2(r[0] | (static_cast<uint32_t>(r[1]) << 16), r[2] | (static_cast<uint32_t>(r[3]) << 16));
+__device__ __forceinline__ uint2 halves(const float4_t& v, float by) {
+    const half2_t a = {static_cast<_Float16>(v[0] * by), static_cast<_Float16>(v[1] * by)}, b = {static_cast<_Float16>(v[2] * by), static_cast<_Float16>(v[3] * by)};
+    return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
 }
 
 // ---------------------------------------------------------------------- a part --
@@ -581,12 +579,24 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         const int others = (part ^ 2) & ~1, with[3] = {part ^ 1, others, others + 1};
         __amdgpu_buffer_rsrc_t from[3];
         float om[3], ol[3], by[3], top = m;
+        u2 st[3];
 #pragma unroll
         for (int x = 0; x < 3; ++x) {
             from[x] = slot(with[x]);
-            const auto st = __builtin_amdgcn_raw_buffer_load_b64(from[x], stat_at, 0, kThrough);
-            om[x] = with[x] < parts ? __uint_as_float(st[0]) : -INFINITY;
-            ol[x] = __uint_as_float(st[1]);
+            st[x] = __builtin_amdgcn_raw_buffer_load_b64(from[x], stat_at, 0, kThrough);
+        }
+        int4_t o[2][3][4];                       // a block's sums are on their way while those before are added
+        auto load = [&](int b) {
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[b % 2][x][i] = __builtin_amdgcn_raw_buffer_load_b128(from[x], mine_at + 1024 * (4 * b + i), 0, kThrough);
+        };
+        load(0);
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            om[x] = with[x] < parts ? __uint_as_float(st[x][0]) : -INFINITY;
+            ol[x] = __uint_as_float(st[x][1]);
             top = fmaxf(top, om[x]);
         }
 #pragma unroll
@@ -596,15 +606,13 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         l = (l * keep + ol[0] * by[0]) + (ol[1] * by[1] + ol[2] * by[2]);
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
-            int4_t o[3][4];
-#pragma unroll
-            for (int x = 0; x < 3; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[x][i] = __builtin_amdgcn_raw_buffer_load_b128(from[x], mine_at + 1024 * (4 * b + i), 0, kThrough);
+            if (b + 1 < MB) load(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const auto& now = o[b % 2];
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                acc[b][i] = (acc[b][i] * keep + __int_as_float(o[0][i / 4][i % 4]) * by[0]) +
-                            (__int_as_float(o[1][i / 4][i % 4]) * by[1] + __int_as_float(o[2][i / 4][i % 4]) * by[2]);
+                acc[b][i] = (acc[b][i] * keep + __int_as_float(now[0][i / 4][i % 4]) * by[0]) +
+                            (__int_as_float(now[1][i / 4][i % 4]) * by[1] + __int_as_float(now[2][i / 4][i % 4]) * by[2]);
         }
     }
     if (!mine) return;
@@ -619,25 +627,40 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     const unsigned long long odds = __ballot(none != 0.f);
     const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
     // Whole rows go out, turned in LDS, a wave in its own part of it: a row's 16-byte chunks in an order of its own, so that
-    // what a lane has of its row meets other banks. (A loop, not its body over and over: code that runs once is fetched from
-    // memory.)
+    // what a lane has of its row meets other banks; and each row's place in `out`, worked out once by the lanes that have it.
     {
-        constexpr int CH = D / 8, CM = CH < 16 ? CH - 1 : 15;
-        uint8_t* const turn = lds + wave * 64 * D;
+        constexpr int CH = D / 8, CM = CH < 16 ? CH - 1 : 15, N = CH / 2 < 8 ? CH / 2 : 8;       // N: stores of a lane in a go
+        typedef __attribute__((address_space(3))) uint64_t* lds_uint64;
+        typedef uint32_t uint4_v __attribute__((ext_vector_type(4)));
+        typedef const __attribute__((address_space(3))) uint4_v* lds_uint4;
         const float by = l > 0.f ? 1.0f / l : 0.f;
-        const uint32_t to = lds_at + wave * 64 * D + 16 * (c * CH + (c & CM)) + 8 * j;
+        const uint32_t mine_at = lds_at + wave * 64 * D, rows_at = lds_at + 64 * D * W + 256 * wave, to = mine_at + 16 * (c * CH + (c & CM)) + 8 * j;
+        *reinterpret_cast<lds_uint64>(rows_at + 8 * c) =
+            wrow + c < rows && !(bad >> c & 1) ? reinterpret_cast<uintptr_t>(p.out + (static_cast<int64_t>(at.s.first + token) * p.Hq + hk * p.group + row - token * p.group) * D) : 0;
 #pragma unroll
         for (int b = 0; b < MB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint2 h = halves(float4_t{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]}, by, l == 0.f);
+                const uint2 h = halves(float4_t{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]}, by);
                 *reinterpret_cast<lds_uint2>((to ^ (64 * (b % ((CM + 1) / 4)) + 16 * i)) + 16 * (CM + 1) * (b / ((CM + 1) / 4))) = uint2_v{h.x, h.y};
             }
+        const int r0 = lane / CH, ch = lane % CH;
 #pragma unroll 1
-        for (int i = lane; i < 32 * CH; i += 64) {
-            const int r = i / CH, ch = i % CH;
-            const uint4 v = *reinterpret_cast<const uint4*>(turn + 16 * (r * CH + (ch ^ (r & CM))));
-            if (wrow + r < rows && !(bad >> r & 1)) *reinterpret_cast<uint4*>(out_row(p, at, hk, wrow + r, D) + 8 * ch) = v;
+        for (int r = r0; r < 32; r += 64 / CH * N) {
+            uint64_t place[N];
+            uint4_v v[N];
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+                const int rx = r + 64 / CH * x;
+                place[x] = *reinterpret_cast<lds_uint64>(rows_at + 8 * rx);
+                v[x] = *reinterpret_cast<lds_uint4>(mine_at + 16 * (rx * CH + (ch ^ (rx & CM))));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < N; ++x) asm volatile("" : "+v"(v[x]), "+v"(place[x]));       // (read before the first is stored)
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+                if (place[x]) *reinterpret_cast<__attribute__((address_space(1))) uint4_v*>(place[x] + 16 * ch) = v[x];
         }
     }
 #pragma unroll 1
@@ -742,7 +765,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
         uint16_t* to = out_row(p, at, hk, wrow + c, D) + 32 * b + 4 * j;
         const float by = l > 0.f ? 1.0f / l : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(to + 8 * i) = halves(sum[i], by, l == 0.f);
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(to + 8 * i) = halves(sum[i], by);
     }
 #pragma unroll 1
     for (uint32_t left = bad; left; left &= left - 1) {
