@@ -1,6 +1,7 @@
 """A small decoder of linear-attention and full-attention layers on the framework's operators:
-W4A16 projections, RMSNorm, the gated delta rule, several-axis rotary positions with the
-write into a paged cache, one-token paged attention, and the greedy lm_head.
+W4A16 projections, RMSNorm with the residual row's addition, the gated delta rule, pages dealt
+out on the GPU, several-axis rotary positions with the write into a paged cache, attention of
+whole prompts and of single tokens over it, and the greedy lm_head.
 
     python examples/hybrid_decoder.py [--layers 8] [--tokens 32]
 
@@ -56,8 +57,10 @@ class Decoder:
         self.head = weight(rng, H, -(-VOCAB // 64) * 64)
         self.freq, self.axis = mcv.rotary_axes_table(ROT, 1e7, (11, 11, 10))
         self.B, width = sequences, -(-max_len // PAGE)
-        # one table for all layers, its pages dealt out in mixed order; every layer has its own caches and states
-        self.table = torch.from_numpy(rng.permutation(sequences * width).astype(np.int32)).cuda().view(sequences, width)
+        # one table and one stack of free pages for all layers; every layer has its own caches and states
+        self.table = torch.full((sequences, width), -1, dtype=torch.int32, device="cuda")
+        self.free = torch.from_numpy(rng.permutation(sequences * width).astype(np.int32)).cuda()
+        self.free_count = torch.tensor([sequences * width], dtype=torch.int32, device="cuda")
         self.caches, self.states = {}, {}
         for i, layer in enumerate(self.layers):
             if layer.full:
@@ -66,20 +69,23 @@ class Decoder:
                 self.states[i] = torch.zeros(sequences, HV, DL, DL, dtype=torch.float32, device="cuda")
         self.lens = torch.zeros(sequences, dtype=torch.int32, device="cuda")         # tokens each sequence holds
 
-    def run(self, tokens, positions, seq, at, cu):
-        """Hidden rows [T, H] of packed tokens: their sequence, place in it and positions [3, T].
+    def run(self, tokens, positions, cu):
+        """Normed rows [T, H] of packed tokens at positions [3, T], which the sequences get as their next ones.
         cu: where the sequences' tokens begin; None: one token for each sequence in order."""
         T = len(tokens)
+        slots, _, _ = mcv.paged_append(self.table, self.lens, cu, PAGE, tokens=T, free_pages=self.free, free_count=self.free_count)
         x = self.embedding[tokens]
-        slots = self.table[seq, at // PAGE].long() * PAGE + at % PAGE
-        rows_table, rows_len = (self.table, (at + 1).int()) if cu is None else (self.table[seq], (at + 1).int())
+        h = mcv.rms_norm(x, self.layers[0].norm, EPS)
         for i, layer in enumerate(self.layers):
-            qkv = mcv.matmul_w4a16(mcv.rms_norm(x, layer.norm, EPS), layer.qkv)
+            qkv = mcv.matmul_w4a16(h, layer.qkv)
             if layer.full:
                 q, k, v = (t.view(T, -1, DF) for t in qkv.split((HQ * DF, HKV * DF, HKV * DF), 1))
                 kc, vc = self.caches[i]
                 q = mcv.rotary_axes_cached(q, k, v, positions, self.freq, self.axis, kc, vc, slots)
-                y = mcv.paged_attention_decode(q, kc, vc, rows_table, rows_len)      # a prompt: each token a row of its own
+                if cu is None:
+                    y = mcv.paged_attention_decode(q, kc, vc, self.table, self.lens)
+                else:
+                    y = mcv.paged_attention_chunk(q, kc, vc, self.table, self.lens, cu)
             else:
                 qkv = torch.nn.functional.silu(qkv)
                 q, k, v = (t.view(T, -1, DL) for t in qkv.split((HK * DL, HK * DL, HV * DL), 1))
@@ -90,32 +96,27 @@ class Decoder:
                     y, _ = mcv.gated_delta_rule_step(q, k, v, g, beta, state, normalize=True)
                 else:
                     y, _ = mcv.gated_delta_rule(q, k, v, g, beta, state, cu_seqlens=cu, normalize=True, state_out=state)
-            x = x + mcv.matmul_w4a16(y.reshape(T, -1), layer.o)
-            h = mcv.rms_norm(x, layer.mlp_norm, EPS)
-            x = x + mcv.matmul_w4a16(mcv.mlp_gate_up_silu_w4a16(h, layer.gate, layer.up), layer.down)
-        return x
+            h, x = mcv.rms_norm_add(mcv.matmul_w4a16(y.reshape(T, -1), layer.o), x, layer.mlp_norm, EPS)
+            down = mcv.matmul_w4a16(mcv.mlp_gate_up_silu_w4a16(h, layer.gate, layer.up), layer.down)
+            h, x = mcv.rms_norm_add(down, x, self.layers[i + 1].norm if i + 1 < len(self.layers) else self.final_norm, EPS)
+        return h
 
-    def logits(self, x):
-        return mcv.matmul_w4a16(mcv.rms_norm(x, self.final_norm, EPS), self.head)[:, :VOCAB].contiguous()
+    def logits(self, h):
+        return mcv.matmul_w4a16(h, self.head)[:, :VOCAB].contiguous()
 
     def read(self, prompts, positions):
         """Whole prompts at once, from empty states and caches; the last rows' logits."""
         n = torch.tensor([len(p) for p in prompts])
         cu = torch.cat((torch.zeros(1, dtype=torch.int64), n.cumsum(0))).int().cuda()
-        seq = torch.repeat_interleave(torch.arange(self.B), n).cuda()
-        at = torch.cat([torch.arange(int(m)) for m in n]).cuda()
         for s in self.states.values():
             s.zero_()
-        self.lens.copy_(n)
-        x = self.run(torch.cat(prompts).cuda(), torch.cat(positions, 1).contiguous().cuda(), seq, at, cu)
-        return self.logits(x[cu[1:].long() - 1].contiguous())
+        mcv.paged_truncate(self.table, self.lens, None, PAGE, self.free, self.free_count)      # all pages back
+        h = self.run(torch.cat(prompts).cuda(), torch.cat(positions, 1).contiguous().cuda(), cu)
+        return self.logits(h[cu[1:].long() - 1].contiguous())
 
     def step(self, tokens, positions):
         """One more token for every sequence."""
-        at = self.lens.long()
-        x = self.run(tokens, positions, torch.arange(self.B, device="cuda"), at, None)
-        self.lens += 1
-        return self.logits(x)
+        return self.logits(self.run(tokens, positions, None))
 
 
 def text(n, start=0):
