@@ -93,14 +93,15 @@ int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
  *   cu_seqlens  int32 [B + 1], values clamped to [0, T]; rows of no sequence are left
  *           as they are.  NULL: T / B rows each (T % B == 0)
  * A row that sees nothing (seq_lens[b] < n, or its pages are not there) gives zeros.  An
- * infinity or NaN reaches the rows that see its token and no others.  The softmax is in 32
- * bits; its weights are rounded to fp16, which leaves those below 2^-39 of a row's
- * largest out.
- * Where the rows are few the cache is split over workgroups, whose parts a second
- * launch joins in order (deterministic): workspace of
- * mcv_paged_attention_chunk_workspace_bytes bytes, 256-byte aligned, of any content,
- * that no other call uses between the two launches (NULL or too small: no split).  The
- * bytes for a T and a max_seq_len are enough for any smaller ones. */
+ * infinity or NaN reaches the rows that see its token and no others; such rows are made
+ * token by token, some hundred times slower.  The softmax is in 32 bits; its weights are
+ * rounded to fp16, which leaves those below 2^-33 of a row's largest out.
+ * Where the rows are few the cache is split over workgroups, whose parts meet in an order
+ * that does not depend on who is last (deterministic): workspace of
+ * mcv_paged_attention_chunk_workspace_bytes bytes, 256-byte aligned, whose first 8 KiB are
+ * zero before its first use, and again after every call (NULL or too small: no split).
+ * One call at a time may use it.  The bytes for a T and a max_seq_len are enough for any
+ * smaller ones, and 144 MiB for all. */
 int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
                               int64_t k_token, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_token,
                               int64_t v_head, int64_t pages, int64_t page_size, const void* block_table,

@@ -777,8 +777,9 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
 // Rows of a workgroup, and tokens that it takes at a time.
 constexpr int kRows = 128;
 constexpr int tokens_of(int64_t D) { return D == 256 ? 32 : 64; }
-// Parts to cut for, of rows that read up to `most` tokens: what the chip holds at once.  -1: nothing to cut.
-int choose_slots_log2(int64_t most, int64_t D) { return most <= kLeast ? -1 : D == 64 ? 10 : 9; }
+// Parts to cut for, of rows that read up to `most` tokens: what the chip holds at once.  -1: nothing to cut. (Two parts of 128
+// tokens are joined in more time than they save: 200 new tokens, heads 8/2 of 256, 16.5 us in one, 18.4 in two.)
+int choose_slots_log2(int64_t most, int64_t D) { return most <= 2 * kLeast ? -1 : D == 64 ? 10 : 9; }
 // Tokens of a part, at least. Where there are tiles enough for the chip, a quarter of the longest sequence's: no tile is then in
 // more parts than the last of them joins, and no launch follows for those that are. Measured with a quarter and with kLeast, us:
 // 1100 new tokens, heads 8/2 of 256 (70 tiles) 31.2, 37.0; 2048 47.6, 54.1; 3000 70.0, 78.3; 16 x 32 over 1000, heads 32/8 of
