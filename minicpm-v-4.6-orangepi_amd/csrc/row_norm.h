@@ -64,7 +64,10 @@ struct AddRows {
 // 256 * 32, strided loops, each with only the loads and stores it needs (with the
 // store conditional inside: M=1 H=16384 27.8 us, now 26.3, as before PER).
 // ADD: the row is fp16(x + other), which goes to `sum` too; normed and int8 are what
-// they are for a row that holds it.
+// they are for a row that holds it.  VEC then loads every element once, as chunks, and
+// thread t finds the elements t, t + 256, ... of the sum in LDS: bound by HBM from some
+// 1000 rows on.  M=8192 H=1024 12.3 us (5.4 TB/s; each element twice, as without ADD:
+// 19.2), M=1024 H=8192 11.3 (5.9 TB/s), M=1100 H=3592 to int8 9.8 (17), M=1 H=1024 2.0.
 template <int PER, bool VEC, bool QUANT, bool ADD = false>
 __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ gamma,
                                                       int H, float eps, uint16_t* __restrict__ normed,
@@ -203,6 +206,60 @@ __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict
     }
 }
 
+// The sum's norm of rows of up to 256: a wave a row, four to a workgroup, with the sums of rms_row_kernel's four waves one after
+// another in one, and no barrier.  M=16384 H=200
+// 10.4 us, 15.0 with a workgroup a row; M=8192 H=64 4.5 / 6.2.  (Beyond 256 the chunks' loads are wider than a wave's.)
+template <bool QUANT>
+__global__ __launch_bounds__(256) void rms_add_short_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ gamma, int M, int H,
+                                                            float eps, uint16_t* __restrict__ normed, int8_t* __restrict__ xq,
+                                                            float* __restrict__ s32, uint16_t* __restrict__ s16, AddRows add) {
+    const int row = 4 * blockIdx.x + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= M) return;
+    const uint16_t* xr = x + row * add.x_row;
+    const uint16_t* ar = add.other + row * add.other_row;
+    uint16_t* sr = add.sum + row * add.sum_row;
+    uint16_t xs[4], as[4], gs[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int i = lane + 64 * w;
+        xs[w] = i < H ? xr[i] : uint16_t(0);
+        as[w] = i < H ? ar[i] : uint16_t(0);
+        gs[w] = i < H ? gamma[i] : uint16_t(0);
+    }
+    float tot = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int i = lane + 64 * w;
+        xs[w] = add_f16(xs[w], as[w]);
+        if (i < H) sr[i] = xs[w];
+        const float v = h2f(xs[w]);                      // zero past the row
+        tot += wave_butterfly(fmaf(v, v, 0.f), [](float p, float q) { return p + q; });
+    }
+    const float rstd = rms_rstd(tot, H, eps);
+    float m = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int i = lane + 64 * w;
+        xs[w] = rms_apply(xs[w], rstd, gs[w]);
+        if (i < H && normed) normed[static_cast<int64_t>(row) * H + i] = xs[w];
+        const float v = i < H ? fabsf(h2f(xs[w])) : 0.f;
+        m = v > m ? v : m;
+    }
+    if constexpr (QUANT) {
+        m = wave_butterfly(m, [](float p, float q) { return q > p ? q : p; });
+        const float scale = act_scale(m), inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int i = lane + 64 * w;
+            if (i < H) xq[static_cast<int64_t>(row) * H + i] = act_quant(xs[w], inv);
+        }
+        if (lane == 0) {
+            if (s32) s32[row] = scale;
+            if (s16) s16[row] = f2h(scale);
+        }
+    }
+}
+
 using RmsFn = void (*)(const uint16_t*, const uint16_t*, int, float, uint16_t*, int8_t*, float*, uint16_t*, AddRows);
 
 // Launches the kernel for M rows of H; VEC needs whole 16-byte chunks: H a
@@ -219,6 +276,12 @@ void launch_rms(const uint16_t* x, const uint16_t* gamma, int64_t M, int64_t H, 
                          static_cast<uintptr_t>(2 * (add.x_row | add.other_row | add.sum_row));
     const bool vec = H % 8 == 0 && at % 16 == 0;
     const int h = static_cast<int>(H);
+    if constexpr (ADD)
+        if (H <= 256) {
+            hipLaunchKernelGGL(rms_add_short_kernel<QUANT>, dim3(static_cast<unsigned>(ceil_div(M, 4))), dim3(256), 0, stream, x, gamma, static_cast<int>(M), h, eps,
+                               normed, xq, s32, s16, add);
+            return;
+        }
     RmsFn fn = rms_row_kernel<0, false, QUANT, ADD>;
     if (H <= 256) fn = rms_row_kernel<1, false, QUANT, ADD>;
     else if (H <= 1024) fn = vec ? rms_row_kernel<4, true, QUANT, ADD> : rms_row_kernel<4, false, QUANT, ADD>;
