@@ -1,4 +1,37 @@
 // chunk_attention.hip -- attention of chunks of new tokens over a paged cache, gfx950.
+//
+//   out[row][h] = sum_t w_t V[t] / sum_t w_t,  w_t = exp(scale q[row][h] . K[t] - max),  t up to the row's own place
+//
+// Rows and heads. The heads of a group read the same K and V: a sequence's (token, head) pairs of one cache head, token by
+// token, are the rows of one matrix, of which a workgroup has a tile of 128, a wave 32. So 8 heads over 2 and 32 over 8 fill
+// the matrix cores from 8 or 32 tokens on, and one token's heads share one read of the cache.
+//
+// A wave's step, 32 tokens: S^T = K q^T on 32x32x16 matrix instructions, q in registers from the start, K from LDS; a lane then
+// has 16 scores of one row, so that a row's maximum and sum are in two lanes and the weights, rounded, are where the second
+// product wants them: out^T += V^T w^T, V read from LDS transposed. Weights are fp16, the operand type of the matrix cores:
+// half a step of 2^-11 each, and the sum that divides them is of the rounded ones. Scores, maxima and sums are in 32 bits. The
+// reference that weights are taken against moves only when a score passes it by 2^6, a whole power of two: few rows ever scale
+// what they have.
+//
+// K and V come to LDS by copies that pass no register, 32 tokens (heads of 256) or 64 at a time, in two buffers: the next
+// tile's are on their way while one is taken. Rows of LDS have their chunks in orders of their own, so that no read meets
+// another's bank (counted: none). Operands of the products are read three ahead.
+//
+// Parts. All reads of a call are cut evenly, on the device and from the lengths alone, into as many parts as workgroups that
+// the chip holds at once (two a CU); a unit is a tile's part. Up to four parts are joined by the last of them to arrive, more
+// by a launch that follows. Partial sums are 128 KiB a tile of 128 rows of 256, what 128 tokens of cache are: no part is
+// smaller than that.
+//
+// What bounds it, heads 8/2 of 256. 8192 new tokens 286 to 303 us by the card's clock, 0.91 to 0.96 PFLOP/s (a large matrix
+// product 1.14 to 1.31): the matrix cores are busy in 51% of cycles, LDS in 28%, and the clock falls to 1.7 GHz; what is left
+// is the softmax between the products, which two waves a SIMD hide by half. 512 over 100000 415 to 450 us, the same. 32
+// sequences' 5 over up to 9000 46.5 us, 3.1 TB/s: 33 of them at the cache's 145 MB, then the join. Small calls are latencies:
+// 24 over 1100 16.1 us, 1100 over none 27.6: the lengths, the table and the first tile, three loads that wait for one another,
+// 4 us; 1.3 us a step of 32 tokens; a part written and read 2 and 4 us.
+//
+// Tried and not better: 64 rows a wave (halves what LDS reads; registers spill), two waves on the same rows, 64 tokens of 256 at
+// a time with one workgroup a CU (8192: 394 us), eight waves with one workgroup a CU (325), copies spread over the products
+// (307), longest parts first (303), four reads ahead (the same), workgroups of the join over several tiles (the same).
 #include <algorithm>
 #include <cmath>
 
@@ -13,7 +46,8 @@ constexpr int kNearLog2 = 2;                     // 1 << kNearLog2 units side by
 constexpr int64_t kMaxLen = int64_t(1) << 30;    // tokens of one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's reference exponent m is a whole number, so that what it once stood for is brought to another by an exact product,
-// and is raised only when a score passes it by kRoom: the weights 2^(s - m + kTop) end below fp16's 65504.
+// and is raised only when a score passes it by kRoom: the weights 2^(s - m + kTop) end at 2^15, below fp16's 65504, and the
+// row's largest begins above 2^8: those that are lost, below 2^-25, are less than 2^-33 of it.
 constexpr float kRoom = 6.f, kTop = 9.f;
 
 struct ChunkArgs {
@@ -34,7 +68,6 @@ struct ChunkArgs {
     int least;                                   // tokens of a part, at least
     int64_t slot_bytes;
 };
-
 
 constexpr int kFan = 4;                          // parts of a tile that the last of them to arrive joins; where there are more, a launch of its own does
 constexpr int64_t kCounterBytes = 8192;          // a counter for each part
@@ -182,7 +215,7 @@ __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Coun
 
 // The number of the unit that workgroup b takes. Workgroup b runs on XCD b % 8: runs of `near` units, which read the same K
 // and V, go to one XCD, whose L2 they share; every other round of eight runs goes to them in reverse, as the first of a
-// sequence read most.
+// sequence read most. Runs of four against single units, 8192 new tokens 300, 310 us (mixed lengths of 128 86.9, 85.4).
 __device__ __forceinline__ int unit_of(int b) {
     const int x = b & 7, i = (b >> 3) & ((1 << kNearLog2) - 1), round = b >> (3 + kNearLog2);
     return (((round << 3) + (round & 1 ? 7 - x : x)) << kNearLog2) + i;
@@ -288,7 +321,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     constexpr int MB = D / 32;                   // blocks of 32 d
     constexpr int RC = D / 8;                    // 16-byte chunks of a row
     constexpr int RPI = 64 / RC;                 // rows that a copy takes
-    constexpr int CR = KT / W;          // rows of K and of V that a wave copies
+    constexpr int CR = KT / W;                   // rows of K and of V that a wave copies
     constexpr int ROW = 2 * D;                   // bytes
     constexpr int KM = RC < 16 ? RC - 1 : 15;
     constexpr int QL = D == 256 ? 3 : 0;         // of q's operands, those that lie in LDS: the registers are one or two short
@@ -672,7 +705,8 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
 
 // ------------------------------------------------------------------- many parts' sum --
 // Of the tiles that are in more than kFan parts: a workgroup has 32 rows and 32 d, as their parts have them in a wave's
-// registers, each of its waves a quarter of the parts.
+// registers, each of its waves a quarter of the parts. Bound by the partial sums' bytes and by its own start: 4.3 us for 24 new
+// tokens over 1100 (2.4 MB), 17 for 512 over 100000 (67 MB, 4 TB/s), 5 where it finds nothing to do.
 template <int D, int R>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     constexpr int MB = D / 32;
