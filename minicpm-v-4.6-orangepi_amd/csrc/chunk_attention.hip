@@ -30,8 +30,9 @@
 // 4 us; 1.3 us a step of 32 tokens; a part written and read 2 and 4 us.
 //
 // Tried and not better: 64 rows a wave (halves what LDS reads; registers spill), two waves on the same rows, 64 tokens of 256 at
-// a time with one workgroup a CU (8192: 394 us), eight waves with one workgroup a CU (325), copies spread over the products
-// (307), longest parts first (303), four reads ahead (the same), workgroups of the join over several tiles (the same).
+// a time with one workgroup a CU (8192: 394 us), 256 rows and one workgroup a CU (1% better here, 10% worse for mixed lengths), copies spread over the products
+// (307), longest parts first (303), four reads ahead (the same), the tile after the next fetched into L2 (321), workgroups of the
+// join over several tiles (the same).
 #include <algorithm>
 #include <cmath>
 
@@ -382,9 +383,17 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     const int32_t* table = p.table + at.b * p.table_row;
     const uint16_t* kh = p.k + hk * p.k_head;
     const uint16_t* vh = p.v + hk * p.v_head;
-    // A lane holds that of one of the 64 groups of 16 tokens from token `known` on.
-    int my_page = -1, my_row = 0, known = t_begin;
-    page_of(p, table, known / 16 + lane, t_end, my_page, my_row);
+    // A lane holds where K and V of one of the 64 groups of 16 tokens from token `known` on begin; above all addresses: nowhere.
+    uint64_t my_k, my_v;
+    int known = t_begin;
+    auto know = [&]() {
+        int page, row;
+        page_of(p, table, known / 16 + lane, t_end, page, row);
+        const uint64_t none = page < 0 ? uint64_t(1) << 63 : 0;
+        my_k = reinterpret_cast<uintptr_t>(kh + (page < 0 ? 0 : page) * p.k_page + static_cast<int64_t>(row) * p.k_token) | none;
+        my_v = reinterpret_cast<uintptr_t>(vh + (page < 0 ? 0 : page) * p.v_page + static_cast<int64_t>(row) * p.v_token) | none;
+    };
+    know();
     half8_t all[KS];
     if (mine) {
         const uint16_t* qr = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head;
@@ -406,15 +415,13 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     auto aim = [&](int t, int buf) {
         copy_to = lds_at + buf * 2 * KT * ROW + wave * CR * ROW;
         const int g = (t - known) / 16, own = g + wave * CR / 16;
-        gone_then = static_cast<uint32_t>(__ballot(my_page < 0) >> g) & (KT == 64 ? 15u : 3u);
-        const int page = __builtin_amdgcn_readlane(my_page, own), prow = __builtin_amdgcn_readlane(my_row, own);
-        auto rows16 = [&](const uint16_t* base, int64_t page_stride, int token_stride) {
-            const uint16_t* at = base + (page < 0 ? 0 : page) * page_stride + static_cast<int64_t>(prow) * token_stride;
-            const uintptr_t a = reinterpret_cast<uintptr_t>(at);
-            return int4_t{static_cast<int>(a), static_cast<int>(a >> 32 & 0xffff), page < 0 ? 0 : 2 * (15 * token_stride + D), 0x00020000};
+        gone_then = static_cast<uint32_t>(__ballot(static_cast<int64_t>(my_k) < 0) >> g) & (KT == 64 ? 15u : 3u);
+        auto rows16 = [&](uint64_t at, int token_stride) {
+            const int lo = __builtin_amdgcn_readlane(static_cast<int>(at), own), hi = __builtin_amdgcn_readlane(static_cast<int>(at >> 32), own);
+            return int4_t{lo, hi & 0xffff, hi < 0 ? 0 : 2 * (15 * token_stride + D), 0x00020000};
         };
-        k_from = rows16(kh, p.k_page, p.k_token);
-        v_from = rows16(vh, p.v_page, p.v_token);
+        k_from = rows16(my_k, p.k_token);
+        v_from = rows16(my_v, p.v_token);
     };
     const uint32_t lr = static_cast<uint32_t>(lane) / RC, lc = static_cast<uint32_t>(lane) % RC;
     const uint32_t k_row = 2 * lr * p.k_token, v_row = 2 * lr * p.v_token, k_chunk = 16 * (lc ^ (lr & KM)), v_chunk = 16 * (lc ^ turn_of_v(lr));
@@ -483,7 +490,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         __builtin_amdgcn_sched_barrier(0);
         if (t + 2 * KT - known >= 1024) {        // (before the copies: it is waited for)
             known += 1024;
-            page_of(p, table, known / 16 + lane, t_end, my_page, my_row);
+            know();
         }
         // (Copies and what aims the next ones go out before the products: between them they cost more than they hide, 8192 new
         // tokens 307 us against 286.)
