@@ -90,8 +90,9 @@ int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
  *   out[row][h] = sum_t softmax_t(scale q[row][h] . K[t][h / (Hq / Hkv)]) V[t][..]
  *   q, out  fp16 [T][Hq][D] (q: row and head strides; out contiguous)
  *   caches, block_table, seq_lens, max_seq_len  as for mcv_paged_attention
- *   cu_seqlens  int32 [B + 1], values clamped to [0, T]; rows of no sequence are left
- *           as they are.  NULL: T / B rows each (T % B == 0)
+ *   cu_seqlens  int32 [B + 1], ascending (else no row is written), values clamped to
+ *           [0, T]; rows of no sequence are left as they are.  NULL: T / B rows each
+ *           (T % B == 0)
  * A row that sees nothing (seq_lens[b] < n, or its pages are not there) gives zeros.  An
  * infinity or NaN reaches the rows that see its token and no others; such rows are made
  * token by token, some hundred times slower.  The softmax is in 32 bits; its weights are

@@ -92,19 +92,19 @@ __device__ __forceinline__ scalar_ints as_scalar(const int32_t* p) { return (sca
 
 // ---------------------------------------------------------------- who does what --
 struct Seq {
-    int first, n, len;                           // first new row, new tokens, tokens in the cache
+    int first, n, len;                           // first new row, new tokens (below zero: cu_seqlens falls), tokens in the cache
 };
 template <class Ints>
 __device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b, Ints lens, Ints cu) {
-    if (b >= p.B) return {0, 0, 0};
+    const int at = b < p.B ? b : p.B - 1;        // (no branch: several are loaded at once)
     int first, next;
-    const int held = lens[b];
-    if (cu) first = cu[b], next = cu[b + 1];
-    else first = b * (p.T / p.B), next = first + p.T / p.B;
+    const int held = lens[at];
+    if (cu) first = cu[at], next = cu[at + 1];
+    else first = at * (p.T / p.B), next = first + p.T / p.B;
     auto inside = [](int v, int most) { return v < 0 ? 0 : v > most ? most : v; };
     first = inside(first, p.T);
     next = inside(next, p.T);
-    return {first, next > first ? next - first : 0, inside(held, p.max_len)};
+    return {first, b < p.B ? next - first : 0, inside(held, p.max_len)};
 }
 __device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b) { return seq_of(p, b, p.lens, p.cu); }
 __device__ __forceinline__ int token_of(const ChunkArgs& p, int row) {         // row / group
@@ -116,7 +116,7 @@ __device__ __forceinline__ int token_of(const ChunkArgs& p, int row) {         /
 // R: rows of a tile.
 template <int R>
 __device__ __forceinline__ int tiles_of(const ChunkArgs& p, const Seq& s) {
-    return static_cast<int>((static_cast<int64_t>(s.n) * p.group + R - 1) / R);
+    return s.n < 0 ? 0 : static_cast<int>((static_cast<int64_t>(s.n) * p.group + R - 1) / R);
 }
 // Tokens that the first i tiles of rows read, at most (of one cache head).
 template <int R>
@@ -150,7 +150,10 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
     return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-// The sequence that has this kernel's unit `me`, where sequence s has count(s, S) of them.
+// The sequence that has this kernel's unit `me`, where sequence s has count(s, S) of them. A lane has a sequence, or, where
+// there are more than 64, a thread of the workgroup several, which then meet in LDS (4096 sequences' tokens over 200 each, heads
+// 8/2 of 256: 520 us, 933 with a wave's lanes alone). False in every thread: there is no such unit. Nor is there any where
+// cu_seqlens falls: rows would have two sequences, and more units than workgroups.
 struct Place {
     Seq s;
     int b, unit;                                 // the unit's number in it
@@ -158,59 +161,107 @@ struct Place {
     int S;                                       // tokens of a part
 };
 template <int R, class Count>
-__device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Count count) {
+__device__ __forceinline__ bool search(const ChunkArgs& p, int me, Place& at, Count count) {
     auto part_of = [&](int64_t total) {
         if (p.slots_log2 < 0) return 0x40000000;
         const int64_t S = (((total - 1) >> p.slots_log2) + kTile) / kTile * kTile;
         return static_cast<int>(S < p.least ? p.least : S < 0x40000000 ? S : 0x40000000);
     };
+    auto reads = [&](const Seq& s) { return p.Hkv * reads_below<R>(p, s, tiles_of<R>(p, s)); };
+    at.read = 0;
+    at.b = 0;
     if (p.B == 1) {                              // (nothing to look for)
         at.s = seq_of(p, 0, as_scalar(p.lens), as_scalar(p.cu));
-        at.b = 0;
         at.unit = me;
-        at.read = 0;
-        at.S = part_of(p.Hkv * reads_below<R>(p, at.s, tiles_of<R>(p, at.s)));
+        at.S = part_of(reads(at.s));
         return me < count(at.s, at.S);
     }
-    const int lane = threadIdx.x & 63, span = (p.B + 63) / 64;
-    Seq s = seq_of(p, lane);                     // (of span 1)
-    auto reads = [&](const Seq& s) { return p.Hkv * reads_below<R>(p, s, tiles_of<R>(p, s)); };
-    int64_t read = 0;
-    if (span == 1) read = reads(s);
-    else
-        for (int i = 0; i < span; ++i) read += reads(seq_of(p, lane * span + i));
-    int64_t read_upto = wave_scan(read);
-    at.S = part_of(lane_of(read_upto, 63));
-    int units = 0;
-    if (span == 1) units = count(s, at.S);
-    else
-        for (int i = 0; i < span; ++i) units += count(seq_of(p, lane * span + i), at.S);
-    int upto = wave_scan(units);
-    unsigned long long past = __ballot(upto > me);
-    if (!past) return false;
-    int l = __builtin_ctzll(past), before = 0;
-    at.read = 0;
-    auto go_to = [&]() {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    // of the 64 sequences from at.b on, whose units begin at `before`; false: it is none of theirs
+    auto look = [&](const Seq& s, int upto, int64_t read_upto) {
+        const unsigned long long past = __ballot(before + upto > me);
+        const int l = past ? __builtin_ctzll(past) : 64;
         if (l) {
             before += __builtin_amdgcn_readlane(upto, l - 1);
             at.read += lane_of(read_upto, l - 1);
         }
-    };
-    go_to();
-    at.b = l * span;
-    while (span > 1) {                           // the chosen lane's sequences, 64 at a time
-        s = seq_of(p, at.b + lane);
-        upto = wave_scan(count(s, at.S));
-        read_upto = wave_scan(reads(s));
-        past = __ballot(before + upto > me);
-        l = past ? __builtin_ctzll(past) : 64;
-        go_to();
         at.b += l;
-        if (past) break;
-        if (at.b >= p.B) return false;           // (lengths that changed meanwhile)
+        if (!past) return false;
+        at.s = {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l)};
+        at.unit = me - before;
+        return true;
+    };
+    if (p.B <= 64) {
+        const Seq s = seq_of(p, lane);
+        if (__any(s.n < 0)) return false;
+        const int64_t read_upto = wave_scan(reads(s));
+        at.S = part_of(lane_of(read_upto, 63));
+        return look(s, wave_scan(count(s, at.S)), read_upto);
     }
-    at.s = {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l)};
-    at.unit = me - before;
+    constexpr int kWaves = 4;
+    __shared__ int64_t wave_reads[kWaves];
+    __shared__ int wave_units[kWaves], falls[kWaves], owner[2];
+    __shared__ int64_t owner_read;
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), span = (p.B + 64 * kWaves - 1) / (64 * kWaves);
+    int64_t read = 0;
+    bool fall = false;
+#pragma unroll 1
+    for (int i = 0; i < span; ++i) {
+        const Seq s = seq_of(p, t * span + i);
+        read += reads(s);
+        fall |= s.n < 0;
+    }
+    const int64_t read_upto = wave_scan(read);
+    const bool falling = __any(fall);
+    if (lane == 63) wave_reads[wave] = read_upto, falls[wave] = falling;
+    __syncthreads();
+    int64_t total = 0;
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += wave_reads[w], any |= falls[w];
+    at.S = part_of(lane_of(total, 0));
+    int units = 0;
+#pragma unroll 1
+    for (int i = 0; i < span; ++i) units += count(seq_of(p, t * span + i), at.S);
+    const int upto = wave_scan(units);
+    if (lane == 63) wave_units[wave] = upto;
+    __syncthreads();
+    int w = 0;                                   // the wave that has it
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) {
+        const int its = __builtin_amdgcn_readfirstlane(wave_units[x]);
+        if (w == x && before + its <= me) {
+            before += its;
+            at.read += lane_of(wave_reads[x], 0);
+            ++w;
+        }
+    }
+    if (__builtin_amdgcn_readfirstlane(any) || w == kWaves) return false;
+    if (w == wave) {
+        const int l = __builtin_ctzll(__ballot(before + upto > me));
+        const int its = l ? __builtin_amdgcn_readlane(upto, l - 1) : 0;
+        const int64_t below = l ? lane_of(read_upto, l - 1) : 0;
+        owner[0] = (64 * w + l) * span;
+        owner[1] = before + its;
+        owner_read = at.read + below;
+    }
+    __syncthreads();
+    at.b = __builtin_amdgcn_readfirstlane(owner[0]);
+    before = __builtin_amdgcn_readfirstlane(owner[1]);
+    at.read = lane_of(owner_read, 0);
+    while (at.b < p.B) {                         // the chosen thread's sequences, 64 at a time
+        const Seq s = seq_of(p, at.b + lane);
+        if (look(s, wave_scan(count(s, at.S)), wave_scan(reads(s)))) return true;
+    }
+    return false;                                // (lengths that changed meanwhile)
+}
+
+template <int R, class Count>
+__device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Count count) {
+    if (!__builtin_amdgcn_readfirstlane(search<R>(p, me, at, count))) return false;
+    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    at = {{one(at.s.first), one(at.s.n), one(at.s.len)}, one(at.b), one(at.unit), lane_of(at.read, 0), one(at.S)};
     return true;
 }
 
@@ -366,6 +417,9 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         hk = i / of;
         tile = tiles - 1 - first - (i - hk * of);
     }
+    part = __builtin_amdgcn_readfirstlane(part);         // (the same in all lanes, which the compiler does not see)
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    hk = __builtin_amdgcn_readfirstlane(hk);
     const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1;
     auto seen_by = [&](int row) {                // tokens that a row sees
         const int n = base + token_of(p, row) + 1;

@@ -134,6 +134,38 @@ def test_its_counters_end_at_zero(mcv, cuda):
     assert held and all((ws[:mcv.mixers._CHUNK_COUNTER_BYTES] == 0).all() for ws in held)
 
 
+@pytest.mark.parametrize("B", [1, 3, 64, 65, 700])
+def test_offsets_that_fall(mcv, cuda, B):
+    """Rows would have two sequences: none is written, and the next call finds the workspace as it was."""
+    torch = _torch()
+    a = _several(cuda)[2]
+    want = mcv.paged_attention_chunk(*a)
+    T = len(a[0])
+    cu = torch.linspace(0, T, B + 1, device=cuda).int()
+    cu[B // 2:] = cu[B // 2:].flip(0)
+    table, lens = a[3].expand(B, -1).contiguous(), a[4].expand(B).contiguous()
+    out = torch.full_like(a[0], LEFT)
+    mcv.paged_attention_chunk(*a[:3], table, lens, cu, out=out)
+    assert (out == LEFT).all()
+    assert (mcv.paged_attention_chunk(*a) == want).all()
+    torch.cuda.synchronize()
+    assert all((ws[:mcv.mixers._CHUNK_COUNTER_BYTES] == 0).all() for ws in mcv.mixers._CHUNK_WS.values())
+
+
+def test_more_sequences_than_threads(mcv, cuda):
+    """1500 sequences, some without new tokens, some with one and a few with many, in a batch with rows of no sequence."""
+    from test_gpu_chunk_attention import _case
+    torch = _torch()
+    n = [(0, 1, 1, 2, 5)[i % 5] if i % 400 else 90 for i in range(1500)]
+    held = [(7 * i) % 70 if i % 311 else 700 for i in range(1500)]
+    q, k, v, table, lens, cu, kv = _case(8, n, held, 4, 2, 64, 16)
+    q = torch.cat((q, q[:9]))
+    out = torch.full_like(q, LEFT).to(cuda)
+    mcv.paged_attention_chunk(*(x.to(cuda) for x in (q, k, v, table, lens, cu)), out=out)
+    _close(out[:sum(n)], _ref(q[:sum(n)], kv, n, lens.tolist(), 64 ** -0.5))
+    assert (out[sum(n):] == LEFT).all()
+
+
 def test_one_size_a_stream(mcv, cuda):
     torch = _torch()
     side = torch.cuda.Stream()
