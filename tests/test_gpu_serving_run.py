@@ -134,6 +134,34 @@ def test_its_counters_end_at_zero(mcv, cuda):
     assert held and all((ws[:mcv.mixers._CHUNK_COUNTER_BYTES] == 0).all() for ws in held)
 
 
+def test_given_a_workspace_of_its_own(mcv, cuda):
+    """Through the C interface: none (nothing is cut), the bytes it asks for and not one more, and those of a larger call."""
+    torch = _torch()
+    lib, stream = mcv.lib(), torch.cuda.current_stream().cuda_stream
+    for a in _several(cuda):
+        q, k, v, table, lens, cu = a
+        (T, Hq, D), (pages, page, Hkv, _), (B, width) = q.shape, k.shape, table.shape
+        want = mcv.paged_attention_chunk(*a)
+        least = lib.mcv_paged_attention_chunk_workspace_bytes(B, T, Hq, Hkv, D, width * page)
+        most = lib.mcv_paged_attention_chunk_workspace_bytes(B, 9 * T, Hq, Hkv, D, 1 << 20)
+        assert most >= least
+        for nbytes in (0, least, most):
+            ws = torch.zeros(max(nbytes, 256) + 4096, dtype=torch.uint8, device=cuda)
+            ws[nbytes:] = 91
+            for _ in range(2):
+                out = torch.full_like(q, LEFT)
+                rc = lib.mcv_paged_attention_chunk(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], pages,
+                                                   page, table.data_ptr(), table.stride(0), width, lens.data_ptr(), width * page, cu.data_ptr(), B, T, Hq, Hkv,
+                                                   D, D ** -0.5, out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, stream)
+                assert rc == 0
+                torch.cuda.synchronize()
+                # cut or not, a sum of the same weights in 32 bits, rounded once: at most a step of fp16 apart
+                assert ((out.float() - want.float()).abs() <= 2.0 ** -9 * want.float().abs() + 2.0 ** -9).all()
+                if nbytes:
+                    assert (out == want).all()
+            assert (ws[nbytes:] == 91).all() and (ws[:min(nbytes, 8192)] == 0).all()
+
+
 @pytest.mark.parametrize("B", [1, 3, 64, 65, 700])
 def test_offsets_that_fall(mcv, cuda, B):
     """Rows would have two sequences: none is written, and the next call finds the workspace as it was."""
