@@ -42,7 +42,7 @@ namespace mcv {
 namespace {
 
 constexpr int kTile = 64;                        // a part has whole ones of so many tokens
-constexpr int kLeast = 2 * kTile;                // tokens of a part, at least
+constexpr int kLeast = 2 * kTile;                // tokens of a part, at least, but for few tiles
 constexpr int kNearLog2 = 2;                     // 1 << kNearLog2 units side by side on one XCD
 constexpr int64_t kMaxLen = int64_t(1) << 30;    // tokens of one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -879,8 +879,10 @@ int choose_slots_log2(int64_t most, int64_t D) { return most <= 2 * kLeast ? -1 
 // more parts than the last of them joins, and no launch follows for those that are. Measured with a quarter and with kLeast, us:
 // 1100 new tokens, heads 8/2 of 256 (70 tiles) 31.2, 37.0; 2048 47.6, 54.1; 3000 70.0, 78.3; 16 x 32 over 1000, heads 32/8 of
 // 128 (128 tiles) 15.1, 18.8. Otherwise 300 over 800 (20 tiles) 30.0, 25.2; 16 x 32 over 2000 (32 tiles) 30.7, 22.6; 1000 over
-// 3000 (64 tiles) 61.2, 57.3.
-int choose_least(int64_t most, int64_t tiles) {
+// 3000 (64 tiles) 61.2, 57.3. A few tiles of 256, whose tokens take longest, are cut down to kTile: 24 over 1100 (2 tiles) 15.4
+// us, 16.8 with kLeast; 2 x 16 over 700 (4) 13.7, 19.5; otherwise 8 over 4000 18.1, 17.0, 8 x 4 over 500 (16 tiles) 16.5, 14.6.
+int choose_least(int64_t most, int64_t tiles, int64_t D) {
+    if (D == 256 && tiles <= 8 && most <= 2048) return kTile;
     if (tiles < 40 || most > std::min<int64_t>(50 * tiles, 4096)) return kLeast;
     return static_cast<int>(std::max<int64_t>(ceil_div(most, kFan * kTile) * kTile, kLeast));
 }
@@ -932,7 +934,7 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     if (slots_log2 >= 0 && (!workspace || workspace_bytes < split_bytes(slots_log2, slot_bytes))) slots_log2 = -1;
     if (slots_log2 >= 0 && reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return fail(MCV_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", who);
-    const int least = choose_least(most, tiles * Hkv);
+    const int least = choose_least(most, tiles * Hkv, D);
     const int64_t slots = slots_log2 < 0 ? 0 : int64_t(1) << slots_log2;
     if (tiles * Hkv + slots > 0x7fffff00) return fail(MCV_ERR_SHAPE, "%s: too many rows B=%lld T=%lld Hq=%lld", who, (long long)B, (long long)T, (long long)Hq);
     const uint32_t page16 = static_cast<uint32_t>(page_size / 16);
