@@ -24,10 +24,10 @@
 //
 // What bounds it, heads 8/2 of 256. 8192 new tokens 286 to 303 us by the card's clock, 0.91 to 0.96 PFLOP/s (a large matrix
 // product 1.14 to 1.31): the matrix cores are busy in 51% of cycles, LDS in 28%, and the clock falls to 1.7 GHz; what is left
-// is the softmax between the products, which two waves a SIMD hide by half. 512 over 100000 415 to 450 us, the same. 32
-// sequences' 5 over up to 9000 46.5 us, 3.1 TB/s: 33 of them at the cache's 145 MB, then the join. Small calls are latencies:
-// 24 over 1100 16.1 us, 1100 over none 27.6: the lengths, the table and the first tile, three loads that wait for one another,
-// 4 us; 1.3 us a step of 32 tokens; a part written and read 2 and 4 us.
+// is the softmax between the products, which two waves a SIMD hide by half. 512 over 100000 415 to 450 us: 61% at 1.5 GHz, the
+// copies cost a fifth of it. 32 sequences' 5 over up to 9000 46.3 us, 3.1 TB/s: 33 of them at the cache's 145 MB, then the
+// join. Small calls are latencies: 24 over 1100 15.4 us, 1100 over none 27.6: the lengths, the table and the first tile, three
+// loads that wait for one another, 4 us; 1.3 us a step of 32 tokens; a part written and read 2 and 4 us.
 //
 // Tried and not better: 64 rows a wave (halves what LDS reads; registers spill), two waves on the same rows, 64 tokens of 256 at
 // a time with one workgroup a CU (8192: 394 us), 256 rows and one workgroup a CU (1% better here, 10% worse for mixed lengths), copies spread over the products
