@@ -127,3 +127,12 @@ def test_workspace_bytes(mcv):
         assert 0 < size(8, T, 8, 2, 256, length) <= most
     for bad in ((0, 5, 8, 2, 256, 999), (1, 0, 8, 2, 256, 999), (1, 5, 8, 3, 256, 999), (1, 5, 8, 2, 0, 999), (1, 5, 8, 2, 256, -1), (1, 2 ** 30, 8, 2, 256, 999)):
         assert size(*bad) == 0
+
+
+def test_python_keeps_enough_for_every_call(mcv):
+    size = mcv.lib().mcv_paged_attention_chunk_workspace_bytes
+    for D in (64, 128, 256):
+        for Hq, Hkv in ((8, 2), (1, 1), (500, 1)):
+            for T in (1, 3, 128, 100000):
+                for length in (0, 256, 257, 2048, 1 << 30, 1 << 40):
+                    assert size(1, T, Hq, Hkv, D, length) <= mcv.mixers.CHUNK_WORKSPACE_BYTES
