@@ -93,6 +93,10 @@ void w8a8_quantize(const Tensor& x, Tensor& x_int8, Tensor& x_scale, hipStream_t
 // may be null when nothing else reads the fp16 row.
 void rms_norm_w8a8_quantize(const Tensor& x, const Tensor& gamma, double epsilon, Tensor* normed, Tensor& x_int8,
                             Tensor& x_scale, hipStream_t stream);
+// The same of the row residual_out = x + residual (fp16), which may be either of them.
+void rms_norm_add_w8a8_quantize(const Tensor& x, const Tensor& residual, const Tensor& gamma, double epsilon,
+                                Tensor* normed, Tensor& x_int8, Tensor& x_scale, Tensor& residual_out,
+                                hipStream_t stream);
 
 // Up to four W4A16 projections of the same x [M, K] in one launch (q/k/v,
 // decoder_layer.cpp:970-972; qkv and z, :1108-1110).  outs[i] is fp16 [M, N_i].
@@ -147,5 +151,9 @@ void matmul_b_transposed(const Tensor& a, const Tensor& b, Tensor& out, hipStrea
 
 // y = fp16(x / sqrt(mean(x^2) + eps) * gamma) per row, fp32 in between.
 void rms_norm(const Tensor& x, const Tensor& gamma, Tensor& out, double epsilon, hipStream_t stream);
+// residual_out = x + residual (fp16; may be either of them), out = rms_norm(residual_out), in one
+// launch and to the bit what the two would give.
+void rms_norm_add(const Tensor& x, const Tensor& residual, const Tensor& gamma, Tensor& out, Tensor& residual_out,
+                  double epsilon, hipStream_t stream);
 
 }  // namespace minicpmv

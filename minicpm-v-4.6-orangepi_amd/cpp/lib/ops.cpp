@@ -260,6 +260,32 @@ void rms_norm_w8a8_quantize(const Tensor& x, const Tensor& gamma, double epsilon
               "rms_norm_w8a8_quantize");
 }
 
+void rms_norm_add_w8a8_quantize(const Tensor& x, const Tensor& residual, const Tensor& gamma, double epsilon,
+                                Tensor* normed, Tensor& x_int8, Tensor& x_scale, Tensor& residual_out,
+                                hipStream_t stream) {
+    require(x.dtype() == DType::Float16 && residual.dtype() == DType::Float16 && gamma.dtype() == DType::Float16 &&
+                residual_out.dtype() == DType::Float16,
+            "rms_norm_add_w8a8_quantize needs fp16 x, residual, gamma, residual_out");
+    require(x.shape().size() == 2, "rms_norm_add_w8a8_quantize x must be [M, H]");
+    require(residual.shape() == x.shape() && residual_out.shape() == x.shape(),
+            "rms_norm_add_w8a8_quantize residual and residual_out must match x");
+    const int64_t M = x.shape()[0], H = x.shape()[1];
+    require(static_cast<int64_t>(gamma.numel()) == H, "rms_norm_add_w8a8_quantize gamma must be [H]");
+    require(!normed || (normed->dtype() == DType::Float16 && normed->shape() == x.shape()),
+            "rms_norm_add_w8a8_quantize normed must be fp16 [M, H]");
+    require(x_int8.dtype() == DType::Int8 && x_int8.shape() == x.shape(),
+            "rms_norm_add_w8a8_quantize x_int8 must be int8 [M, H]");
+    require(static_cast<int64_t>(x_scale.numel()) == M, "rms_norm_add_w8a8_quantize x_scale must be [M]");
+    const bool f32 = x_scale.dtype() == DType::Float32;
+    require(f32 || x_scale.dtype() == DType::Float16, "rms_norm_add_w8a8_quantize x_scale must be fp16 or fp32");
+    check_mcv(mcv_rms_norm_add_w8a8_quantize(x.data(), H, residual.data(), H, gamma.data(), M, H, epsilon,
+                                             residual_out.data(), H, normed ? normed->data() : nullptr,
+                                             static_cast<int8_t*>(x_int8.data()),
+                                             f32 ? static_cast<float*>(x_scale.data()) : nullptr,
+                                             f32 ? nullptr : x_scale.data(), stream),
+              "rms_norm_add_w8a8_quantize");
+}
+
 DecodeMlpW8A8 make_decode_mlp_w8a8(const W8A8QuantizedWeight& gate, const W8A8QuantizedWeight& up,
                                    const W8A8QuantizedWeight& down, bool f32_scales) {
     require(up.K == gate.K && up.N == gate.N, "decode MLP (W8A8) gate and up must have the same shape");
@@ -414,6 +440,19 @@ void rms_norm(const Tensor& x, const Tensor& gamma, Tensor& out, double epsilon,
     require(gamma.shape() == std::vector<int64_t>{H}, "rms_norm gamma must be [H]");
     check_mcv(mcv_rms_norm(x.data(), gamma.data(), static_cast<int64_t>(x.numel()) / H, H, epsilon, out.data(), stream),
               "rms_norm");
+}
+
+void rms_norm_add(const Tensor& x, const Tensor& residual, const Tensor& gamma, Tensor& out, Tensor& residual_out,
+                  double epsilon, hipStream_t stream) {
+    for (const Tensor* t : {&x, &residual, &gamma, static_cast<const Tensor*>(&out), static_cast<const Tensor*>(&residual_out)})
+        require(t->dtype() == DType::Float16, "rms_norm_add requires fp16 tensors");
+    require(!x.shape().empty() && residual.shape() == x.shape() && out.shape() == x.shape() && residual_out.shape() == x.shape(),
+            "rms_norm_add residual, out and residual_out must match x");
+    const int64_t H = x.shape().back();
+    require(gamma.shape() == std::vector<int64_t>{H}, "rms_norm_add gamma must be [H]");
+    check_mcv(mcv_rms_norm_add(x.data(), H, residual.data(), H, gamma.data(), static_cast<int64_t>(x.numel()) / H, H, epsilon,
+                               residual_out.data(), H, out.data(), stream),
+              "rms_norm_add");
 }
 
 // Row-major out[M, N] = a[M, K] . B.  In rocBLAS's column-major terms that is

@@ -14,13 +14,13 @@
 // what they have.
 //
 // K and V come to LDS by copies that pass no register, 32 tokens (heads of 256) or 64 at a time, in two buffers: the next
-// tile's are on their way while one is taken. Rows of LDS have their chunks in orders of their own, so that no read meets
-// another's bank (counted: none). Operands of the products are read three ahead.
+// tile's are on their way while one is taken. Rows of LDS have their chunks in orders of their own, so that reads meet
+// other banks (counted: conflicts in 0.7% of LDS cycles). Operands of the products are read three ahead.
 //
 // Parts. All reads of a call are cut evenly, on the device and from the lengths alone, into as many parts as workgroups that
 // the chip holds at once (two a CU); a unit is a tile's part. Up to four parts are joined by the last of them to arrive, more
-// by a launch that follows. Partial sums are 128 KiB a tile of 128 rows of 256, what 128 tokens of cache are: no part is
-// smaller than that.
+// by a launch that follows. Partial sums are 128 KiB a tile of 128 rows of 256, what 128 tokens of cache are: but for few tiles
+// no part is smaller than that.
 //
 // What bounds it, heads 8/2 of 256. 8192 new tokens 286 to 303 us by the card's clock, 0.91 to 0.96 PFLOP/s (a large matrix
 // product 1.14 to 1.31): the matrix cores are busy in 51% of cycles, LDS in 28%, and the clock falls to 1.7 GHz; what is left
