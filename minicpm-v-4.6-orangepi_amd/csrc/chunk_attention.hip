@@ -476,6 +476,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         };
         k_from = rows16(my_k, p.k_token);
         v_from = rows16(my_v, p.v_token);
+        asm volatile("s_nop 4" : "+s"(k_from), "+s"(v_from));     // from a readlane to a copy, whose operands the compiler does not watch
     };
     const uint32_t lr = static_cast<uint32_t>(lane) / RC, lc = static_cast<uint32_t>(lane) % RC;
     const uint32_t k_row = 2 * lr * p.k_token, v_row = 2 * lr * p.v_token, k_chunk = 16 * (lc ^ (lr & KM)), v_chunk = 16 * (lc ^ turn_of_v(lr));
