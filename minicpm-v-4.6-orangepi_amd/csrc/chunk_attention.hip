@@ -26,7 +26,7 @@
 // product 1.14 to 1.31): the matrix cores are busy in 51% of cycles, LDS in 28%, and the clock falls to 1.7 GHz; what is left
 // is the softmax between the products, which two waves a SIMD hide by half. 512 over 100000 415 to 450 us: 61% at 1.5 GHz, the
 // copies cost a fifth of it. 32 sequences' 5 over up to 9000 46.3 us, 3.1 TB/s: 33 of them at the cache's 145 MB, then the
-// join. Small calls are latencies: 24 over 1100 15.4 us, 1100 over none 27.6: the lengths, the table and the first tile, three
+// join. Small calls are latencies: 24 over 1100 14.6 us, 1100 over none 27.6: the lengths, the table and the first tile, three
 // loads that wait for one another, 4 us; 1.3 us a step of 32 tokens; a part written and read 2 and 4 us.
 //
 // Tried and not better: 64 rows a wave (halves what LDS reads; registers spill), two waves on the same rows, 64 tokens of 256 at
@@ -767,8 +767,8 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
 
 // ------------------------------------------------------------------- many parts' sum --
 // Of the tiles that are in more than kFan parts: a workgroup has 32 rows and 32 d, as their parts have them in a wave's
-// registers, each of its waves a quarter of the parts. Bound by the partial sums' bytes and by its own start: 4.3 us for 24 new
-// tokens over 1100 (2.4 MB), 17 for 512 over 100000 (67 MB, 4 TB/s), 5 where it finds nothing to do.
+// registers, each of its waves a quarter of the parts. Bound by the partial sums' bytes and by its own start: 4 us for 24 new
+// tokens over 1100 (3.5 MB), 17 for 512 over 100000 (67 MB, 4 TB/s), 5 where it finds nothing to do.
 template <int D, int R>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     constexpr int MB = D / 32;
@@ -785,7 +785,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     const int w0 = first_id<R>(p, at, tile, hk), per = (parts + 3) / 4, end = (quarter + 1) * per < parts ? (quarter + 1) * per : parts;
     float4_t sum[4] = {};
     float top = -INFINITY, l = 0.f;
-    constexpr int kBatch = 4;                    // loads of a batch go out together
+    constexpr int kBatch = 6;                    // parts whose loads go out together (24 over 1100, 18 parts: 14.6 us, 15.4 with four)
     for (int u0 = quarter * per; u0 < end; u0 += kBatch) {
         float4_t o[kBatch][4];
         float2 st[kBatch];
