@@ -196,12 +196,12 @@ int check_pages(const char* who, const PageArgs& a, int64_t page, int64_t width,
 // `items`, which a workgroup of 256 threads has `per` of in a pass. In place, what some workgroups read others may not write:
 // then the state has a launch of its own, unless one workgroup does it all, which is faster up to `alone` items (apart: up to
 // alone / 4). Append, us, one workgroup / several: 512 tokens apart 4.9, 4.5, in place 5.0, 7.6; 2048 7.3, 4.6, in place 7.5,
-// 7.8; 4096 in place 11.4, 7.8. Over 256 sequences a thread has several to add up, and workgroups are of 1024 threads: 4000
-// tokens of 1000 sequences apart 6.5, 7.6 with 256. Truncate, in place: 32 sequences 4.9, 6.7; 64 7.0, 6.6.
+// 7.8; 4096 in place 11.4, 7.8. Over 512 sequences a thread has several to add up, and workgroups are of 1024 threads: 4000
+// tokens of 1000 sequences apart 6.5, 7.6 with 256; 65536 of 300 5.9, 5.4. Truncate, in place: 32 sequences 4.9, 6.7; 64 7.0, 6.6.
 int launch_pages(const char* who, void (*fn)(PageArgs), PageArgs& a, int64_t items, int64_t per, int64_t alone, mcv_stream_t stream) {
     const bool in_place = a.lens_out == a.lens || a.lens_out == a.cu || a.count_out == a.count;
     const bool one = items <= (in_place ? alone : alone / 4);
-    const int threads = one || a.B > 256 ? kThreads : 256;
+    const int threads = one || a.B > 512 ? kThreads : 256;
     a.what = !one && in_place ? kPages : kPages | kState;
     hipLaunchKernelGGL(fn, dim3(one ? 1 : static_cast<unsigned>(std::min<int64_t>(ceil_div(items, per * (threads / 256)), 1024))), dim3(threads), 0,
                        static_cast<hipStream_t>(stream), a);
