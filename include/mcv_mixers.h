@@ -135,8 +135,10 @@ int mcv_paged_append(void* block_table, int64_t table_row, int64_t table_width, 
                      void* free_count_out, mcv_stream_t stream);
 /* The reverse: sequence b keeps its first keep[b] tokens (int32 [B], clamped to [0,
  * seq_lens[b]]; NULL: none), and the pages behind them go on top of the free list, sequence
- * by sequence.  Table entries stay.  seq_lens_out may be seq_lens or keep.  free_count_out above free_capacity: so many pages did
- * not fit and are lost (as when a page is given back twice). */
+ * by sequence.  Table entries stay.  A page that several sequences hold is given back by each
+ * of them that ends before it: what is shared is for the caller to keep.  seq_lens_out may be
+ * seq_lens or keep.  free_count_out above free_capacity: so many pages did not fit and are
+ * lost (as when a page is given back twice). */
 int mcv_paged_truncate(const void* block_table, int64_t table_row, int64_t table_width, const void* seq_lens,
                        const void* keep, int64_t B, int64_t page_size, void* free_pages, int64_t free_capacity,
                        const void* free_count, void* seq_lens_out, void* free_count_out, mcv_stream_t stream);
