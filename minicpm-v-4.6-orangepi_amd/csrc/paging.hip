@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(PageArgs p) {
             p.positions[i] = position;
         }
     if ((p.what & kState) && blockIdx.x == 0) {
-        if (p.what & kPages) __syncthreads();    // lens_out may be lens
+        __syncthreads();                         // all have read: lens_out may be lens, count_out count
         int given = upto[t];
         for (int b = b0; b < b1; ++b) {
             const Growth g = growth_of(p, b);
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void truncate_kernel(PageArgs p) {
         }
     }
     if ((p.what & kState) && blockIdx.x == 0) {
-        if (p.what & kPages) __syncthreads();    // lens_out may be lens
+        __syncthreads();                         // all have read: lens_out may be lens, count_out count
         for (int b = b0; b < b1; ++b) p.lens_out[b] = kept_by(p, b);
         if (t == 0) *p.count_out = static_cast<int32_t>(count + upto[kThreads]);
     }
