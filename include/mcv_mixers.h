@@ -94,8 +94,8 @@ int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
  *           [0, T]; rows of no sequence are left as they are.  NULL: T / B rows each
  *           (T % B == 0)
  * A row that sees nothing (seq_lens[b] < n, or its pages are not there) gives zeros.  An
- * infinity or NaN reaches the rows that see its token and no others; such rows are made
- * token by token, some hundred times slower.  The softmax is in 32 bits; its weights are
+ * infinity or NaN reaches the rows that see its token and no others; workgroups whose part of
+ * a cache holds one in V take that part twice.  The softmax is in 32 bits; its weights are
  * rounded to fp16, which leaves those below 2^-33 of a row's largest out.
  * Where the rows are few the cache is split over workgroups, whose parts meet in an order
  * that does not depend on who is last (deterministic): workspace of

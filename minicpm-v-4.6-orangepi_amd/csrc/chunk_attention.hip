@@ -316,58 +316,19 @@ __device__ __forceinline__ uint16_t* out_row(const ChunkArgs& p, const Place& at
     return p.out + (static_cast<int64_t>(at.s.first + token) * p.Hq + hk * p.group + row - token * p.group) * D;
 }
 
-// A row that is not finite, token by token, its d from d0 to d1: an infinity or NaN in V reaches the rows that see its token,
-// where on the matrix cores it reaches every row of its tile (zero weights times it are NaN).
-template <int D>
-__device__ __forceinline__ void slow_row(const ChunkArgs& p, const Place& at, int hk, int row, int d0, int d1) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63, token = token_of(p, row);
-    const uint16_t* from = p.q + static_cast<int64_t>(at.s.first + token) * p.q_row + static_cast<int64_t>(hk * p.group + row - token * p.group) * p.q_head + E * lane;
-    float q[E], sum[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = h2f(from[e]) * p.q_by, sum[e] = 0.f;
-    const int upto = at.s.len - at.s.n + token + 1;
-    float top = -INFINITY, tot = 0.f;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {       // the largest score; the weights
-        const float less = top == -INFINITY ? 0.f : top;
-        for (int t = 0; t < upto; t += 16) {
-            int page, first;
-            page_of(p, p.table + at.b * p.table_row, t / 16, upto, page, first);
-#pragma unroll 1
-            for (int x = 0; page >= 0 && x < 16 && t + x < upto; ++x) {
-                const uint16_t* k = p.k + hk * p.k_head + page * p.k_page + static_cast<int64_t>(first + x) * p.k_token + E * lane;
-                float dot = 0.f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) dot = fmaf(q[e], h2f(k[e]), dot);
-                const float s = wave_butterfly(dot, [](float a, float b) { return a + b; }) * p.scale_log2;
-                if (pass == 0) {
-                    top = fmaxf(top, s);
-                    continue;
-                }
-                const uint16_t* v = p.v + hk * p.v_head + page * p.v_page + static_cast<int64_t>(first + x) * p.v_token + E * lane;
-                const float w = exp2_of(s - less);
-                tot += w;
-#pragma unroll
-                for (int e = 0; e < E; ++e) sum[e] = fmaf(w, h2f(v[e]), sum[e]);
-            }
-        }
-    }
-    const float by = tot > 0.f ? 1.0f / tot : (tot == 0.f ? 0.f : tot);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (E * lane + e >= d0 && E * lane + e < d1) out_row(p, at, hk, row, D)[E * lane + e] = f2h(tot == 0.f ? 0.f : sum[e] * by);
-}
-
 __device__ __forceinline__ uint2 halves(const float4_t& v, float by) {
     const half2_t a = {static_cast<_Float16>(v[0] * by), static_cast<_Float16>(v[1] * by)}, b = {static_cast<_Float16>(v[2] * by), static_cast<_Float16>(v[3] * by)};
     return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
 }
 
 // ---------------------------------------------------------------------- a part --
-// W: waves, each with 32 rows. KT: tokens that are staged and taken at a time.
+// W: waves, each with 32 rows. KT: tokens that are staged and taken at a time. True, in every thread: V is not finite
+// somewhere, and the part has to be taken `again`. On the matrix cores such an element reaches every row of its tile, as zero
+// weights times it are NaN; the second time it is taken out of V, and its d's first token that has it is kept: the rows that see
+// that one get in the end what it makes of them. 8192 new tokens, heads 8/2 of 256: 287 us, with one infinity in the first page
+// 607, in every 16th token 717; 512 over 100000 487, 877, 1058.
 template <int D, int W, int KT>
-__global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p) {
+__device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool again, unsigned block, unsigned thread) {
     constexpr int R = 32 * W;                    // (token, head) rows of a workgroup
     constexpr int KS = D / 16;                   // steps of the score product
     constexpr int MB = D / 32;                   // blocks of 32 d
@@ -378,11 +339,10 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     constexpr int KM = RC < 16 ? RC - 1 : 15;
     constexpr int QL = D == 256 ? 3 : 0;         // of q's operands, those that lie in LDS: the registers are one or two short
     constexpr int kAhead = 3;                    // operands on their way from LDS while a product runs
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // [2][K, V][KT][D]
-    __shared__ int flag;
+    __shared__ int flag, odd_of[W], odd_from[2][D];
     constexpr int kThrough = 16;                 // accesses that all XCDs see
-    const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = thread & 63, c = lane & 31, j = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
 
     Place at;
     auto units = [&](const Seq& s, int S) {
@@ -392,7 +352,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         for (int i = whole + 1; i < parts; ++i) sum += tiles_with<R>(p, s, tiles, static_cast<int64_t>(i) * S);
         return sum * p.Hkv;
     };
-    if (!find<R>(p, unit_of(blockIdx.x), at, units)) return;
+    if (!find<R>(p, unit_of(block), at, units)) return false;
     const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
     // Part by part; in one, `near` tiles of a cache head after another, those that read most first.
     int part, tile, hk;
@@ -406,7 +366,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             i -= part * tiles * p.Hkv;
             for (;;) {
                 have = tiles_with<R>(p, at.s, tiles, static_cast<int64_t>(part) * at.S);
-                if (have == 0) return;           // (lengths that changed meanwhile)
+                if (have == 0) return false;           // (lengths that changed meanwhile)
                 if (i < have * p.Hkv) break;
                 i -= have * p.Hkv;
                 ++part;
@@ -497,7 +457,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         for (int i = 0; i < 2 * CP; ++i) copy(i);
         aim(t_begin + KT, 1);                    // (past the end: copies of nothing)
     }
-    half8_t q[KS - QL], *const q_held = reinterpret_cast<half8_t*>(lds + 4 * KT * ROW) + threadIdx.x;
+    half8_t q[KS - QL], *const q_held = reinterpret_cast<half8_t*>(lds + 4 * KT * ROW) + thread;
     if (mine) {
         if (p.q_by != 1.f)
 #pragma unroll
@@ -525,6 +485,10 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
     // Of a SIMD's two waves the one in the odd slot goes first: alike, they share the matrix cores and come to their softmaxes at
     // one time. 9 prompts of 1 to 1501 tokens, heads 32/8 of 128: 81.6 us, 86.9 without; with heads of 256 within 3% either way.
     if (D < 256 && (__builtin_amdgcn_s_getreg((3 << 11) | 4) & 1)) __builtin_amdgcn_s_setprio(2);
+    if (again) {
+        for (int i = threadIdx.x; i < 2 * D; i += 64 * W) odd_from[i / D][i % D] = 0x7fffffff;
+        __syncthreads();
+    }
     int buf = 0;
     for (int t = t_begin; t < t_end; t += KT, buf ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -532,11 +496,29 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         const uint32_t k_now = lds_at + buf * 2 * KT * ROW + k_at, v_now = lds_at + buf * 2 * KT * ROW + v_at;
         gone = gone_next;
         gone_next = gone_then;
-        if (t + KT > t_end || gone) {
+        if (t + KT > t_end || gone || again) {
             // what lies past the end or is not there may be NaN, whose product with a weight of zero is no zero
-            for (int i = lane; i < CR * RC; i += 64) {
+            int first = lane;                    // (opaque, as the chunk of a copy)
+            asm volatile("" : "+v"(first));
+#pragma unroll 1
+            for (int i = first; i < CR * RC; i += 64) {
                 const int r = CR * wave + i / RC;
-                if (t + r >= t_end || (gone >> (CR * wave / 16) & 1)) *reinterpret_cast<float4_t*>(vl + r * ROW + 16 * (i % RC)) = float4_t{0, 0, 0, 0};
+                uint4* const chunk = reinterpret_cast<uint4*>(vl + r * ROW + 16 * (i % RC));
+                if (t + r >= t_end || (gone >> (CR * wave / 16) & 1)) *chunk = make_uint4(0, 0, 0, 0);
+                else if (again) {
+                    uint4 v = *chunk;
+                    uint32_t* const w = &v.x;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t h = w[e / 2] >> (16 * (e % 2)) & 0xffff;
+                        if ((h & 0x7c00) != 0x7c00) continue;
+                        const int d = 8 * (i % RC ^ turn_of_v(r)) + e;
+                        if (h != 0xfc00) atomicMin(&odd_from[0][d], t + r);      // a NaN is both infinities
+                        if (h != 0x7c00) atomicMin(&odd_from[1][d], t + r);
+                        w[e / 2] &= e % 2 ? 0xffffu : 0xffff0000u;
+                    }
+                    *chunk = v;
+                }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
@@ -645,19 +627,25 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
             add(h, w, v);
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();                // K and V have been read, no copy is on its way
-    asm volatile("" ::: "memory");
-
-    // Up to four parts meet in the last of them to arrive; always (0 + 1) + (2 + 3), so that the bits do not depend on who is
-    // last: scaling by powers of two is exact, and a sum of two has one value.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no copy is on its way
+    if (again)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int d = 32 * b + 8 * (i / 4) + 4 * j + i % 4;
+                const bool up = odd_from[0][d] < seen, down = odd_from[1][d] < seen;
+                acc[b][i] = up ? down ? NAN : INFINITY : down ? -INFINITY : acc[b][i];
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+    int w0 = 0;
+    const int mine_at = wave * static_cast<int>(part_bytes(D)) + 16 * lane, stat_at = wave * static_cast<int>(part_bytes(D)) + 128 * D + 8 * lane;
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    auto slot = [&](int i) {                     // of nothing where there is no such part
+        return __builtin_amdgcn_make_buffer_rsrc(slot_of(p, w0, i), 0, i < parts ? static_cast<int>(p.slot_bytes) : 0, 0x00020000);
+    };
     if (parts > 1) {
-        const int w0 = first_id<R>(p, at, tile, hk);
-        const int mine_at = wave * static_cast<int>(part_bytes(D)) + 16 * lane, stat_at = wave * static_cast<int>(part_bytes(D)) + 128 * D + 8 * lane;
-        typedef unsigned u2 __attribute__((ext_vector_type(2)));
-        auto slot = [&](int i) {                 // of nothing where there is no such part
-            return __builtin_amdgcn_make_buffer_rsrc(slot_of(p, w0, i), 0, i < parts ? static_cast<int>(p.slot_bytes) : 0, 0x00020000);
-        };
+        w0 = first_id<R>(p, at, tile, hk);
         if (mine) {
             const auto to = slot(part);
 #pragma unroll
@@ -669,8 +657,32 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
                                                            to, mine_at + 1024 * (4 * b + i), 0, kThrough);
             __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(m), __float_as_uint(l)}, to, stat_at, 0, kThrough);
         }
-        if (parts > kFan) return;
-        if (!last_in(reinterpret_cast<unsigned*>(p.ws) + w0, parts, &flag) || !mine) return;
+    }
+    if (!again) {                                // while the part is on its way out, which another pass replaces
+        float4_t some = {};                      // (the sums' products two by two pass no 2^127: a sum is below 2^62)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) some[i / 2 % 4] = fmaf(acc[b][i], acc[b][i + 1], some[i / 2 % 4]);
+        const float none = (some[0] + some[1]) + (some[2] + some[3]);
+        const float sum = sum2(l);               // not finite itself: nor are the row's values, and rightly
+        odd_of[wave] = __any(mine && !(fabsf(none) < INFINITY) && fabsf(sum) < INFINITY);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                // K and V have been read
+    asm volatile("" ::: "memory");
+    if (!again) {
+        int odd = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) odd |= odd_of[w];
+        if (__builtin_amdgcn_readfirstlane(odd)) return true;
+    }
+
+    // Up to four parts meet in the last of them to arrive; always (0 + 1) + (2 + 3), so that the bits do not depend on who is
+    // last: scaling by powers of two is exact, and a sum of two has one value.
+    if (parts > 1) {
+        if (parts > kFan) return false;
+        if (!last_in(reinterpret_cast<unsigned*>(p.ws) + w0, parts, &flag) || !mine) return false;
         const int others = (part ^ 2) & ~1, with[3] = {part ^ 1, others, others + 1};
         __amdgpu_buffer_rsrc_t from[3];
         float om[3], ol[3], by[3], top = m;
@@ -710,17 +722,15 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
                             (__int_as_float(now[1][i / 4][i % 4]) * by[1] + __int_as_float(now[2][i / 4][i % 4]) * by[2]);
         }
     }
-    if (!mine) return;
+    if (!mine) return false;
 
     l = sum2(l);
     // acc[b][i]: d = 32 b + 8 (i / 4) + 4 j + i % 4 of this lane's row
-    float none = 0.f * l;                        // NaN where anything is not finite
+    if (__any(l == 0.f))                         // no weight but zeros: nothing, whatever V holds
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
+        for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) none = fmaf(acc[b][i], 0.f, none);
-    const unsigned long long odds = __ballot(none != 0.f);
-    const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
+            for (int i = 0; i < 16; ++i) acc[b][i] = l == 0.f ? 0.f : acc[b][i];
     // Whole rows go out, turned in LDS, a wave in its own part of it: a row's 16-byte chunks in an order of its own, so that
     // what a lane has of its row meets other banks; and each row's place in `out`, worked out once by the lanes that have it.
     {
@@ -731,7 +741,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
         const float by = l > 0.f ? 1.0f / l : 0.f;
         const uint32_t mine_at = lds_at + wave * 64 * D, rows_at = lds_at + 64 * D * W + 256 * wave, to = mine_at + 16 * (c * CH + (c & CM)) + 8 * j;
         *reinterpret_cast<lds_uint64>(rows_at + 8 * c) =
-            wrow + c < rows && !(bad >> c & 1) ? reinterpret_cast<uintptr_t>(p.out + (static_cast<int64_t>(at.s.first + token) * p.Hq + hk * p.group + row - token * p.group) * D) : 0;
+            wrow + c < rows ? reinterpret_cast<uintptr_t>(p.out + (static_cast<int64_t>(at.s.first + token) * p.Hq + hk * p.group + row - token * p.group) * D) : 0;
 #pragma unroll
         for (int b = 0; b < MB; ++b)
 #pragma unroll
@@ -758,10 +768,21 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
                 if (place[x]) *reinterpret_cast<__attribute__((address_space(1))) uint4_v*>(place[x] + 16 * ch) = v[x];
         }
     }
+    return false;
+}
+
+template <int D, int W, int KT>
+__global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // [2][K, V][KT][D]; the last of q's operands
+    bool again = false;
 #pragma unroll 1
-    for (uint32_t left = bad; left; left &= left - 1) {
-        const int rr = wrow + __builtin_ctz(left);
-        if (rr < rows) slow_row<D>(p, at, hk, rr, 0, D);
+    for (;;) {
+        unsigned block = blockIdx.x, thread = threadIdx.x;
+        auto args = (const __attribute__((address_space(4))) ChunkArgs*)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(block), "+v"(thread), "+s"(args));    // (opaque: what is made from them would be kept for a second time, in registers that the loop needs)
+        p = *(const ChunkArgs*)args;
+        if (!take_part<D, W, KT>(p, lds, again, block, thread)) return;
+        again = true;
     }
 }
 
@@ -850,23 +871,11 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
         }
     }
     l = sum2(l);
-    float none = 0.f * l;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) none = fmaf(sum[i][e], 0.f, none);
-    const unsigned long long odds = __ballot(none != 0.f);
-    const uint32_t bad = static_cast<uint32_t>(odds) | static_cast<uint32_t>(odds >> 32);
-    if (wrow + c <= last_row && !(bad >> c & 1)) {
+    if (wrow + c <= last_row) {
         uint16_t* to = out_row(p, at, hk, wrow + c, D) + 32 * b + 4 * j;
         const float by = l > 0.f ? 1.0f / l : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(to + 8 * i) = halves(sum[i], by);
-    }
-#pragma unroll 1
-    for (uint32_t left = bad; left; left &= left - 1) {
-        const int rr = wrow + __builtin_ctz(left);
-        if (rr <= last_row) slow_row<D>(p, at, hk, rr, 32 * b, 32 * b + 32);
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(to + 8 * i) = halves(l == 0.f ? float4_t{0, 0, 0, 0} : sum[i], by);
     }
 }
 
