@@ -447,8 +447,11 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
         const int row = first_row + (of_v ? i - CP : i) * RPI;
         uint32_t chunk = of_v ? v_chunk : k_chunk;       // (opaque: what is made from it would be kept through the loop)
         asm volatile("" : "+v"(chunk));
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"            // (m0 is reserved: it is set anew wherever it is used, unless an older value is known to stand)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(copy_to + (of_v ? KT * ROW + (i - CP) * 1024 : i * 1024)),
                      "v"((chunk ^ (16 * (of_v ? turn_of_v(row) : row & KM))) + (of_v ? v_row : k_row)), "s"(of_v ? v_from : k_from), "s"(2 * row * (of_v ? p.v_token : p.k_token)) : "m0", "memory");
+#pragma clang diagnostic pop
     };
     if (t_begin < t_end) {
         aim(t_begin, 0);
