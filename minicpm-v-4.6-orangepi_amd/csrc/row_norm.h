@@ -1,6 +1,6 @@
 // row_norm.h -- RMSNorm of fp16 rows, alone (elementwise.hip) or followed by
 // the W8A8 activation quantisation (w8a8.hip), and either of them of the sum of two
-// rows; one 256-thread workgroup per row.
+// rows; one 256-thread workgroup per row, or a wave for short rows of a sum.
 #pragma once
 
 #include "common.h"
@@ -276,15 +276,16 @@ void launch_rms(const uint16_t* x, const uint16_t* gamma, int64_t M, int64_t H, 
                          static_cast<uintptr_t>(2 * (add.x_row | add.other_row | add.sum_row));
     const bool vec = H % 8 == 0 && at % 16 == 0;
     const int h = static_cast<int>(H);
-    if constexpr (ADD)
-        if (H <= 256) {
+    RmsFn fn = rms_row_kernel<0, false, QUANT, ADD>;
+    if (H <= 256) {
+        if constexpr (ADD) {
             hipLaunchKernelGGL(rms_add_short_kernel<QUANT>, dim3(static_cast<unsigned>(ceil_div(M, 4))), dim3(256), 0, stream, x, gamma, static_cast<int>(M), h, eps,
                                normed, xq, s32, s16, add);
             return;
+        } else {
+            fn = rms_row_kernel<1, false, QUANT>;
         }
-    RmsFn fn = rms_row_kernel<0, false, QUANT, ADD>;
-    if (H <= 256) fn = rms_row_kernel<1, false, QUANT, ADD>;
-    else if (H <= 1024) fn = vec ? rms_row_kernel<4, true, QUANT, ADD> : rms_row_kernel<4, false, QUANT, ADD>;
+    } else if (H <= 1024) fn = vec ? rms_row_kernel<4, true, QUANT, ADD> : rms_row_kernel<4, false, QUANT, ADD>;
     else if (H <= 2048) fn = vec ? rms_row_kernel<8, true, QUANT, ADD> : rms_row_kernel<8, false, QUANT, ADD>;
     else if (H <= 4096) fn = vec ? rms_row_kernel<16, true, QUANT, ADD> : rms_row_kernel<16, false, QUANT, ADD>;
     else if (H <= 8192) fn = vec ? rms_row_kernel<32, true, QUANT, ADD> : rms_row_kernel<32, false, QUANT, ADD>;
