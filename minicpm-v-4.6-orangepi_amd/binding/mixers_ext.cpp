@@ -333,6 +333,7 @@ PyObject* append(PyObject* const* a) {
     const at::Tensor *slots_given = maybe(who, "slots", a[9]), *positions_given = maybe(who, "positions", a[10]);
     const int64_t page = whole(a[3]), B = lens.numel();
     const int64_t T = a[4] != Py_None ? whole(a[4]) : slots_given ? slots_given->numel() : B;
+    if (cu && a[4] == Py_None && !slots_given) refuse("%s: cu_seqlens needs tokens, or the slots to write", who);
     if (T < 0) refuse("%s: tokens must not be negative (tokens=%lld)", who, (long long)T);
     ints(who, "seq_lens", lens, B);
     check_table(who, table, B);

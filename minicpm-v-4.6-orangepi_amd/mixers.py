@@ -146,7 +146,8 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
 def paged_append(block_table, seq_lens, cu_seqlens=None, page_size=16, *, tokens=None, free_pages=None, free_count=None,
                  seq_lens_out=None, free_count_out=None, slots=None, positions=None, stream=None):
     """Room in a paged cache for new tokens: sequence b, of seq_lens[b] tokens, gets the rows cu_seqlens[b] ..
-    cu_seqlens[b + 1] - 1 of a packed batch of `tokens` rows (None: the rows of `slots`, else one each) as its next.
+    cu_seqlens[b + 1] - 1 of a packed batch of `tokens` rows (None: the rows of `slots`; without cu_seqlens else one each) as
+    its next.
 
     Pages that a sequence lacks are taken from the top of the stack free_pages int32 [n], free_count int32 [1] and written
     into block_table int32 [B, width]; without free_pages the table is complete.  Returns (slots int64 [tokens], where
