@@ -128,7 +128,8 @@ int64_t mcv_paged_attention_chunk_workspace_bytes(int64_t B, int64_t T, int64_t 
  *   seq_lens_out  int32 [B]: lengths with the new tokens that have room (a table row
  *           is width * page_size tokens); may be seq_lens
  *   free_count_out  int32 [1]: pages left; below zero: so many were lacking, and the
- *           last sequences' last tokens have no room.  May be free_count */
+ *           last sequences' last tokens have no room.  May be free_count; NULL without
+ *           free_pages */
 int mcv_paged_append(void* block_table, int64_t table_row, int64_t table_width, const void* seq_lens,
                      const void* cu_seqlens, int64_t B, int64_t T, int64_t page_size, const void* free_pages,
                      int64_t free_capacity, const void* free_count, void* slots, void* positions, void* seq_lens_out,

@@ -340,6 +340,7 @@ PyObject* append(PyObject* const* a) {
     if (cu) ints(who, "cu_seqlens", *cu, B + 1);
     else if (B ? T % B != 0 : T != 0) refuse("%s: %lld rows for %lld sequences need cu_seqlens", who, (long long)T, (long long)B);
     if (!free != !count) refuse("%s: free_pages and free_count come together", who);
+    if (count_given && !free) refuse("%s: free_count_out without free_pages", who);
     if (free) ints(who, "free_pages", *free, free->numel()), ints(who, "free_count", *count, 1);
     if (lens_given) ints(who, "seq_lens_out", *lens_given, B);
     if (count_given) ints(who, "free_count_out", *count_given, 1);

@@ -225,6 +225,7 @@ int mcv_paged_append(void* block_table, int64_t table_row, int64_t table_width, 
     const char* who = "paged_append";
     if (!block_table || !seq_lens || !seq_lens_out || (T > 0 && (!slots || !positions)) || (free_pages && (!free_count || !free_count_out)))
         return fail(MCV_ERR_INVALID_ARG, "%s: null pointer", who);
+    if (!free_pages && free_count_out) return fail(MCV_ERR_INVALID_ARG, "%s: free_count_out without free_pages", who);
     if (T < 0 || T > 0x7fffffff || (!cu_seqlens && B > 0 && T % B != 0)) return fail(MCV_ERR_SHAPE, "%s: bad shape B=%lld T=%lld", who, (long long)B, (long long)T);
     PageArgs a{static_cast<int32_t*>(block_table), static_cast<const int32_t*>(seq_lens), static_cast<const int32_t*>(cu_seqlens),
                static_cast<int32_t*>(const_cast<void*>(free_pages)), static_cast<const int32_t*>(free_count), static_cast<int64_t*>(slots),
