@@ -437,6 +437,7 @@ void rms_norm(const Tensor& x, const Tensor& gamma, Tensor& out, double epsilon,
             "rms_norm requires fp16 tensors");
     require(!x.shape().empty() && out.shape() == x.shape(), "rms_norm out must match x");
     const int64_t H = x.shape().back();
+    require(H > 0, "rms_norm rows must not be empty");
     require(gamma.shape() == std::vector<int64_t>{H}, "rms_norm gamma must be [H]");
     check_mcv(mcv_rms_norm(x.data(), gamma.data(), static_cast<int64_t>(x.numel()) / H, H, epsilon, out.data(), stream),
               "rms_norm");
@@ -449,6 +450,7 @@ void rms_norm_add(const Tensor& x, const Tensor& residual, const Tensor& gamma, 
     require(!x.shape().empty() && residual.shape() == x.shape() && out.shape() == x.shape() && residual_out.shape() == x.shape(),
             "rms_norm_add residual, out and residual_out must match x");
     const int64_t H = x.shape().back();
+    require(H > 0, "rms_norm_add rows must not be empty");
     require(gamma.shape() == std::vector<int64_t>{H}, "rms_norm_add gamma must be [H]");
     check_mcv(mcv_rms_norm_add(x.data(), H, residual.data(), H, gamma.data(), static_cast<int64_t>(x.numel()) / H, H, epsilon,
                                residual_out.data(), H, out.data(), stream),
