@@ -88,7 +88,8 @@ int64_t mcv_paged_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
  * sequence b has the n = cu[b + 1] - cu[b] rows cu[b] .. of q, its last n tokens.
  * Its token i, at place seq_lens[b] - n + i, sees the tokens up to and with itself:
  *   out[row][h] = sum_t softmax_t(scale q[row][h] . K[t][h / (Hq / Hkv)]) V[t][..]
- *   q, out  fp16 [T][Hq][D] (q: row and head strides; out contiguous, apart from q)
+ *   q, out  fp16 [T][Hq][D] (q: row and head strides; out contiguous, apart from q, or
+ *           q itself where that is contiguous)
  *   caches, block_table, seq_lens, max_seq_len  as for mcv_paged_attention
  *   cu_seqlens  int32 [B + 1], ascending (else no row is written), values clamped to
  *           [0, T]; rows of no sequence are left as they are.  NULL: T / B rows each

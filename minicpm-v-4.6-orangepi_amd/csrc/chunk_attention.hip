@@ -900,6 +900,17 @@ int choose_least(int64_t most, int64_t tiles, int64_t D) {
     return static_cast<int>(std::max<int64_t>(ceil_div(most, kFan * kTile) * kTile, kLeast));
 }
 int64_t slot_bytes_of(int64_t T, int64_t group, int64_t D) { return ceil_div(std::min<int64_t>(kRows, T * group), 32) * part_bytes(D); }
+// A workgroup reads its rows of q before it writes them and nobody else's, so that out may be q; but no rows otherwise placed.
+bool meets(const void* q, int64_t row, int64_t head, const void* out, int64_t T, int64_t Hq, int64_t D) {
+    if (q == out && (T == 1 || row == Hq * D) && (Hq == 1 || head == D)) return false;
+    const int64_t begin = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(q)) / 2, end = begin + T * Hq * D;      // elements from q on
+    for (int64_t h = 0; h < Hq; ++h) {
+        const int64_t past = begin - D - h * head;       // the first token whose head ends behind out's first element
+        const int64_t t = past < 0 ? 0 : row > 0 ? past / row + 1 : T;
+        if (t < T && t * row + h * head < end) return true;
+    }
+    return false;
+}
 int64_t split_bytes(int slots_log2, int64_t slot_bytes) { return slots_log2 < 0 ? 0 : kCounterBytes + 2 * ((int64_t(1) << slots_log2) + 2) * slot_bytes; }
 
 }  // namespace
@@ -936,6 +947,7 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
         !chunked16(out, {}))
         return fail(MCV_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned, strides multiples of 8 elements", who);
     if (k_token > (1 << 25) || v_token > (1 << 25)) return fail(MCV_ERR_UNSUPPORTED, "%s: tokens of one page too far apart", who);
+    if (meets(q, q_row, q_head, out, T, Hq, D)) return fail(MCV_ERR_INVALID_ARG, "%s: out overlaps q without being it", who);
     int rc = require_device();
     if (rc != MCV_OK) return rc;
     // (width counted in pages first: width * page_size could pass 64 bits)

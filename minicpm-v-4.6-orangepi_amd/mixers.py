@@ -139,7 +139,7 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
     tokens among them) and max_seq_len as for paged_attention_decode.
 
     Prompts, their chunks and single tokens may share a call.  A row that sees nothing gives zeros, a row of no sequence is
-    left as it is, and so is all of `out` that no row writes.  Returns out fp16 [T, Hq, D]."""
+    left as it is, and so is all of `out` that no row writes.  `out` may be a contiguous q.  Returns out fp16 [T, Hq, D]."""
     return (_BINDING or binding()).chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, stream)
 
 
