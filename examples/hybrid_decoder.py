@@ -73,7 +73,7 @@ class Decoder:
         """Normed rows [T, H] of packed tokens at positions [3, T], which the sequences get as their next ones.
         cu: where the sequences' tokens begin; None: one token for each sequence in order."""
         T = len(tokens)
-        slots, _, _ = mcv.paged_append(self.table, self.lens, cu, PAGE, tokens=T, free_pages=self.free, free_count=self.free_count)
+        slots, places, _ = mcv.paged_append(self.table, self.lens, cu, PAGE, tokens=T, free_pages=self.free, free_count=self.free_count)
         x = self.embedding[tokens]
         h = mcv.rms_norm(x, self.layers[0].norm, EPS)
         for i, layer in enumerate(self.layers):
@@ -85,7 +85,7 @@ class Decoder:
                 if cu is None:
                     y = mcv.paged_attention_decode(q, kc, vc, self.table, self.lens)
                 else:
-                    y = mcv.paged_attention_chunk(q, kc, vc, self.table, self.lens, cu)
+                    y = mcv.paged_attention_chunk(q, kc, vc, self.table, self.lens, cu, positions=places)
             else:
                 qkv = torch.nn.functional.silu(qkv)
                 q, k, v = (t.view(T, -1, DL) for t in qkv.split((HK * DL, HK * DL, HV * DL), 1))

@@ -110,6 +110,17 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
                               int64_t table_row, int64_t table_width, const void* seq_lens, int64_t max_seq_len,
                               const void* cu_seqlens, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                               double scale, void* out, void* workspace, int64_t workspace_bytes, mcv_stream_t stream);
+/* The same with each sequence's new tokens at the places positions[cu[b]] on (int64 [T], which
+ * mcv_paged_append writes; the first of each sequence is read), whatever seq_lens[b] is: after an
+ * append without room for all tokens, whose lengths end where the room does, tokens that have
+ * room see what they should, and those that have none all seq_lens[b].  NULL: seq_lens[b] - n. */
+int mcv_paged_attention_chunk_at(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
+                                 int64_t k_token, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_token,
+                                 int64_t v_head, int64_t pages, int64_t page_size, const void* block_table,
+                                 int64_t table_row, int64_t table_width, const void* seq_lens, int64_t max_seq_len,
+                                 const void* cu_seqlens, const void* positions, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                 int64_t D, double scale, void* out, void* workspace, int64_t workspace_bytes,
+                                 mcv_stream_t stream);
 int64_t mcv_paged_attention_chunk_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                                   int64_t max_seq_len);
 

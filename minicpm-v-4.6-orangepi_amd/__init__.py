@@ -138,6 +138,9 @@ _SIGS = {
     "mcv_paged_attention_chunk": (_c_int, [_vp, _c_i64, _c_i64, *[_vp, _c_i64, _c_i64, _c_i64] * 2, _c_i64, _c_i64,
                                            _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, *[_c_i64] * 5, ctypes.c_double, _vp, _vp,
                                            _c_i64, _vp]),
+    "mcv_paged_attention_chunk_at": (_c_int, [_vp, _c_i64, _c_i64, *[_vp, _c_i64, _c_i64, _c_i64] * 2, _c_i64, _c_i64,
+                                              _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, *[_c_i64] * 5, ctypes.c_double, _vp, _vp,
+                                              _c_i64, _vp]),
     "mcv_paged_attention_chunk_workspace_bytes": (_c_i64, [_c_i64] * 6),
     "mcv_paged_append": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, *[_vp] * 6]),
     "mcv_paged_truncate": (_c_int, [_vp, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, *[_vp] * 4]),

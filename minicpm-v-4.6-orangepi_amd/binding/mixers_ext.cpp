@@ -288,12 +288,12 @@ int64_t whole(PyObject* o) {
     return v;
 }
 
-// (q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, stream) -> out
+// (q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, positions, stream) -> out
 PyObject* chunk(PyObject* const* a) {
     const char* who = "paged_attention_chunk";
     const at::Tensor &q = tensor(who, "q", a[0]), &kc = tensor(who, "k_cache", a[1]), &vc = tensor(who, "v_cache", a[2]);
     const at::Tensor &table = tensor(who, "block_table", a[3]), &lens = tensor(who, "seq_lens", a[4]);
-    const at::Tensor *cu = maybe(who, "cu_seqlens", a[5]), *given = maybe(who, "out", a[8]);
+    const at::Tensor *cu = maybe(who, "cu_seqlens", a[5]), *given = maybe(who, "out", a[8]), *positions = maybe(who, "positions", a[9]);
     if (q.dim() != 3 || kc.dim() != 4) refuse("%s: q must be [T, Hq, D] and the caches [pages, page_size, Hkv, D]", who);
     const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), pages = kc.size(0), page = kc.size(1), Hkv = kc.size(2), B = lens.numel();
     const Heads qa = heads(who, "q", q, T);
@@ -304,20 +304,22 @@ PyObject* chunk(PyObject* const* a) {
     else if (B ? T % B != 0 : T != 0) refuse("%s: %lld rows for %lld sequences need cu_seqlens", who, (long long)T, (long long)B);
     if (given && (given->scalar_type() != at::kHalf || given->sizes() != q.sizes() || !given->is_contiguous()))
         refuse("%s: out must be contiguous fp16 %s", who, shape(q).c_str());
-    same_device(who, q, {&kc, &vc, &table, &lens, cu, given});
+    if (positions && (positions->scalar_type() != at::kLong || !is_shape(*positions, {T}) || !positions->is_contiguous()))
+        refuse("%s: positions must be contiguous int64 [%lld]", who, (long long)T);
+    same_device(who, q, {&kc, &vc, &table, &lens, cu, given, positions});
     const int64_t most = a[7] == Py_None ? table.size(1) * page : whole(a[7]);
     const auto device = on_gpu(who, q);
-    const mcv_stream_t h = handle(a[9]);
-    const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q, a[9], h);
+    const mcv_stream_t h = handle(a[10]);
+    const at::Tensor out = given ? *given : fresh(q.sizes(), at::kHalf, q, a[10], h);
     if (B == 0 || T == 0) {                      // nothing to launch, of shapes that a batch would be taken of
         if (Hq == 0 || Hkv == 0 || Hq % Hkv != 0 || (D != 64 && D != 128 && D != 256) || page == 0 || page % 16 != 0)
             refuse("%s: bad shape q %s, caches %s", who, shape(q).c_str(), shape(kc).c_str());
         return wrapped(out);
     }
     const int64_t bytes = mcv_paged_attention_chunk_workspace_bytes(B, T, Hq, Hkv, D, most);
-    void* ws = bytes ? chunk_workspace(bytes, q, a[9], h) : nullptr;
-    check(mcv_paged_attention_chunk(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
-                                    table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), most, ptr(cu), B, T, Hq, Hkv, D,
+    void* ws = bytes ? chunk_workspace(bytes, q, a[10], h) : nullptr;
+    check(mcv_paged_attention_chunk_at(qa.p, qa.row, qa.head, ka.p, ka.page, ka.token, ka.head, va.p, va.page, va.token, va.head, pages, page,
+                                    table.data_ptr(), stride_of(table, 0), table.size(1), lens.data_ptr(), most, ptr(cu), ptr(positions), B, T, Hq, Hkv, D,
                                     number(a[6], 1.0 / std::sqrt(static_cast<double>(D))), out.data_ptr(), ws, ws ? bytes : 0, h),
           who);
     return wrapped(out);
@@ -518,7 +520,7 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F f) {
 
 PyObject* py_delta(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 15, [&] { return delta(a); }); }
 PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 9, [&] { return paged(a); }); }
-PyObject* py_chunk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 10, [&] { return chunk(a); }); }
+PyObject* py_chunk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 11, [&] { return chunk(a); }); }
 PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 12, [&] { return append(a); }); }
 PyObject* py_truncate(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 9, [&] { return truncate(a); }); }
 PyObject* py_norm_add(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 7, [&] { return norm_add(a, false); }); }

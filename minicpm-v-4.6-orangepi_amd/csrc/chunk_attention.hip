@@ -58,6 +58,7 @@ struct ChunkArgs {
     const int32_t* table;
     const int32_t* lens;
     const int32_t* cu;
+    const int32_t* positions;                    // int64 [T], or null
     uint16_t* out;
     uint8_t* ws;
     int64_t q_row, q_head, k_page, k_head, v_page, v_head, table_row;
@@ -92,10 +93,10 @@ __device__ __forceinline__ scalar_ints as_scalar(const int32_t* p) { return (sca
 
 // ---------------------------------------------------------------- who does what --
 struct Seq {
-    int first, n, len;                           // first new row, new tokens (below zero: cu_seqlens falls), tokens in the cache
+    int first, n, len, base;                     // first new row, new tokens (below zero: cu_seqlens falls), tokens in the cache, of them before the first new one
 };
 template <class Ints>
-__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b, Ints lens, Ints cu) {
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b, Ints lens, Ints cu, Ints positions) {
     const int at = b < p.B ? b : p.B - 1;        // (no branch: several are loaded at once)
     int first, next;
     const int held = lens[at];
@@ -104,14 +105,27 @@ __device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b, Ints lens, Ints
     auto inside = [](int v, int most) { return v < 0 ? 0 : v > most ? most : v; };
     first = inside(first, p.T);
     next = inside(next, p.T);
-    return {first, b < p.B ? next - first : 0, inside(held, p.max_len)};
+    Seq s{first, b < p.B ? next - first : 0, inside(held, p.max_len), 0};
+    s.base = s.len - s.n;
+    if (positions) {                             // (the first new token sees the last there is, at most)
+        const int64_t row = 2 * static_cast<int64_t>(first < p.T ? first : p.T - 1);
+        const int lo = positions[row], hi = positions[row + 1], most = s.len > 0 ? s.len - 1 : 0;
+        s.base = hi < 0 ? 0 : hi > 0 || static_cast<uint32_t>(lo) > static_cast<uint32_t>(most) ? most : lo;
+    }
+    return s;
 }
-__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b) { return seq_of(p, b, p.lens, p.cu); }
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& p, int b) { return seq_of(p, b, p.lens, p.cu, p.positions); }
 __device__ __forceinline__ int token_of(const ChunkArgs& p, int row) {         // row / group
     if (p.group == 1) return row;
     int t = static_cast<int>(__umulhi(static_cast<uint32_t>(row), p.group_inv));      // one too many at most
     if (t * static_cast<int64_t>(p.group) > row) --t;
     return t;
+}
+// Tokens that a new one sees.
+__device__ __forceinline__ int sees(const Seq& s, int token) {
+    if (token >= s.len - s.base) return s.len;
+    const int n = s.base + token + 1;
+    return n < 0 ? 0 : n;
 }
 // R: rows of a tile.
 template <int R>
@@ -121,13 +135,13 @@ __device__ __forceinline__ int tiles_of(const ChunkArgs& p, const Seq& s) {
 // Tokens that the first i tiles of rows read, at most (of one cache head).
 template <int R>
 __device__ __forceinline__ int64_t reads_below(const ChunkArgs& p, const Seq& s, int i) {
-    const int base = s.len > s.n ? s.len - s.n : 0, step = token_of(p, R + p.group - 1);
+    const int base = s.base > 0 ? s.base : 0, step = token_of(p, R + p.group - 1);
     return static_cast<int64_t>(i) * (base + kTile) + step * (static_cast<int64_t>(i) * (i + 1) / 2);
 }
 // Tiles of rows that have a part p > 0, which begins at token p S: the last ones.
 template <int R>
 __device__ __forceinline__ int tiles_with(const ChunkArgs& p, const Seq& s, int tiles, int64_t begin) {
-    const int64_t x = begin - (s.len - s.n);     // the first new token that sees it
+    const int64_t x = begin - s.base;            // the first new token that sees it
     return x <= 0 ? tiles : x >= s.n ? 0 : tiles - static_cast<int>(x * p.group / R);
 }
 
@@ -171,7 +185,7 @@ __device__ __forceinline__ bool search(const ChunkArgs& p, int me, Place& at, Co
     at.read = 0;
     at.b = 0;
     if (p.B == 1) {                              // (nothing to look for)
-        at.s = seq_of(p, 0, as_scalar(p.lens), as_scalar(p.cu));
+        at.s = seq_of(p, 0, as_scalar(p.lens), as_scalar(p.cu), as_scalar(p.positions));
         at.unit = me;
         at.S = part_of(reads(at.s));
         return me < count(at.s, at.S);
@@ -188,7 +202,8 @@ __device__ __forceinline__ bool search(const ChunkArgs& p, int me, Place& at, Co
         }
         at.b += l;
         if (!past) return false;
-        at.s = {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l)};
+        at.s = {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.len, l),
+                __builtin_amdgcn_readlane(s.base, l)};
         at.unit = me - before;
         return true;
     };
@@ -261,7 +276,7 @@ template <int R, class Count>
 __device__ __forceinline__ bool find(const ChunkArgs& p, int me, Place& at, Count count) {
     if (!__builtin_amdgcn_readfirstlane(search<R>(p, me, at, count))) return false;
     auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    at = {{one(at.s.first), one(at.s.n), one(at.s.len)}, one(at.b), one(at.unit), lane_of(at.read, 0), one(at.S)};
+    at = {{one(at.s.first), one(at.s.n), one(at.s.len), one(at.s.base)}, one(at.b), one(at.unit), lane_of(at.read, 0), one(at.S)};
     return true;
 }
 
@@ -346,14 +361,14 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
 
     Place at;
     auto units = [&](const Seq& s, int S) {
-        const int tiles = tiles_of<R>(p, s), base = s.len - s.n, parts = (s.len + S - 1) / S;
-        const int whole = base > 0 ? base / S : 0;
+        const int tiles = tiles_of<R>(p, s), parts = (s.len + S - 1) / S;
+        const int whole = s.base > 0 ? s.base / S : 0;
         int sum = tiles * (1 + whole);
         for (int i = whole + 1; i < parts; ++i) sum += tiles_with<R>(p, s, tiles, static_cast<int64_t>(i) * S);
         return sum * p.Hkv;
     };
     if (!find<R>(p, unit_of(block), at, units)) return false;
-    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
+    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.base;
     // Part by part; in one, `near` tiles of a cache head after another, those that read most first.
     int part, tile, hk;
     {
@@ -381,10 +396,7 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
     tile = __builtin_amdgcn_readfirstlane(tile);
     hk = __builtin_amdgcn_readfirstlane(hk);
     const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1;
-    auto seen_by = [&](int row) {                // tokens that a row sees
-        const int n = base + token_of(p, row) + 1;
-        return n < 0 ? 0 : n;
-    };
+    auto seen_by = [&](int row) { return sees(at.s, token_of(p, row)); };
     const int end = seen_by(last_row), parts = end <= at.S ? 1 : (end + at.S - 1) / at.S;
     const int t_begin = part * at.S, t_end = part < parts - 1 ? t_begin + at.S : end;
 
@@ -799,13 +811,13 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     Place at;
     auto many = [&](const Seq& s, int S) { return s.len > kFan * static_cast<int64_t>(S) ? tiles_with<R>(p, s, tiles_of<R>(p, s), kFan * static_cast<int64_t>(S)) * p.Hkv : 0; };
     if (!find<R>(p, blockIdx.x, at, many)) return;
-    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s), base = at.s.len - at.s.n;
+    const int rows = at.s.n * p.group, tiles = tiles_of<R>(p, at.s);
     const int hk = at.unit % p.Hkv, tile = tiles - 1 - at.unit / p.Hkv;
     const int lane = threadIdx.x & 63, c = lane & 31, j = lane >> 5, quarter = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = blockIdx.y / MB, b = blockIdx.y % MB;
     const int row0 = tile * R, last_row = (row0 + R < rows ? row0 + R : rows) - 1, wrow = row0 + 32 * wave;
     if (wrow > last_row) return;
-    const int parts = (base + token_of(p, last_row) + at.S) / at.S;      // ceil(what the last row sees / S)
+    const int parts = (sees(at.s, token_of(p, last_row)) + at.S - 1) / at.S;
     const int w0 = first_id<R>(p, at, tile, hk), per = (parts + 3) / 4, end = (quarter + 1) * per < parts ? (quarter + 1) * per : parts;
     float4_t sum[4] = {};
     float top = -INFINITY, l = 0.f;
@@ -931,6 +943,17 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
                               int64_t table_row, int64_t table_width, const void* seq_lens, int64_t max_seq_len,
                               const void* cu_seqlens, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, double scale,
                               void* out, void* workspace, int64_t workspace_bytes, mcv_stream_t stream) {
+    return mcv_paged_attention_chunk_at(q, q_row, q_head, k_cache, k_page, k_token, k_head, v_cache, v_page, v_token, v_head, pages, page_size,
+                                        block_table, table_row, table_width, seq_lens, max_seq_len, cu_seqlens, nullptr, B, T, Hq, Hkv, D, scale,
+                                        out, workspace, workspace_bytes, stream);
+}
+
+int mcv_paged_attention_chunk_at(const void* q, int64_t q_row, int64_t q_head, const void* k_cache, int64_t k_page,
+                                 int64_t k_token, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_token,
+                                 int64_t v_head, int64_t pages, int64_t page_size, const void* block_table,
+                                 int64_t table_row, int64_t table_width, const void* seq_lens, int64_t max_seq_len,
+                                 const void* cu_seqlens, const void* positions, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                 double scale, void* out, void* workspace, int64_t workspace_bytes, mcv_stream_t stream) {
     const char* who = "paged_attention_chunk";
     if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !out) return fail(MCV_ERR_INVALID_ARG, "%s: null pointer", who);
     if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || T > 0x7fffffff / Hq || B > 0x7fffffff / Hq || (!cu_seqlens && T % B != 0))
@@ -966,7 +989,7 @@ int mcv_paged_attention_chunk(const void* q, int64_t q_row, int64_t q_head, cons
     auto inverse = [](uint64_t n) { return n > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + n - 1) / n) : 0; };
     const ChunkArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache),
                       static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(seq_lens), static_cast<const int32_t*>(cu_seqlens),
-                      static_cast<uint16_t*>(out), static_cast<uint8_t*>(workspace), q_row, q_head, k_page, k_head, v_page, v_head, table_row,
+                      static_cast<const int32_t*>(positions), static_cast<uint16_t*>(out), static_cast<uint8_t*>(workspace), q_row, q_head, k_page, k_head, v_page, v_head, table_row,
                       static_cast<int>(k_token), static_cast<int>(v_token), static_cast<int>(pages), static_cast<int>(page16), static_cast<int>(most),
                       static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
                       inverse(page16), inverse(group), scale == 0.0 ? 1.f : std::fabs(static_cast<float>(scale) * kLog2e), scale < 0.0 ? -1.f : scale == 0.0 ? 0.f : 1.f,

@@ -132,15 +132,19 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale=
 
 
 def paged_attention_chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens=None, *, scale=None, max_seq_len=None,
-                          out=None, stream=None):
+                          out=None, positions=None, stream=None):
     """Attention of chunks of new tokens over a paged cache that holds them already (rotary_axes_cached): q fp16 [T, Hq, D],
     sequence b's rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device; None: T / B rows each) its last
     tokens.  Each sees the tokens of its sequence up to and with itself.  Caches, block_table, seq_lens int32 [B] (the new
     tokens among them) and max_seq_len as for paged_attention_decode.
 
+    positions int64 [T], paged_append's: each sequence's new tokens are at positions[cu_seqlens[b]] and on, in place of the
+    last ones of seq_lens[b]. So tokens that had room in an append without room for all see what they should; those that
+    had none see all of their sequence.
+
     Prompts, their chunks and single tokens may share a call.  A row that sees nothing gives zeros, a row of no sequence is
     left as it is, and so is all of `out` that no row writes.  `out` may be a contiguous q.  Returns out fp16 [T, Hq, D]."""
-    return (_BINDING or binding()).chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, stream)
+    return (_BINDING or binding()).chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, positions, stream)
 
 
 def paged_append(block_table, seq_lens, cu_seqlens=None, page_size=16, *, tokens=None, free_pages=None, free_count=None,

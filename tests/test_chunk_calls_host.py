@@ -1,4 +1,5 @@
-"""CPU tests of calls of paged_attention_chunk whose `out` lies on q's rows, and of those whose rows only lie around it."""
+"""CPU tests of calls of paged_attention_chunk whose `out` lies on q's rows, of those whose rows only lie around it, and of
+positions that are none."""
 import pytest
 
 from test_chunk_host import CHUNK, INVALID, NO_DEVICE, P, _call
@@ -42,3 +43,14 @@ def test_out_is_q(mcv, change):
     if torch.cuda.is_available():
         pytest.skip("would launch on addresses that are not memory")
     assert _call(mcv, "mcv_paged_attention_chunk", CHUNK, **change) == NO_DEVICE
+
+
+def test_positions_of_another_shape(mcv):
+    import torch
+    half, i32, i64 = (lambda *s, t=t: torch.zeros(*s, dtype=t) for t in (torch.float16, torch.int32, torch.int64))
+    args = dict(q=half(6, 8, 64), k_cache=half(5, 16, 2, 64), v_cache=half(5, 16, 2, 64), block_table=i32(2, 4), seq_lens=i32(2), cu_seqlens=i32(3))
+    for bad in (i32(6), i64(5), i64(6, 1), i64(12)[::2]):
+        with pytest.raises(mcv.McvError, match=r"^paged_attention_chunk: positions must be contiguous int64 \[6\]"):
+            mcv.paged_attention_chunk(**args, positions=bad)
+    with pytest.raises(mcv.McvError, match="tensors must be on a GPU"):
+        mcv.paged_attention_chunk(**args, positions=i64(6))
