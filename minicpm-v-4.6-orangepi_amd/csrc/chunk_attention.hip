@@ -34,6 +34,7 @@
 // (307), longest parts first (303), four reads ahead (the same), the tile after the next fetched into L2 (321), workgroups of the
 // join over several tiles (the same).
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "mixers.h"
@@ -987,12 +988,14 @@ int mcv_paged_attention_chunk_at(const void* q, int64_t q_row, int64_t q_head, c
     if (tiles * Hkv + slots > 0x7fffff00) return fail(MCV_ERR_SHAPE, "%s: too many rows B=%lld T=%lld Hq=%lld", who, (long long)B, (long long)T, (long long)Hq);
     const uint32_t page16 = static_cast<uint32_t>(page_size / 16);
     auto inverse = [](uint64_t n) { return n > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + n - 1) / n) : 0; };
+    // (A scale that 32 bits do not hold weighs all tokens alike, as the least that they do; the product with zero would not leave -inf what it is.)
+    const float scale_log2 = scale == 0.0 ? 1.f : std::max(std::fabs(static_cast<float>(scale) * kLog2e), FLT_MIN);
     const ChunkArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache),
                       static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(seq_lens), static_cast<const int32_t*>(cu_seqlens),
                       static_cast<const int32_t*>(positions), static_cast<uint16_t*>(out), static_cast<uint8_t*>(workspace), q_row, q_head, k_page, k_head, v_page, v_head, table_row,
                       static_cast<int>(k_token), static_cast<int>(v_token), static_cast<int>(pages), static_cast<int>(page16), static_cast<int>(most),
                       static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(group),
-                      inverse(page16), inverse(group), scale == 0.0 ? 1.f : std::fabs(static_cast<float>(scale) * kLog2e), scale < 0.0 ? -1.f : scale == 0.0 ? 0.f : 1.f,
+                      inverse(page16), inverse(group), scale_log2, scale < 0.0 ? -1.f : scale == 0.0 ? 0.f : 1.f,
                       slots_log2, least, slot_bytes};
     const auto s = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(ceil_div(tiles * Hkv + slots, 8 << kNearLog2) * (8 << kNearLog2)));
