@@ -438,11 +438,12 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
     uint32_t copy_to;
     // Groups of 16 tokens that are not there, of the tile that is being taken, of the one that is on its way and
     // of the one after it.
-    uint32_t gone = 0, gone_next = 0, gone_then = 0;
+    constexpr uint32_t kAgain = 1u << 31;        // (among them, as the loop has no register for it)
+    uint32_t gone = 0, gone_next = 0, gone_then = again ? kAgain : 0;
     auto aim = [&](int t, int buf) {
         copy_to = lds_at + buf * 2 * KT * ROW + wave * CR * ROW;
         const int g = (t - known) / 16, own = g + wave * CR / 16;
-        gone_then = static_cast<uint32_t>(__ballot(static_cast<int64_t>(my_k) < 0) >> g) & (KT == 64 ? 15u : 3u);
+        gone_then = (gone_then & kAgain) | (static_cast<uint32_t>(__ballot(static_cast<int64_t>(my_k) < 0) >> g) & (KT == 64 ? 15u : 3u));
         auto rows16 = [&](uint64_t at, int token_stride) {
             const int lo = __builtin_amdgcn_readlane(static_cast<int>(at), own), hi = __builtin_amdgcn_readlane(static_cast<int>(at >> 32), own);
             return int4_t{lo, hi & 0xffff, hi < 0 ? 0 : 2 * (15 * token_stride + D), 0x00020000};
@@ -512,7 +513,7 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
         const uint32_t k_now = lds_at + buf * 2 * KT * ROW + k_at, v_now = lds_at + buf * 2 * KT * ROW + v_at;
         gone = gone_next;
         gone_next = gone_then;
-        if (t + KT > t_end || gone || again) {
+        if (t + KT > t_end || gone) {
             // what lies past the end or is not there may be NaN, whose product with a weight of zero is no zero
             int first = lane;                    // (opaque, as the chunk of a copy)
             asm volatile("" : "+v"(first));
@@ -521,7 +522,7 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
                 const int r = CR * wave + i / RC;
                 uint4* const chunk = reinterpret_cast<uint4*>(vl + r * ROW + 16 * (i % RC));
                 if (t + r >= t_end || (gone >> (CR * wave / 16) & 1)) *chunk = make_uint4(0, 0, 0, 0);
-                else if (again) {
+                else if (gone & kAgain) {
                     uint4 v = *chunk;
                     uint32_t* const w = &v.x;
 #pragma unroll
