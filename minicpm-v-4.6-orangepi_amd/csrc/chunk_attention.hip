@@ -47,10 +47,11 @@ constexpr int kLeast = 2 * kTile;                // tokens of a part, at least, 
 constexpr int kNearLog2 = 2;                     // 1 << kNearLog2 units side by side on one XCD
 constexpr int64_t kMaxLen = int64_t(1) << 30;    // tokens of one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
-// A row's reference exponent m is a whole number, so that what it once stood for is brought to another by an exact product,
-// and is raised only when a score passes it by kRoom: the weights 2^(s - m + kTop) end at 2^15, below fp16's 65504, and the
-// row's largest begins above 2^8: those that are lost, below 2^-25, are less than 2^-33 of it.
-constexpr float kRoom = 6.f, kTop = 9.f;
+// A row's weights are 2^(s - m). m is a whole number, so that what it once stood for is brought to another by an exact product; it
+// begins kTop below a row's largest score and moves only when one passes it by kMost: the weights end at 2^15, below fp16's
+// 65504, and the row's largest begins above 2^8: those that are lost, below 2^-25, are less than 2^-33 of it. From kFar on,
+// where 32 bits end to hold every whole number, scores are rounded to 32 bits before m is taken from them, and m is the largest.
+constexpr float kMost = 15.f, kTop = 9.f, kFar = 8388608.f;
 
 struct ChunkArgs {
     const uint16_t* q;
@@ -581,19 +582,27 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
             float mx = s[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-            mx = max2(mx) * p.scale_log2;
-            if (__any(mx > m + (m == -INFINITY ? 0.f : kRoom))) {
-                const float to = fmaxf(m, ceilf(mx)), keep = m == -INFINITY ? 0.f : exp2_of(m - to);
+            mx = max2(mx);
+            if (__any(fmaf(mx, p.scale_log2, -m) > kMost || fabsf(m) >= kFar)) {
+                const float top = mx * p.scale_log2, to = fmaxf(m, fabsf(top) < kFar ? ceilf(top) - kTop : top), keep = m == -INFINITY ? 0.f : exp2_of(m - to);
                 m = to;
                 l *= keep;
 #pragma unroll
                 for (int b = 0; b < MB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[b][i] *= keep;
+                const bool far = fabsf(m) >= kFar && fabsf(m) < INFINITY;
+                if (__any(far)) {
+                    float by = p.scale_log2;     // (opaque: its reciprocal would be kept through the loop)
+                    asm volatile("" : "+s"(by));
+                    const float back = __builtin_amdgcn_rcpf(by);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = far ? (s[i] * p.scale_log2 - m) * back : s[i];
+                }
             }
         };
         auto weigh = [&](const float16_t& s, half8_t (&w)[2]) {
-            const float from = m == -INFINITY ? 0.f : m - kTop;
+            const float from = fabsf(m) < kFar ? m : 0.f;        // (-inf: nothing seen; past kFar: taken off already)
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
                 const half2_t e = {static_cast<_Float16>(exp2_of(fmaf(s[i], p.scale_log2, -from))),
