@@ -407,6 +407,7 @@ void check_rows(const char* who, const char* name, const at::Tensor& t, int64_t 
 PyObject* norm_add(PyObject* const* a, bool quantize) {
     const char* who = quantize ? "rms_norm_add_w8a8_quantize" : "rms_norm_add";
     const at::Tensor &x = tensor(who, "x", a[0]), &residual = tensor(who, "residual", a[1]), &gamma = tensor(who, "gamma", a[2]);
+    if (a[3] == Py_None) refuse("%s: eps must be a number", who);
     const double eps = number(a[3], 0.0);
     const at::Tensor* given = maybe(who, quantize ? "normed" : "out", a[4]);
     const at::Tensor* scale16 = quantize ? maybe(who, "x_scale_f16", a[6]) : nullptr;
