@@ -10,8 +10,8 @@
 // has 16 scores of one row, so that a row's maximum and sum are in two lanes and the weights, rounded, are where the second
 // product wants them: out^T += V^T w^T, V read from LDS transposed. Weights are fp16, the operand type of the matrix cores:
 // half a step of 2^-11 each, and the sum that divides them is of the rounded ones. Scores, maxima and sums are in 32 bits. The
-// reference that weights are taken against moves only when a score passes it by 2^6, a whole power of two: few rows ever scale
-// what they have.
+// reference that weights are taken against is a whole power of two and moves only when a row's largest grows past 2^6 times
+// what it was set for: few rows ever scale what they have.
 //
 // K and V come to LDS by copies that pass no register, 32 tokens (heads of 256) or 64 at a time, in two buffers: the next
 // tile's are on their way while one is taken. Rows of LDS have their chunks in orders of their own, so that reads meet
@@ -22,11 +22,11 @@
 // by a launch that follows. Partial sums are 128 KiB a tile of 128 rows of 256, what 128 tokens of cache are: but for few tiles
 // no part is smaller than that.
 //
-// What bounds it, heads 8/2 of 256. 8192 new tokens 286 to 303 us by the card's clock, 0.91 to 0.96 PFLOP/s (a large matrix
-// product 1.14 to 1.31): the matrix cores are busy in 51% of cycles, LDS in 28%, and the clock falls to 1.7 GHz; what is left
-// is the softmax between the products, which two waves a SIMD hide by half. 512 over 100000 415 to 450 us: 61% at 1.5 GHz, the
+// What bounds it, heads 8/2 of 256. 8192 new tokens 278 to 303 us by the card's clock, 0.91 to 0.99 PFLOP/s (a large matrix
+// product 1.14 to 1.31): the matrix cores are busy in 51 to 58% of cycles, LDS in 28 to 32%, and the clock falls to 1.7 GHz; what is left
+// is the softmax between the products, which two waves a SIMD hide by half. 512 over 100000 412 to 450 us: 61% at 1.5 GHz, the
 // copies cost a fifth of it. 32 sequences' 5 over up to 9000 46.3 us, 3.1 TB/s: 33 of them at the cache's 145 MB, then the
-// join. Small calls are latencies: 24 over 1100 14.6 us, 1100 over none 27.6: the lengths, the table and the first tile, three
+// join. Small calls are latencies: 24 over 1100 14.7 us, 1100 over none 27.5: the lengths, the table and the first tile, three
 // loads that wait for one another, 4 us; 1.3 us a step of 32 tokens; a part written and read 2 and 4 us.
 //
 // Tried and not better: 64 rows a wave (halves what LDS reads; registers spill), two waves on the same rows, 64 tokens of 256 at
@@ -815,7 +815,7 @@ __global__ __launch_bounds__(64 * W, 2) void chunk_attention_kernel(ChunkArgs p)
 // ------------------------------------------------------------------- many parts' sum --
 // Of the tiles that are in more than kFan parts: a workgroup has 32 rows and 32 d, as their parts have them in a wave's
 // registers, each of its waves a quarter of the parts. Bound by the partial sums' bytes and by its own start: 4 us for 24 new
-// tokens over 1100 (3.5 MB), 17 for 512 over 100000 (67 MB, 4 TB/s), 5 where it finds nothing to do.
+// tokens over 1100 (3.5 MB), 15 for 512 over 100000 (67 MB, 4.4 TB/s), 5 where it finds nothing to do.
 template <int D, int R>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs p) {
     constexpr int MB = D / 32;

@@ -68,6 +68,8 @@ struct AddRows {
 // thread t finds the elements t, t + 256, ... of the sum in LDS: bound by HBM from some
 // 1000 rows on.  M=8192 H=1024 12.3 us (5.4 TB/s; each element twice, as without ADD:
 // 19.2), M=1024 H=8192 11.3 (5.9 TB/s), M=1100 H=3592 to int8 9.8 (17), M=1 H=1024 2.0.
+// Not for PER = 0, whose thread writes the sum element by element and reads it back for
+// each pass: M=1024 H=16384 65 us (2.1 TB/s), without ADD 38.
 template <int PER, bool VEC, bool QUANT, bool ADD = false>
 __global__ __launch_bounds__(256) void rms_row_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ gamma,
                                                       int H, float eps, uint16_t* __restrict__ normed,

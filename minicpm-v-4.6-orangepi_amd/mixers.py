@@ -139,11 +139,12 @@ def paged_attention_chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens
     tokens among them) and max_seq_len as for paged_attention_decode.
 
     positions int64 [T], paged_append's: each sequence's new tokens are at positions[cu_seqlens[b]] and on, in place of the
-    last ones of seq_lens[b]. So tokens that had room in an append without room for all see what they should; those that
+    last ones of seq_lens[b].  So tokens that had room in an append without room for all see what they should; those that
     had none see all of their sequence.
 
     Prompts, their chunks and single tokens may share a call.  A row that sees nothing gives zeros, a row of no sequence is
-    left as it is, and so is all of `out` that no row writes.  `out` may be a contiguous q.  Returns out fp16 [T, Hq, D]."""
+    left as it is, and so is all of `out` that no row writes.  `out` may be a contiguous q.  The softmax's
+    weights are rounded to fp16 (paged_attention_decode keeps them in two parts).  Returns out fp16 [T, Hq, D]."""
     return (_BINDING or binding()).chunk(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_seq_len, out, positions, stream)
 
 
