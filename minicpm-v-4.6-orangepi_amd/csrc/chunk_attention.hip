@@ -383,7 +383,7 @@ __device__ __forceinline__ bool take_part(const ChunkArgs& p, uint8_t* lds, bool
             i -= part * tiles * p.Hkv;
             for (;;) {
                 have = tiles_with<R>(p, at.s, tiles, static_cast<int64_t>(part) * at.S);
-                if (have == 0) return false;           // (lengths that changed meanwhile)
+                if (have == 0) return false;     // (lengths that changed meanwhile)
                 if (i < have * p.Hkv) break;
                 i -= have * p.Hkv;
                 ++part;

@@ -99,6 +99,28 @@ def test_keys_and_values_together(mcv, cuda):
     assert got[:60].isfinite().all() and got[90:].isfinite().all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,held", [([40], [30]), ([300], [90]), ([700], [0]), ([3, 4], [3000, 5])])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_a_key_in_any_part(mcv, cuda, D, n, held, value):
+    """A score that is infinite or NaN makes its row NaN in all its d, in whichever part of the cache the key lies, and its
+    head's later rows; the other cache head's and earlier rows keep their bits."""
+    torch = _torch()
+    q, k, v, table, lens, cu, _ = _case(6, n, held, 8, 2, D, 16, sharp=0.1)
+    q = q.abs() + 0.01
+    a = [x.to(cuda) for x in (q, k, v, table, lens, cu)]
+    clean = mcv.paged_attention_chunk(*a).cpu()
+    for at in (0, (n[0] + held[0]) // 2, n[0] + held[0] - 2):
+        bad = k.clone()
+        bad[table[0, at // 16], at % 16, 1, 3] = value
+        a[1] = bad.to(cuda)
+        got = mcv.paged_attention_chunk(*a).cpu()
+        first = max(0, at - held[0])
+        assert got[first:n[0], 4:].isnan().all()
+        got[first:n[0], 4:] = clean[first:n[0], 4:]
+        assert (got == clean).all()
+
+
 def test_rows_of_no_weight(mcv, cuda):
     """All scores -inf: zeros, whatever V holds; a query that is not finite: its own rows only."""
     torch = _torch()
